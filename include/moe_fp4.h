@@ -54,7 +54,8 @@ int mfi_version(void);
  * a peer, 8 missing return from a peer), or invalid data (4 expert id out of
  * range, 5 expert region overflow: a repeated id or counters not zeroed,
  * 9 a received exchange block whose row count lies outside [0, capacity],
- * treated as empty).
+ * treated as empty, 11 a page id, length or row range of a 4-bit KV cache call
+ * outside the pool, table or rows, 12 a token slot past its pool).
  * The flag only reports: a set flag does not stop later calls.  Synchronous;
  * clear != 0 resets it.  Returns -1 if the flag cannot be read. */
 int mfi_device_error(int clear);
@@ -215,6 +216,63 @@ int mfi_attn_decode_batched(const void* q, const uint8_t* kvk, const uint8_t* kv
                             int M, int Hq, int Hkv, int D, int max_pos, const float* k_scale,
                             const float* v_scale, void* workspace, size_t workspace_bytes,
                             void* stream);
+
+/* ------------------------------------------------------------------------
+ * Paged 4-bit KV cache (no reference counterpart; head_dim D = 64 or 128).
+ *
+ * Keys and values are MXFP4: blocks of 32 elements of a head, E2M1 nibbles and
+ * one E8M0 code per block (exponent e = ceil(log2(max(amax / 6, 1e-30))), code
+ * e + 127; a block with a value that is not finite has code 255 and reads as
+ * NaN).  The pool is uint8 (num_pages, Hkv, page / 16, 17 D), 16-byte aligned;
+ * page, the tokens of a page, is a multiple of 16.  A tile of 17 D bytes holds
+ * 16 consecutive tokens of a head:
+ *   16 key rows of D/2 bytes | 16 value rows of D/2 bytes |
+ *   16 rows of D/32 key codes | 16 rows of D/32 value codes
+ * With nb = D/32 blocks, the key row has the 4-byte word t (elements 8t..8t+7,
+ * LSB-first) of block b at word t*nb + b, the value row the 2-byte piece h
+ * (elements 4h..4h+3) of block b at piece h*nb + b.  Token slot s of the pool
+ * is token s % page of page s / page.
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of a pool (0 for invalid sizes). */
+size_t mfi_kv4_pool_bytes(int num_pages, int page, int Hkv, int D);
+
+/* Quantise k, v (T, Hkv, D) of dtype MFI_* into the tokens slots[t] (device
+ * int64) of the pool.  Row and head strides in elements, any value; elements
+ * contiguous.  A negative slot skips its row, a slot past the pool too (device
+ * error 12).  Slots of one call must differ. */
+int mfi_kv4_write(const void* k, long long k_row, long long k_head, const void* v,
+                  long long v_row, long long v_head, int dtype, uint8_t* pool,
+                  const int64_t* slots, int T, int Hkv, int D, int page, int num_pages,
+                  void* stream);
+
+/* The tokens slots[t] as k, v (T, Hkv, D) of dtype MFI_*, contiguous and
+ * 16-byte aligned: the held values, rounded once.  A negative slot gives
+ * zeros, a slot past the pool too (device error 12). */
+int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, int dtype, int T,
+                 int Hkv, int D, int page, int num_pages, void* stream);
+
+/* Attention over the pool.  Sequence i of n_seq owns the query rows cu_q[i] ..
+ * cu_q[i+1] - 1 of q (T, Hq, D) (device int32; cu_q = NULL: rows i*max_q ..
+ * (i+1)*max_q - 1), at most max_q of them, and the first kv_lens[i] tokens of
+ * the pages table[i * table_ld + j], j < width.  Its rows are the last of its
+ * tokens: row r of R sees tokens 0 .. kv_lens[i] - R + r; one that sees none
+ * gets zeros.  out (T, Hq, D), contiguous, of q's type:
+ *   out = softmax(scale q k^T) v, query head h on KV head h / (Hq / Hkv).
+ * q: MFI_BF16 or MFI_F16, row and head strides in elements.  Rows of q that no
+ * sequence owns are not written.  Page ids outside [0, num_pages) are read as
+ * page 0, lengths cut to [0, width * page], sequences with a row range outside
+ * [0, T] or above max_q left out (device error 11).
+ * The workspace (256-byte aligned) is initialised once by
+ * mfi_kv4_attn_init_workspace; each call leaves it ready for the next.  Calls
+ * that overlap on the GPU need one each. */
+size_t mfi_kv4_attn_workspace_bytes(int n_seq, int Hq, int Hkv, int D, int max_q);
+int mfi_kv4_attn_init_workspace(void* workspace, size_t workspace_bytes, void* stream);
+int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long q_head, const uint8_t* pool,
+                 const int32_t* table, long long table_ld, const int32_t* kv_lens,
+                 const int32_t* cu_q, void* out, int T, int max_q, int n_seq, int Hq, int Hkv,
+                 int D, int page, int num_pages, int width, float scale, void* workspace,
+                 size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * Fused device-routed MoE layer (no reference counterpart as a single call:

@@ -79,6 +79,13 @@ SIGNATURES = {
     "mfi_ep_experts_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "mfi_ep_experts_return": (_I, [_VP, _I, _I, _I, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "mfi_ep_unpack_wait": (_I, [_I, _I, _I, _I, _VP, _VP, _VP, _VP, _VP]),
+    "mfi_kv4_pool_bytes": (_SZ, [_I, _I, _I, _I]),
+    "mfi_kv4_write": (_I, [_VP, _LL, _LL, _VP, _LL, _LL, _I, _VP, _VP, _I, _I, _I, _I, _I, _VP]),
+    "mfi_kv4_read": (_I, [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP]),
+    "mfi_kv4_attn_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "mfi_kv4_attn_init_workspace": (_I, [_VP, _SZ, _VP]),
+    "mfi_kv4_attn": (_I, [_VP, _I, _LL, _LL, _VP, _VP, _LL, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I,
+                          _I, _I, _I, ctypes.c_float, _VP, _SZ, _VP]),
 }
 
 MFI_F32, MFI_F16, MFI_BF16 = 0, 1, 2
@@ -117,6 +124,9 @@ DEVICE_ERRORS = {
     7: "a peer rank's dispatch did not arrive in time",
     8: "a peer rank's return did not arrive in time",
     9: "a received exchange block's row count was outside [0, capacity] (treated as empty)",
+    11: "a page id, length or row range of a 4-bit KV cache call lay outside the pool, the page "
+        "table or the query rows",
+    12: "a token slot lay past the pool of a 4-bit KV cache",
 }
 
 # MFI_CHECK_DEVICE=1: every checked call synchronises the device and raises
