@@ -257,7 +257,7 @@ int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, in
  * (i+1)*max_q - 1), at most max_q of them, and the first kv_lens[i] tokens of
  * the pages table[i * table_ld + j], j < width.  Its rows are the last of its
  * tokens: row r of R sees tokens 0 .. kv_lens[i] - R + r; one that sees none
- * gets zeros.  out (T, Hq, D), contiguous, of q's type:
+ * gets zeros.  out (T, Hq, D), contiguous, 16-byte aligned, of q's type:
  *   out = softmax(scale q k^T) v, query head h on KV head h / (Hq / Hkv).
  * q: MFI_BF16 or MFI_F16, row and head strides in elements.  Rows of q that no
  * sequence owns are not written.  Page ids outside [0, num_pages) are read as

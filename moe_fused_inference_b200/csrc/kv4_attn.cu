@@ -9,6 +9,8 @@
 
 #include "../../include/moe_fp4.h"
 #include "kv4.cuh"
+#include "tc_ptx.cuh"
+#include "tmap.cuh"
 #include "work.cuh"
 
 namespace mfi {
@@ -27,6 +29,8 @@ struct AttnArgs {
   const int* cu_q;           // (n_seq + 1) or null: max_q rows each
   void* out;                 // (T, Hq, D)
   int* err;
+  unsigned* counters;        // one per CTA, zero between calls
+  float* part;               // two slots per CTA
   int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
   float scale;
 };
@@ -53,91 +57,649 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
   return s;
 }
 
-__device__ __forceinline__ const uint8_t* tile_at(const AttnArgs& a, int seq, int head, int pos,
-                                                  int D) {
-  const int p = pos / a.page, in = pos - p * a.page;
-  int id = a.table[seq * a.table_ld + p];
-  if (id < 0 || id >= a.num_pages) {
-    kv4::report(a.err, kv4::kErrPage);
-    id = 0;
+// ---- few rows: vectors of a group on the legacy tensor path --------------------
+// A vector is one row of one query head; the R G vectors of a sequence and KV
+// head (v = r G + h) are taken 8 kNT at a time (a "set").  The work is the list
+// of all (sequence, KV head, set, tile of 16 tokens), in that order; CTA c takes
+// the c-th of `ctas` equal shares, whatever the sequences' lengths, and splits
+// each piece (sequence, head, set) of its share over its warps.
+//
+// Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
+//   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
+//   the blocks joined by their codes: s = sum_b 2^(c_b - 127) S_b
+//   O^T (D x 8 vectors) += V_b^T . P_b,  P_b = p 2^(c_b - 127)
+// The E2M1 values are exact in fp16 and never multiplied by a scale (the codes
+// go to the few scores and weights), and the query rows are scaled by a power of
+// two to a maximum in [2^14, 2^15), which keeps all bits of a bf16 or fp16 row
+// down to 2^-39 of its maximum.  P_b is rounded to fp16 (2^-12) after a factor
+// 2^(14 - top), top the largest value code so far: it keeps all its bits down to
+// 2^-28 and vanishes below 2^-39 of the largest weight times the largest scale.
+// As top is a whole power of two it changes no other bit of P_b.
+constexpr int kChunk = 2;    // tiles of a pipeline stage
+constexpr int kStages = 3;
+constexpr int kCtas = 148;   // one per SM
+
+template <int D, int kNT>
+struct Few {
+  static constexpr int kWarps = kNT == 1 ? 16 : 8;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kVec = 8 * kNT;
+  static constexpr int kStageBytes = kChunk * kv4::tile_bytes(D);
+  static constexpr int kAcc = D + 4;                          // floats of a vector's sum: D, max, sum, pad
+  static constexpr int kRing = kStages * kStageBytes;
+  static constexpr int kMerge = kVec * kAcc * 4;
+  static constexpr int kWarpBytes = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
+  static constexpr int kSmem = kWarps * kWarpBytes;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The four bytes of w, each two E2M1 values, to fp16x2 (low nibble: low half).
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
+}
+// E8M0 codes (nb bytes) to fp32; 255 gives NaN.
+template <int nb>
+__device__ __forceinline__ void codes(uint32_t w, float (&f)[nb]) {
+#pragma unroll
+  for (int i = 0; i < nb / 2; ++i) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(uint16_t(i ? w >> 16 : w)));
+    f[2 * i] = __uint_as_float(r << 16);
+    f[2 * i + 1] = __uint_as_float(r & 0xFFFF0000u);
   }
-  return a.pool + ((long long)id * a.Hkv + head) * kv4::head_bytes(D, a.page) +
-         (long long)(in / kv4::kTile) * kv4::tile_bytes(D);
+}
+// The larger of m (two 16-bit halves) and the nb codes of w plus one; a code of
+// 255 (NaN) counts as 0 (two such neighbours may carry one too many).
+template <int nb>
+__device__ __forceinline__ uint32_t more_codes(uint32_t m, uint32_t w) {
+  if (nb == 2) return __vmaxu2(m, ((w & 0xFFu) | ((w << 8) & 0x00FF0000u)) + 0x00010001u & 0x00FF00FFu);
+  m = __vmaxu2(m, (w + 0x00010001u) & 0x00FF00FFu);
+  return __vmaxu2(m, ((w >> 8) + 0x00010001u) & 0x00FF00FFu);
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// One warp per (sequence, row, query head); lane = token for the scores, lane
-// = D/32 elements for the sum.
-template <class E, int D>
-__global__ void __launch_bounds__(128) kv4_attn_kernel(AttnArgs a) {
+template <class E>
+__device__ __forceinline__ void q8(const E* p, float (&v)[8]) {
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
+    const E* e = reinterpret_cast<const E*>(&raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = float(e[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = float(p[j]);
+  }
+}
+
+// Tiles of sequence s's pieces and their count of sets.
+__device__ __forceinline__ int seq_tiles(const Seq& s) {
+  return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
+}
+
+// A warp's state: the running maximum and sum of each vector, and O^T times
+// 2^(127 + 14 - top), top the largest value code plus one so far.
+template <int D, int kNT>
+struct Running {
+  uint32_t top;
+  float m[kNT][2], l[kNT][2];
+  float o[kNT][D / 16][4];
+};
+
+// One stage: n tiles at `base` (shared memory), the first holding token `pos0`.
+// lim: tokens seen by the thread's vectors; tokens below `all` are seen by all,
+// tokens from `len` on by none (their bytes may be anything).
+template <int D, int kNT>
+__device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* base, int n,
+                                             int pos0, int all, int len,
+                                             const int (&lim)[kNT][2],
+                                             const float (&qs)[kNT][2],
+                                             const uint32_t (&qf)[kNT][D / 16][2]) {
   constexpr int nb = D / 32;
-  __shared__ float s_q[4][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = blockIdx.x * 4LL + warp;
-  const int head = int(item % a.Hq);
-  const int r = int(item / a.Hq % a.max_q);
-  const int i = int(item / a.Hq / a.max_q);
-  if (i >= a.n_seq) return;
-  const Seq s = sequence(a, i);
-  if (r >= s.rows) return;
-  const int kvh = head / (a.Hq / a.Hkv);
-  const E* q = static_cast<const E*>(a.q) + (s.row0 + r) * a.q_row + head * a.q_head;
-  for (int d = lane; d < D; d += 32) s_q[warp][d] = float(q[d]) * a.scale;
-  __syncwarp();
-  const int see = s.len - s.rows + r + 1;  // tokens this row sees
-  float m = -INFINITY, l = 0.0f, o[nb];
+  const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  // row r of the score tile is token (r & 1) * 4 + r / 2 (+ 8): the weights'
+  // fragment then pairs tokens t and t + 4, so that the four lanes of a quad
+  // read neighbouring value rows
+  const int tok = (gid & 1) * 4 + (gid >> 1);
+  float s[kChunk][kNT][4];
+  uint32_t vw[kChunk][2], tops = 0;
 #pragma unroll
-  for (int b = 0; b < nb; ++b) o[b] = 0.0f;
-  for (int p0 = 0; p0 < see; p0 += 32) {
-    const int p = p0 + lane;
-    float x = -INFINITY;
-    if (p < see) {
-      const uint8_t* tile = tile_at(a, i, kvh, p, D);
-      const int row = p % kv4::kTile;
-      const uint32_t* kw = reinterpret_cast<const uint32_t*>(tile + row * (D / 2));
-      x = 0.0f;
+  for (int i = 0; i < kChunk; ++i) {
+    if (i < n) {
+      const uint8_t* tile = base + i * kv4::tile_bytes(D);
+      uint32_t ka[nb], kb[nb];
+      uint32_t cka, ckb;
+      if (D == 128) {
+        const uint4 a = *reinterpret_cast<const uint4*>(tile + tok * 64 + tig * 16);
+        const uint4 b = *reinterpret_cast<const uint4*>(tile + (tok + 8) * 64 + tig * 16);
+        ka[0] = a.x; ka[1] = a.y; ka[nb - 2] = a.z; ka[nb - 1] = a.w;
+        kb[0] = b.x; kb[1] = b.y; kb[nb - 2] = b.z; kb[nb - 1] = b.w;
+        cka = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4);
+        ckb = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4 + 32);
+        vw[i][0] = *reinterpret_cast<const uint32_t*>(tile + 16 * D + D / 2 + tok * 4);
+        vw[i][1] = *reinterpret_cast<const uint32_t*>(tile + 16 * D + D / 2 + tok * 4 + 32);
+      } else {
+        const uint2 a = *reinterpret_cast<const uint2*>(tile + tok * 32 + tig * 8);
+        const uint2 b = *reinterpret_cast<const uint2*>(tile + (tok + 8) * 32 + tig * 8);
+        ka[0] = a.x; ka[1] = a.y;
+        kb[0] = b.x; kb[1] = b.y;
+        cka = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2);
+        ckb = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2 + 16);
+        vw[i][0] = *reinterpret_cast<const uint16_t*>(tile + 16 * D + D / 2 + tok * 2);
+        vw[i][1] = *reinterpret_cast<const uint16_t*>(tile + 16 * D + D / 2 + tok * 2 + 16);
+      }
+      float fa[nb], fb[nb];
+      codes<nb>(cka, fa);
+      codes<nb>(ckb, fb);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) s[i][j][0] = s[i][j][1] = s[i][j][2] = s[i][j][3] = 0.0f;
+#pragma unroll
       for (int b = 0; b < nb; ++b) {
-        float dot = 0.0f;
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t w = kw[t * nb + b];
+        uint32_t xa[4], xb[4];
+        e2m1x8(ka[b], xa);
+        e2m1x8(kb[b], xb);
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            dot = fmaf(kv4::nibble_value(w >> (4 * j)), s_q[warp][32 * b + 8 * t + j], dot);
+        for (int j = 0; j < kNT; ++j) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma16816(d, xa[0], xb[0], xa[1], xb[1], qf[j][2 * b][0], qf[j][2 * b][1]);
+          mma16816(d, xa[2], xb[2], xa[3], xb[3], qf[j][2 * b + 1][0], qf[j][2 * b + 1][1]);
+          s[i][j][0] = fmaf(d[0], fa[b], s[i][j][0]);
+          s[i][j][1] = fmaf(d[1], fa[b], s[i][j][1]);
+          s[i][j][2] = fmaf(d[2], fb[b], s[i][j][2]);
+          s[i][j][3] = fmaf(d[3], fb[b], s[i][j][3]);
         }
-        x = fmaf(dot, kv4::code_value(tile[16 * D + row * nb + b]), x);
+      }
+      const int pa = pos0 + i * kv4::kTile + tok, pb = pa + 8;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        s[i][j][0] *= qs[j][0];
+        s[i][j][1] *= qs[j][1];
+        s[i][j][2] *= qs[j][0];
+        s[i][j][3] *= qs[j][1];
+      }
+      if (pos0 + (i + 1) * kv4::kTile > all) {  // a tile with tokens that not all vectors see
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) {
+          if (pa >= lim[j][0]) s[i][j][0] = -INFINITY;
+          if (pa >= lim[j][1]) s[i][j][1] = -INFINITY;
+          if (pb >= lim[j][0]) s[i][j][2] = -INFINITY;
+          if (pb >= lim[j][1]) s[i][j][3] = -INFINITY;
+        }
+        if (pa >= len) vw[i][0] = 0;
+        if (pb >= len) vw[i][1] = 0;
+      }
+      tops = more_codes<nb>(more_codes<nb>(tops, vw[i][0]), vw[i][1]);
+    }
+  }
+  const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xFFFFu, tops >> 16));
+  if (top > w.top) {
+    const float c = __uint_as_float(max(127 + int(w.top) - int(top), 0) << 23);
+    w.top = top;
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        w.o[j][k][0] *= c;
+        w.o[j][k][1] *= c;
+        w.o[j][k][2] *= c;
+        w.o[j][k][3] *= c;
+      }
+  }
+  const float unit = __uint_as_float((127 + 127 + 14 - w.top) << 23);  // 2^(127 + 14 - top)
+  // running maximum of the scores (log2 domain), over the stage's tokens
+#pragma unroll
+  for (int j = 0; j < kNT; ++j) {
+    float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+      if (i < n) {
+        t0 = fmaxf(t0, fmaxf(s[i][j][0], s[i][j][2]));
+        t1 = fmaxf(t1, fmaxf(s[i][j][1], s[i][j][3]));
       }
     }
-    float mx = x;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    const float nm = fmax_nan(m, mx);
-    const float ref = nm == -INFINITY ? 0.0f : nm;
-    const float corr = expf(m - ref), pr = expf(x - ref);
-    m = nm;
-    float sum = pr;
+    for (int off = 4; off <= 16; off <<= 1) {
+      t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
+      t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
+    }
+    // the reference moves only when it is passed by more than 1 (P_b <= 2^15)
+    const bool up0 = t0 > w.m[j][0] + 1.0f, up1 = t1 > w.m[j][1] + 1.0f;
+    if (__any_sync(0xffffffffu, up0 || up1)) {
+      const float m0 = up0 ? t0 : w.m[j][0], m1 = up1 ? t1 : w.m[j][1];
+      const float c0 = up0 ? ex2(w.m[j][0] - m0) : 1.0f, c1 = up1 ? ex2(w.m[j][1] - m1) : 1.0f;
+      w.m[j][0] = m0;
+      w.m[j][1] = m1;
+      w.l[j][0] *= c0;
+      w.l[j][1] *= c1;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-    l = l * corr + sum;
-#pragma unroll
-    for (int b = 0; b < nb; ++b) o[b] *= corr;
-    for (int j = 0; j < 32 && p0 + j < see; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, pr, j);
-      const uint8_t* tile = tile_at(a, i, kvh, p0 + j, D);
-      const int row = (p0 + j) % kv4::kTile;
-      const uint8_t* vr = tile + 8 * D + row * (D / 2);
-      // lane = element of each block: piece lane / 4, nibble lane % 4
-#pragma unroll
-      for (int b = 0; b < nb; ++b) {
-        const uint8_t byte = vr[((lane >> 2) * nb + b) * 2 + ((lane & 3) >> 1)];
-        const float v = kv4::nibble_value(uint32_t(byte) >> (4 * (lane & 1))) *
-                        kv4::code_value(tile[16 * D + D / 2 + row * nb + b]);
-        o[b] = fmaf(pj, v, o[b]);
+      for (int k = 0; k < D / 16; ++k) {
+        w.o[j][k][0] *= c0;
+        w.o[j][k][1] *= c1;
+        w.o[j][k][2] *= c0;
+        w.o[j][k][3] *= c1;
       }
     }
   }
-  E* out = static_cast<E*>(a.out) + ((long long)(s.row0 + r) * a.Hq + head) * D;
 #pragma unroll
-  for (int b = 0; b < nb; ++b) out[32 * b + lane] = E(l == 0.0f ? 0.0f : o[b] / l);
+  for (int i = 0; i < kChunk; ++i) {
+    if (i < n) {
+      const uint8_t* tile = base + i * kv4::tile_bytes(D);
+      float fa[nb], fb[nb];
+      codes<nb>(vw[i][0], fa);
+      codes<nb>(vw[i][1], fb);
+      uint32_t pf[kNT][nb][2];  // weights' fragments: tokens 2tig, 2tig+1 (+8) of vector gid
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        // a vector that has seen nothing keeps m = -inf; its scores are all -inf too
+        const float r0 = w.m[j][0] == -INFINITY ? 0.0f : w.m[j][0];
+        const float r1 = w.m[j][1] == -INFINITY ? 0.0f : w.m[j][1];
+        float p0 = ex2(s[i][j][0] - r0), p1 = ex2(s[i][j][1] - r1);
+        float p2 = ex2(s[i][j][2] - r0), p3 = ex2(s[i][j][3] - r1);
+        w.l[j][0] += p0 + p2;
+        w.l[j][1] += p1 + p3;
+        p0 *= unit;
+        p1 *= unit;
+        p2 *= unit;
+        p3 *= unit;
+        if (pos0 + (i + 1) * kv4::kTile > all) {
+          // what a vector does not see may hold anything: codes of 255 make no NaN of its zeros
+#pragma unroll
+          for (int b = 0; b < nb; ++b) {
+            pf[j][b][0] = pack_half(s[i][j][0] == -INFINITY ? 0.0f : p0 * fa[b],
+                                    s[i][j][1] == -INFINITY ? 0.0f : p1 * fa[b]);
+            pf[j][b][1] = pack_half(s[i][j][2] == -INFINITY ? 0.0f : p2 * fb[b],
+                                    s[i][j][3] == -INFINITY ? 0.0f : p3 * fb[b]);
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < nb; ++b) {
+            pf[j][b][0] = pack_half(p0 * fa[b], p1 * fa[b]);
+            pf[j][b][1] = pack_half(p2 * fb[b], p3 * fb[b]);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < nb; ++b) {
+          pf[j][b][0] = transpose8x8(pf[j][b][0]);
+          pf[j][b][1] = transpose8x8(pf[j][b][1]);
+        }
+      }
+      // value rows tig, tig + 4, tig + 8, tig + 12: elements 4 gid .. 4 gid + 3 of each block
+      uint32_t v[4][nb / 2];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const uint8_t* vr = tile + 8 * D + (tig + 4 * r) * (D / 2) + gid * (2 * nb);
+        if (D == 128) {
+          const uint2 x = *reinterpret_cast<const uint2*>(vr);
+          v[r][0] = x.x;
+          v[r][nb / 2 - 1] = x.y;
+        } else {
+          v[r][0] = *reinterpret_cast<const uint32_t*>(vr);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < nb / 2; ++h) {  // blocks 2h and 2h + 1
+        constexpr uint32_t kLo = 0x0F0F0F0Fu;
+        uint32_t a0[4], a1[4], a2[4], a3[4];
+        e2m1x8((v[0][h] & kLo) | ((v[1][h] << 4) & ~kLo), a0);  // even elements, tokens t, t + 4
+        e2m1x8(((v[0][h] >> 4) & kLo) | (v[1][h] & ~kLo), a1);  // odd elements
+        e2m1x8((v[2][h] & kLo) | ((v[3][h] << 4) & ~kLo), a2);  // tokens t + 8, t + 12
+        e2m1x8(((v[2][h] >> 4) & kLo) | (v[3][h] & ~kLo), a3);
+#pragma unroll
+        for (int j = 0; j < kNT; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)  // byte k: block 2h + k / 2, elements 2 (k % 2), + 1
+            mma16816(w.o[j][4 * h + k], a0[k], a1[k], a2[k], a3[k], pf[j][2 * h + (k >> 1)][0],
+                     pf[j][2 * h + (k >> 1)][1]);
+      }
+    }
+  }
 }
+
+// Partial sums of a piece that several CTAs share: slot 0 of a CTA holds the
+// piece that began before its share, slot 1 the one that goes on after it.
+template <int D, int kNT>
+__device__ __forceinline__ float* slot_of(float* part, int cta, int slot) {
+  return part + (size_t(cta) * 2 + slot) * (Few<D, kNT>::kVec * Few<D, kNT>::kAcc);
+}
+
+template <class E>
+__device__ __forceinline__ void store_vector(const AttnArgs& a, const Seq& s, int g, int G, int v,
+                                             int lane, const float (&o)[4], float inv, int D) {
+  const int r = v / G, h = v - r * G;
+  E* dst = static_cast<E*>(a.out) + ((long long)(s.row0 + r) * a.Hq + g * G + h) * D + 4 * lane;
+  E x[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = E(o[i] * inv);
+  *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
+}
+
+template <class E, int D, int kNT>
+__global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(AttnArgs a) {
+  using F = Few<D, kNT>;
+  constexpr int nb = D / 32;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint64_t s_bar[F::kWarps][kStages];
+  __shared__ long long s_scan[F::kWarps];
+  __shared__ long long s_total, s_start;  // all units; first unit of sequence s_first
+  __shared__ int s_first, s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  const int G = a.Hq / a.Hkv;
+  uint8_t* ring = smem + warp * F::kWarpBytes;
+  if (threadIdx.x == 0) tc::cta_abort_init();
+  if (lane == 0)
+    for (int i = 0; i < kStages; ++i) tc::mbar_init(&s_bar[warp][i], 1);
+  tc::fence_mbar_init();
+
+  // ---- this CTA's share of the work: each thread sums a run of sequences
+  const int per = (a.n_seq + F::kThreads - 1) / F::kThreads;
+  const int i0 = min(int(threadIdx.x) * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) {
+    const Seq s = sequence(a, i);
+    mine += (long long)seq_tiles(s) * a.Hkv * ((s.rows * G + F::kVec - 1) / F::kVec);
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, inc, off);
+    if (lane >= off) inc += x;
+  }
+  if (lane == 31) s_scan[warp] = inc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    long long sum = 0;
+    for (int i = 0; i < F::kWarps; ++i) {
+      const long long x = s_scan[i];
+      s_scan[i] = sum;
+      sum += x;
+    }
+    s_total = sum;
+  }
+  __syncthreads();
+  const long long U = s_total;
+  if (U == 0) return;
+  // one tile a warp at least: more CTAs would only add partial sums to join
+  const long long ctas = min((long long)gridDim.x, (U + F::kWarps - 1) / F::kWarps);
+  if (blockIdx.x >= ctas) return;
+  const long long lo = U * blockIdx.x / ctas, hi = U * (blockIdx.x + 1) / ctas;
+  long long before = s_scan[warp] + inc - mine;
+  if (before <= lo && lo < before + mine) {
+    for (int i = i0; i < i1; ++i) {
+      const Seq s = sequence(a, i);
+      const long long n = (long long)seq_tiles(s) * a.Hkv * ((s.rows * G + F::kVec - 1) / F::kVec);
+      if (lo < before + n) {
+        s_first = i;
+        s_start = before;
+        break;
+      }
+      before += n;
+    }
+  }
+  __syncthreads();
+
+  int seq = s_first;
+  long long seq_start = s_start;
+  Seq s = sequence(a, seq);
+  uint32_t it = 0;  // stages this warp has filled
+  for (long long u = lo; u < hi;) {
+    int tiles = seq_tiles(s), sets = (s.rows * G + F::kVec - 1) / F::kVec;
+    while (u >= seq_start + (long long)tiles * a.Hkv * sets) {
+      seq_start += (long long)tiles * a.Hkv * sets;
+      s = sequence(a, ++seq);
+      tiles = seq_tiles(s);
+      sets = (s.rows * G + F::kVec - 1) / F::kVec;
+    }
+    const int piece = int((u - seq_start) / tiles);
+    const int g = piece / sets, set = piece - g * sets;
+    const long long p_lo = seq_start + (long long)piece * tiles, p_hi = p_lo + tiles;
+    const int t_lo = int(u - p_lo), t_hi = int(min(hi, p_hi) - p_lo);
+    u = min(hi, p_hi);
+
+    // ---- the set's query rows as B fragments, scaled to a maximum near 2^15
+    const int v0 = set * F::kVec, nv = s.rows * G;
+    uint32_t qf[kNT][D / 16][2];
+    float qs[kNT][2];
+    int lim[kNT][2];
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      const int v = v0 + 8 * j + gid;
+      float x[nb][8], am = 0.0f;
+#pragma unroll
+      for (int b = 0; b < nb; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
+      if (v < nv) {
+        const int r = v / G, h = v - r * G;
+        const E* q = static_cast<const E*>(a.q) + (s.row0 + r) * a.q_row + (g * G + h) * a.q_head;
+#pragma unroll
+        for (int b = 0; b < nb; ++b) q8(q + 32 * b + 8 * tig, x[b]);
+      }
+#pragma unroll
+      for (int b = 0; b < nb; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[b][i]));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+      am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+      const int e = max(int(__float_as_uint(am) >> 23) - 127, -100);
+      const float f = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+#pragma unroll
+      for (int b = 0; b < nb; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          qf[j][2 * b + (i >> 1)][i & 1] = pack_half(x[b][2 * i] * f, x[b][2 * i + 1] * f);
+      // back to the thread's score columns: vectors 2 tig and 2 tig + 1
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int ee = __shfl_sync(0xffffffffu, e, (2 * tig + i) * 4);
+        qs[j][i] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + ee) << 23);
+        const int c = v0 + 8 * j + 2 * tig + i;
+        lim[j][i] = c < nv ? s.len - s.rows + c / G + 1 : 0;
+      }
+    }
+    const int all = s.len - s.rows + v0 / G + 1;
+
+    // ---- tiles of the piece, in runs of up to kChunk, dealt over the warps
+    Running<D, kNT> w;
+    w.top = 29;  // a block of zeros
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      w.m[j][0] = w.m[j][1] = -INFINITY;
+      w.l[j][0] = w.l[j][1] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) w.o[j][k][0] = w.o[j][k][1] = w.o[j][k][2] = w.o[j][k][3] = 0.0f;
+    }
+    const int run = min(kChunk, (t_hi - t_lo + F::kWarps - 1) / F::kWarps);
+    const int runs = (t_hi - t_lo + run - 1) / run;
+    const int tpp = a.page / kv4::kTile;
+    const int have = (s.len + kv4::kTile - 1) / kv4::kTile;  // tiles with tokens
+    // page id of this lane's tile of a run (loaded one run ahead of its copy)
+    auto page_of = [&](int r) {
+      const int t = t_lo + r * run + lane;
+      return (r < runs && lane < run && t < min(t_hi, have)) ? a.table[seq * a.table_ld + t / tpp] : -1;
+    };
+    auto fill = [&](int r, int id, uint32_t stage) {  // whole warp; r < runs
+      const int t0 = t_lo + r * run;
+      const int n = max(min(min(run, t_hi - t0), have - t0), 0);
+      uint64_t* bar = &s_bar[warp][stage];
+      if (lane == 0) tc::mbar_expect_tx(bar, uint32_t(n) * kv4::tile_bytes(D));
+      __syncwarp();
+      if (lane < n) {
+        if (id < 0 || id >= a.num_pages) {
+          kv4::report(a.err, kv4::kErrPage);
+          id = 0;
+        }
+        const uint8_t* src = a.pool + ((long long)id * a.Hkv + g) * kv4::head_bytes(D, a.page) +
+                             (long long)((t0 + lane) % tpp) * kv4::tile_bytes(D);
+        tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D), src,
+                      kv4::tile_bytes(D), bar);
+      }
+    };
+    uint32_t filled = it;
+    int next = warp, id = page_of(next);
+    for (int k = 0; k < kStages - 1 && next < runs; ++k, ++filled) {
+      fill(next, id, filled % kStages);
+      next += F::kWarps;
+      id = page_of(next);
+    }
+    for (int r = warp; r < runs; r += F::kWarps, ++it) {
+      if (next < runs) {
+        __syncwarp();  // the stage's last readers are done
+        fill(next, id, filled % kStages);
+        ++filled;
+        next += F::kWarps;
+        id = page_of(next);
+      }
+      const uint32_t stage = it % kStages;
+      tc::mbar_wait(&s_bar[warp][stage], (it / kStages) & 1u, a.err, 1);
+      const int t0 = t_lo + r * run;
+      const int n = min(min(run, t_hi - t0), have - t0);
+      attend_tiles<D, kNT>(w, ring + stage * F::kStageBytes, n, t0 * kv4::kTile, all, s.len, lim, qs,
+                           qf);
+    }
+
+    // ---- join the warps: sums of l over the quad's lanes, then through shared memory
+    const float unit = __uint_as_float((w.top - 14) << 23);  // 2^(top - 127 - 14)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int off = 4; off <= 16; off <<= 1)
+          w.l[j][i] += __shfl_xor_sync(0xffffffffu, w.l[j][i], off);
+    __syncwarp();
+    float* acc = reinterpret_cast<float*>(ring);
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float* dst = acc + (8 * j + 2 * tig + i) * F::kAcc;
+#pragma unroll
+        for (int b = 0; b < nb; ++b)
+          *reinterpret_cast<float4*>(dst + 32 * b + 4 * gid) =
+              make_float4(w.o[j][2 * b][i] * unit, w.o[j][2 * b][i + 2] * unit,
+                          w.o[j][2 * b + 1][i] * unit, w.o[j][2 * b + 1][i + 2] * unit);
+        if (gid == 0) {
+          dst[D] = w.m[j][i];
+          dst[D + 1] = w.l[j][i];
+        }
+      }
+    __syncthreads();
+    const bool whole = t_lo == 0 && t_hi == tiles;
+    const int slot = t_lo == 0 ? 1 : 0;
+    float* part = slot_of<D, kNT>(a.part, blockIdx.x, slot);
+    const int busy = min(F::kWarps, runs);  // warps that had a run
+    for (int v = warp; v < F::kVec; v += F::kWarps) {
+      float m = -INFINITY;
+      for (int i = 0; i < busy; ++i)
+        m = fmaxf(m, reinterpret_cast<const float*>(smem + i * F::kWarpBytes)[v * F::kAcc + D]);
+      float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < busy; ++i) {
+        const float* src = reinterpret_cast<const float*>(smem + i * F::kWarpBytes) + v * F::kAcc;
+        const float c = src[D] == -INFINITY ? 0.0f : ex2(src[D] - m);
+        l = fmaf(c, src[D + 1], l);
+        if (4 * lane < D) {
+          const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
+          o[0] = fmaf(c, x.x, o[0]);
+          o[1] = fmaf(c, x.y, o[1]);
+          o[2] = fmaf(c, x.z, o[2]);
+          o[3] = fmaf(c, x.w, o[3]);
+        }
+      }
+      if (whole) {
+        if (v0 + v < nv && 4 * lane < D)
+          store_vector<E>(a, s, g, G, v0 + v, lane, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+      } else {
+        if (4 * lane < D)
+          *reinterpret_cast<float4*>(part + v * F::kAcc + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
+        if (lane == 0) *reinterpret_cast<float2*>(part + v * F::kAcc + D) = make_float2(m, l);
+      }
+    }
+    if (!whole) {
+      // the piece's last CTA to arrive joins the parts, in the CTAs' order
+      const int c_first = int(((p_lo + 1) * ctas - 1) / U), c_last = int((p_hi * ctas - 1) / U);
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0)
+        s_last = atomicInc(a.counters + c_first, unsigned(c_last - c_first)) == unsigned(c_last - c_first);
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        const int parts = c_last - c_first + 1;
+        for (int v = warp; v < F::kVec && v0 + v < nv; v += F::kWarps) {
+          float m = -INFINITY;
+          for (int i = lane; i < parts; i += 32)
+            m = fmaxf(m, __ldcg(slot_of<D, kNT>(a.part, c_first + i, i == 0) + v * F::kAcc + D));
+#pragma unroll
+          for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+          float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+          for (int i = 0; i < parts; ++i) {
+            const float* src = slot_of<D, kNT>(a.part, c_first + i, i == 0) + v * F::kAcc;
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + D));
+            const float4 x = 4 * lane < D ? __ldcg(reinterpret_cast<const float4*>(src + 4 * lane))
+                                          : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float c = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
+            l = fmaf(c, ml.y, l);
+            o[0] = fmaf(c, x.x, o[0]);
+            o[1] = fmaf(c, x.y, o[1]);
+            o[2] = fmaf(c, x.z, o[2]);
+            o[3] = fmaf(c, x.w, o[3]);
+          }
+          if (4 * lane < D)
+            store_vector<E>(a, s, g, G, v0 + v, lane, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+        }
+      }
+    }
+    __syncthreads();  // the warps' sums are read: their memory takes tiles again
+    // the sums were written by ordinary stores, the next tiles by bulk copies
+    tc::fence_proxy_async_smem();
+  }
+  if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], kStages, it);
+}
+
+template <class E, int D, int kNT>
+cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
+  using F = Few<D, kNT>;
+  const void* fn = reinterpret_cast<const void*>(kv4_attn_few_kernel<E, D, kNT>);
+  const cudaError_t e = ensure_dynamic_smem(fn, F::kSmem);
+  if (e != cudaSuccess) return e;
+  kv4_attn_few_kernel<E, D, kNT><<<kCtas, F::kThreads, F::kSmem, s>>>(a);
+  return cudaGetLastError();
+}
+
+// 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
+// are then read and decoded half as often), else 8.
+template <class E, int D>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+  const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
+  return vectors <= 8 ? launch_few<E, D, 1>(a, s) : launch_few<E, D, 2>(a, s);
+}
+
+constexpr size_t kCounterBytes = 1024;  // one counter per CTA
+static_assert(kCounterBytes >= kCtas * sizeof(unsigned), "a counter per CTA");
 
 }  // namespace
 }  // namespace mfi
@@ -145,7 +707,7 @@ __global__ void __launch_bounds__(128) kv4_attn_kernel(AttnArgs a) {
 extern "C" size_t mfi_kv4_attn_workspace_bytes(int n_seq, int Hq, int Hkv, int D, int max_q) {
   if (n_seq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_q <= 0)
     return 0;
-  return 256;
+  return mfi::kCounterBytes + size_t(mfi::kCtas) * 2 * 16 * (D + 4) * sizeof(float);
 }
 
 extern "C" int mfi_kv4_attn_init_workspace(void* workspace, size_t workspace_bytes, void* stream) {
@@ -174,6 +736,10 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   if (T == 0 || n_seq == 0 || max_q == 0) return MFI_OK;
   if (!q || !table || !kv_lens || !out || !workspace)
     return mfi::set_last_error(MFI_ERR_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 15)
+    return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: out must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(workspace) & 255)
+    return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: the workspace must be 256-byte aligned");
   if (workspace_bytes < mfi_kv4_attn_workspace_bytes(n_seq, Hq, Hkv, D, max_q))
     return mfi::set_last_error(MFI_ERR_WORKSPACE, "workspace smaller than the kv4_attn workspace query");
   mfi::AttnArgs a{};
@@ -184,17 +750,13 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   a.T = T; a.max_q = max_q; a.n_seq = n_seq; a.Hq = Hq; a.Hkv = Hkv;
   a.page = page; a.num_pages = num_pages; a.width = width;
   a.scale = scale;
+  a.counters = static_cast<unsigned*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + mfi::kCounterBytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const long long blocks = ((long long)n_seq * max_q * Hq + 3) / 4;
-  if (blocks > 0x7FFFFFFFLL) return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: too many rows");
-  const unsigned g = unsigned(blocks);
-  if (dtype == MFI_BF16) {
-    if (D == 128) mfi::kv4_attn_kernel<__nv_bfloat16, 128><<<g, 128, 0, s>>>(a);
-    else mfi::kv4_attn_kernel<__nv_bfloat16, 64><<<g, 128, 0, s>>>(a);
-  } else {
-    if (D == 128) mfi::kv4_attn_kernel<__half, 128><<<g, 128, 0, s>>>(a);
-    else mfi::kv4_attn_kernel<__half, 64><<<g, 128, 0, s>>>(a);
-  }
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (dtype == MFI_BF16)
+    e = D == 128 ? mfi::launch<__nv_bfloat16, 128>(a, s) : mfi::launch<__nv_bfloat16, 64>(a, s);
+  else
+    e = D == 128 ? mfi::launch<__half, 128>(a, s) : mfi::launch<__half, 64>(a, s);
   return e == cudaSuccess ? MFI_OK : mfi::set_last_error(MFI_ERR_CUDA, cudaGetErrorString(e));
 }
