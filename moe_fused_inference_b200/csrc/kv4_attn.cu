@@ -32,6 +32,8 @@ struct AttnArgs {
   unsigned* counters;        // one per CTA, zero between calls
   float* part;               // two slots per CTA
   int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
+  bool q_vec;                // every query row starts on a 16-byte boundary
+  int tpp_shift;             // log2 of the tiles of a page, -1 if that is no power of two
   float scale;
 };
 
@@ -75,21 +77,19 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 // 2^(14 - top), top the largest value code so far: it keeps all its bits down to
 // 2^-28 and vanishes below 2^-39 of the largest weight times the largest scale.
 // As top is a whole power of two it changes no other bit of P_b.
-constexpr int kChunk = 2;    // tiles of a pipeline stage
-constexpr int kStages = 3;
+constexpr int kChunk = 4;    // tiles of a pipeline stage
+constexpr int kStages = 2;   // one read, one on its way
 constexpr int kCtas = 148;   // one per SM
 
 template <int D, int kNT>
 struct Few {
-  static constexpr int kWarps = kNT == 1 ? 16 : 8;
+  static constexpr int kWarps = kNT == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
   static constexpr int kStageBytes = kChunk * kv4::tile_bytes(D);
   static constexpr int kAcc = D + 4;                          // floats of a vector's sum: D, max, sum, pad
-  static constexpr int kRing = kStages * kStageBytes;
-  static constexpr int kMerge = kVec * kAcc * 4;
-  static constexpr int kWarpBytes = ((kRing > kMerge ? kRing : kMerge) + 127) / 128 * 128;
-  static constexpr int kSmem = kWarps * kWarpBytes;
+  static_assert(kVec * kAcc * 4 <= kStageBytes, "a warp's sums take the place of a stage");
+  static constexpr int kSmem = kWarps * kStages * kStageBytes;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -116,14 +116,6 @@ __device__ __forceinline__ void codes(uint32_t w, float (&f)[nb]) {
     f[2 * i + 1] = __uint_as_float(r & 0xFFFF0000u);
   }
 }
-// The larger of m (two 16-bit halves) and the nb codes of w plus one; a code of
-// 255 (NaN) counts as 0 (two such neighbours may carry one too many).
-template <int nb>
-__device__ __forceinline__ uint32_t more_codes(uint32_t m, uint32_t w) {
-  if (nb == 2) return __vmaxu2(m, ((w & 0xFFu) | ((w << 8) & 0x00FF0000u)) + 0x00010001u & 0x00FF00FFu);
-  m = __vmaxu2(m, (w + 0x00010001u) & 0x00FF00FFu);
-  return __vmaxu2(m, ((w >> 8) + 0x00010001u) & 0x00FF00FFu);
-}
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -142,17 +134,23 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 8 elements of a query row as they are; vec: p is 16-byte aligned.
 template <class E>
-__device__ __forceinline__ void q8(const E* p, float (&v)[8]) {
-  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
-    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p));
-    const E* e = reinterpret_cast<const E*>(&raw);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = float(e[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = float(p[j]);
-  }
+__device__ __forceinline__ uint4 q8(const E* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16,
+                    h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
+}
+template <class E>
+__device__ __forceinline__ float2 two_floats(uint32_t w);
+template <>
+__device__ __forceinline__ float2 two_floats<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
 // Tiles of sequence s's pieces and their count of sets.
@@ -161,7 +159,8 @@ __device__ __forceinline__ int seq_tiles(const Seq& s) {
 }
 
 // A warp's state: the running maximum and sum of each vector, and O^T times
-// 2^(127 + 14 - top), top the largest value code plus one so far.
+// 2^(127 + 14 - top), top the largest value code plus one so far (a code of 255,
+// NaN, counts as 0; two such neighbours may carry one too many).
 template <int D, int kNT>
 struct Running {
   uint32_t top;
@@ -185,7 +184,6 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
   // read neighbouring value rows
   const int tok = (gid & 1) * 4 + (gid >> 1);
   float s[kChunk][kNT][4];
-  uint32_t vw[kChunk][2], tops = 0;
 #pragma unroll
   for (int i = 0; i < kChunk; ++i) {
     if (i < n) {
@@ -199,8 +197,6 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
         kb[0] = b.x; kb[1] = b.y; kb[nb - 2] = b.z; kb[nb - 1] = b.w;
         cka = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4);
         ckb = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4 + 32);
-        vw[i][0] = *reinterpret_cast<const uint32_t*>(tile + 16 * D + D / 2 + tok * 4);
-        vw[i][1] = *reinterpret_cast<const uint32_t*>(tile + 16 * D + D / 2 + tok * 4 + 32);
       } else {
         const uint2 a = *reinterpret_cast<const uint2*>(tile + tok * 32 + tig * 8);
         const uint2 b = *reinterpret_cast<const uint2*>(tile + (tok + 8) * 32 + tig * 8);
@@ -208,8 +204,6 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
         kb[0] = b.x; kb[1] = b.y;
         cka = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2);
         ckb = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2 + 16);
-        vw[i][0] = *reinterpret_cast<const uint16_t*>(tile + 16 * D + D / 2 + tok * 2);
-        vw[i][1] = *reinterpret_cast<const uint16_t*>(tile + 16 * D + D / 2 + tok * 2 + 16);
       }
       float fa[nb], fb[nb];
       codes<nb>(cka, fa);
@@ -248,10 +242,25 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
           if (pb >= lim[j][0]) s[i][j][2] = -INFINITY;
           if (pb >= lim[j][1]) s[i][j][3] = -INFINITY;
         }
-        if (pa >= len) vw[i][0] = 0;
-        if (pb >= len) vw[i][1] = 0;
       }
-      tops = more_codes<nb>(more_codes<nb>(tops, vw[i][0]), vw[i][1]);
+    }
+  }
+  // the largest value code of the stage's seen tokens, each word read by one lane
+  uint32_t tops = 0;
+  {
+    constexpr int kPer = 128 / D;               // tokens of a word of codes
+    constexpr int kWords = kv4::kTile / kPer;   // words of a tile
+#pragma unroll
+    for (int k = 0; k < (kChunk * kWords + 31) / 32; ++k) {
+      const int i = k * (32 / kWords) + lane / kWords, x = lane % kWords;
+      const int seen = len - pos0 - i * kv4::kTile - x * kPer;  // of the word's tokens
+      if (i < n && seen > 0) {
+        uint32_t c = *reinterpret_cast<const uint32_t*>(base + i * kv4::tile_bytes(D) + 16 * D +
+                                                        D / 2 + 4 * x);
+        if (kPer == 2 && seen == 1) c &= 0xFFFFu;
+        tops = __vmaxu2(tops, (c + 0x00010001u) & 0x00FF00FFu);
+        tops = __vmaxu2(tops, ((c >> 8) + 0x00010001u) & 0x00FF00FFu);
+      }
     }
   }
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xFFFFu, tops >> 16));
@@ -308,8 +317,12 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
     if (i < n) {
       const uint8_t* tile = base + i * kv4::tile_bytes(D);
       float fa[nb], fb[nb];
-      codes<nb>(vw[i][0], fa);
-      codes<nb>(vw[i][1], fb);
+      {
+        const uint8_t* c = tile + 16 * D + D / 2 + tok * nb;
+        codes<nb>(nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c), fa);
+        c += 8 * nb;
+        codes<nb>(nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c), fb);
+      }
       uint32_t pf[kNT][nb][2];  // weights' fragments: tokens 2tig, 2tig+1 (+8) of vector gid
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
@@ -387,14 +400,63 @@ __device__ __forceinline__ float* slot_of(float* part, int cta, int slot) {
 
 template <class E>
 __device__ __forceinline__ void store_vector(const AttnArgs& a, const Seq& s, int g, int G, int v,
-                                             int lane, const float (&o)[4], float inv, int D) {
+                                             int d0, const float (&o)[4], float inv, int D) {
   const int r = v / G, h = v - r * G;
-  E* dst = static_cast<E*>(a.out) + ((long long)(s.row0 + r) * a.Hq + g * G + h) * D + 4 * lane;
+  E* dst = static_cast<E*>(a.out) + ((long long)(s.row0 + r) * a.Hq + g * G + h) * D + d0;
   E x[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] = E(o[i] * inv);
   *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(x);
 }
+
+// Join what `count` warps or CTAs left of a set, each a row of kVec sums, read by
+// `at`(i): this warp takes rows first, first + step, .. of all vectors at once.
+template <int D, int kNT, class At>
+__device__ __forceinline__ void join_rows(int first, int step, int count, At at,
+                                          float (&m)[Few<D, kNT>::kVec * D / 128],
+                                          float (&l)[Few<D, kNT>::kVec * D / 128],
+                                          float4 (&o)[Few<D, kNT>::kVec * D / 128]) {
+  using F = Few<D, kNT>;
+  constexpr int kPer = D / 4, kRows = 32 / kPer, kN = F::kVec / kRows;  // lanes of a vector, ..
+  const int lane = threadIdx.x & 31, sub = lane / kPer, d0 = (lane % kPer) * 4;
+#pragma unroll
+  for (int k = 0; k < kN; ++k) {
+    m[k] = -INFINITY;
+    l[k] = 0.0f;
+    o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int i = first; i < count; i += step) {
+    const float* src = at(i);
+    float2 ml[kN];
+    float4 x[kN];
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const float* v = src + (k * kRows + sub) * F::kAcc;
+      ml[k] = __ldcg(reinterpret_cast<const float2*>(v + D));
+      x[k] = __ldcg(reinterpret_cast<const float4*>(v + d0));
+    }
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+      const float nm = fmaxf(m[k], ml[k].x);
+      const float ref = nm == -INFINITY ? 0.0f : nm;
+      const float c0 = ex2(m[k] - ref), c1 = ex2(ml[k].x - ref);
+      m[k] = nm;
+      l[k] = l[k] * c0 + ml[k].y * c1;
+      o[k].x = o[k].x * c0 + x[k].x * c1;
+      o[k].y = o[k].y * c0 + x[k].y * c1;
+      o[k].z = o[k].z * c0 + x[k].z * c1;
+      o[k].w = o[k].w * c0 + x[k].w * c1;
+    }
+  }
+}
+
+// A CTA's part of a piece: tiles [t_lo, t_hi) of the set from vector v0 of KV
+// head g of sequence seq.
+struct Part {
+  Seq s;
+  int seq, g, v0, t_lo, t_hi, tiles;
+  unsigned start;  // the piece's first unit
+};
 
 template <class E, int D, int kNT>
 __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(AttnArgs a) {
@@ -402,54 +464,54 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   constexpr int nb = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[F::kWarps][kStages];
-  __shared__ long long s_scan[F::kWarps];
-  __shared__ long long s_total, s_start;  // all units; first unit of sequence s_first
+  __shared__ unsigned s_scan[F::kWarps];
+  __shared__ unsigned s_start;  // first unit of sequence s_first
   __shared__ int s_first, s_last;
+  __shared__ float* s_sums[F::kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int G = a.Hq / a.Hkv;
-  uint8_t* ring = smem + warp * F::kWarpBytes;
+  uint8_t* ring = smem + warp * (kStages * F::kStageBytes);
   if (threadIdx.x == 0) tc::cta_abort_init();
   if (lane == 0)
     for (int i = 0; i < kStages; ++i) tc::mbar_init(&s_bar[warp][i], 1);
   tc::fence_mbar_init();
 
   // ---- this CTA's share of the work: each thread sums a run of sequences
+  auto sets_of = [&](const Seq& s) { return (s.rows * G + F::kVec - 1) / F::kVec; };
+  auto units_of = [&](const Seq& s) { return unsigned(seq_tiles(s)) * a.Hkv * sets_of(s); };
   const int per = (a.n_seq + F::kThreads - 1) / F::kThreads;
   const int i0 = min(int(threadIdx.x) * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
-  long long mine = 0;
-  for (int i = i0; i < i1; ++i) {
-    const Seq s = sequence(a, i);
-    mine += (long long)seq_tiles(s) * a.Hkv * ((s.rows * G + F::kVec - 1) / F::kVec);
-  }
-  long long inc = mine;
+  unsigned mine = 0;
+  for (int i = i0; i < i1; ++i) mine += units_of(sequence(a, i));
+  unsigned inc = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long x = __shfl_up_sync(0xffffffffu, inc, off);
+    const unsigned x = __shfl_up_sync(0xffffffffu, inc, off);
     if (lane >= off) inc += x;
   }
   if (lane == 31) s_scan[warp] = inc;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    long long sum = 0;
-    for (int i = 0; i < F::kWarps; ++i) {
-      const long long x = s_scan[i];
-      s_scan[i] = sum;
-      sum += x;
-    }
-    s_total = sum;
+  unsigned U = 0, before = inc - mine;
+#pragma unroll
+  for (int i = 0; i < F::kWarps; ++i) {
+    if (i < warp) before += s_scan[i];
+    U += s_scan[i];
   }
-  __syncthreads();
-  const long long U = s_total;
   if (U == 0) return;
-  // one tile a warp at least: more CTAs would only add partial sums to join
-  const long long ctas = min((long long)gridDim.x, (U + F::kWarps - 1) / F::kWarps);
+  // one tile a warp at least: more CTAs would only add partial sums to join.
+  // CTA c takes `base` units, one more for c < more.
+  const unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
   if (blockIdx.x >= ctas) return;
-  const long long lo = U * blockIdx.x / ctas, hi = U * (blockIdx.x + 1) / ctas;
-  long long before = s_scan[warp] + inc - mine;
+  const unsigned base = U / ctas, more = U - base * ctas;
+  auto first_unit = [&](unsigned c) { return c * base + min(c, more); };
+  auto cta_of = [&](unsigned u) {
+    const unsigned x = more * (base + 1);
+    return u < x ? u / (base + 1) : more + (u - x) / base;
+  };
+  const unsigned lo = first_unit(blockIdx.x), hi = first_unit(blockIdx.x + 1);
   if (before <= lo && lo < before + mine) {
     for (int i = i0; i < i1; ++i) {
-      const Seq s = sequence(a, i);
-      const long long n = (long long)seq_tiles(s) * a.Hkv * ((s.rows * G + F::kVec - 1) / F::kVec);
+      const unsigned n = units_of(sequence(a, i));
       if (lo < before + n) {
         s_first = i;
         s_start = before;
@@ -460,47 +522,113 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   }
   __syncthreads();
 
-  int seq = s_first;
-  long long seq_start = s_start;
-  Seq s = sequence(a, seq);
-  uint32_t it = 0;  // stages this warp has filled
-  for (long long u = lo; u < hi;) {
-    int tiles = seq_tiles(s), sets = (s.rows * G + F::kVec - 1) / F::kVec;
-    while (u >= seq_start + (long long)tiles * a.Hkv * sets) {
-      seq_start += (long long)tiles * a.Hkv * sets;
-      s = sequence(a, ++seq);
-      tiles = seq_tiles(s);
-      sets = (s.rows * G + F::kVec - 1) / F::kVec;
+  // the part that holds unit u, of a sequence at or after p.seq (which starts at unit seq_start)
+  unsigned seq_start = s_start;
+  auto part_at = [&](Part& p, unsigned u) {
+    unsigned n = units_of(p.s);
+    while (u >= seq_start + n) {
+      seq_start += n;
+      p.s = sequence(a, ++p.seq);
+      n = units_of(p.s);
     }
-    const int piece = int((u - seq_start) / tiles);
-    const int g = piece / sets, set = piece - g * sets;
-    const long long p_lo = seq_start + (long long)piece * tiles, p_hi = p_lo + tiles;
-    const int t_lo = int(u - p_lo), t_hi = int(min(hi, p_hi) - p_lo);
-    u = min(hi, p_hi);
+    p.tiles = seq_tiles(p.s);
+    const int piece = int((u - seq_start) / p.tiles), sets = sets_of(p.s);
+    p.g = piece / sets;
+    p.v0 = (piece - p.g * sets) * F::kVec;
+    p.start = seq_start + unsigned(piece) * p.tiles;
+    p.t_lo = int(u - p.start);
+    p.t_hi = int(min(hi - p.start, unsigned(p.tiles)));
+  };
+  // tiles go to the warps in runs of up to kChunk
+  auto run_of = [&](const Part& p) { return min(kChunk, (p.t_hi - p.t_lo + F::kWarps - 1) / F::kWarps); };
+  const int tpp = a.page / kv4::kTile;
+  // page id of this lane's tile of run r (loaded well before its copy)
+  auto page_of = [&](const Part& p, int run, int r) {
+    const int t = p.t_lo + r * run + lane;
+    const int have = (p.s.len + kv4::kTile - 1) / kv4::kTile;  // tiles with tokens
+    return lane < run && t < min(p.t_hi, have)
+               ? a.table[p.seq * a.table_ld + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp)]
+               : -1;
+  };
+  auto fill = [&](const Part& p, int run, int r, int id, uint32_t stage) {  // whole warp
+    const int t = p.t_lo + r * run + lane;
+    const int have = (p.s.len + kv4::kTile - 1) / kv4::kTile;
+    const int n = max(min(min(run, p.t_hi - t + lane), have - t + lane), 0);
+    uint64_t* bar = &s_bar[warp][stage];
+    if (lane == 0) tc::mbar_expect_tx(bar, uint32_t(n) * kv4::tile_bytes(D));
+    __syncwarp();
+    if (lane < n) {
+      if (id < 0 || id >= a.num_pages) {
+        kv4::report(a.err, kv4::kErrPage);
+        id = 0;
+      }
+      const int in = a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp;
+      const uint8_t* src = a.pool + ((uint64_t(uint32_t(id)) * a.Hkv + p.g) * tpp + in) *
+                                        uint64_t(kv4::tile_bytes(D));
+      tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D), src,
+                    kv4::tile_bytes(D), bar);
+    }
+  };
+  // the set's query rows as they are: lane (gid, tig) holds elements 8 tig .. of
+  // each block of vector 8 j + gid
+  auto load_q = [&](const Part& p, uint4 (&x)[kNT][nb]) {
+#pragma unroll
+    for (int j = 0; j < kNT; ++j) {
+      const int v = p.v0 + 8 * j + gid;
+#pragma unroll
+      for (int b = 0; b < nb; ++b) x[j][b] = make_uint4(0u, 0u, 0u, 0u);
+      if (v < p.s.rows * G) {
+        const int r = v / G, h = v - r * G;
+        const E* q = static_cast<const E*>(a.q) + (p.s.row0 + r) * a.q_row + (p.g * G + h) * a.q_head + 8 * tig;
+#pragma unroll
+        for (int b = 0; b < nb; ++b) x[j][b] = q8(q + 32 * b, a.q_vec);
+      }
+    }
+  };
 
-    // ---- the set's query rows as B fragments, scaled to a maximum near 2^15
-    const int v0 = set * F::kVec, nv = s.rows * G;
+  Part p;
+  p.seq = s_first;
+  p.s = sequence(a, p.seq);
+  part_at(p, lo);
+  uint32_t it = 0;  // stages this warp has taken
+  uint4 qx[kNT][nb];
+  {
+    const int run = run_of(p);
+    if (warp * run < p.t_hi - p.t_lo) fill(p, run, warp, page_of(p, run, warp), 0);
+    load_q(p, qx);
+  }
+  for (;;) {
+    const int run = run_of(p), runs = (p.t_hi - p.t_lo + run - 1) / run;
+    int id = warp + F::kWarps < runs ? page_of(p, run, warp + F::kWarps) : -1;
+    // the part after this one, and its first page
+    const unsigned u = p.start + p.t_hi;
+    Part np = p;
+    int nrun = 0, nid = -1;
+    if (u < hi) {
+      part_at(np, u);
+      nrun = run_of(np);
+      if (warp * nrun < np.t_hi - np.t_lo) nid = page_of(np, nrun, warp);
+    }
+
+    // ---- query rows to B fragments, scaled to a maximum near 2^15
+    const Seq& s = p.s;
+    const int nv = s.rows * G;
     uint32_t qf[kNT][D / 16][2];
     float qs[kNT][2];
     int lim[kNT][2];
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
-      const int v = v0 + 8 * j + gid;
-      float x[nb][8], am = 0.0f;
+      float2 x[nb][4];
+      float am = 0.0f;
 #pragma unroll
-      for (int b = 0; b < nb; ++b)
+      for (int b = 0; b < nb; ++b) {
+        x[b][0] = two_floats<E>(qx[j][b].x);
+        x[b][1] = two_floats<E>(qx[j][b].y);
+        x[b][2] = two_floats<E>(qx[j][b].z);
+        x[b][3] = two_floats<E>(qx[j][b].w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[b][i] = 0.0f;
-      if (v < nv) {
-        const int r = v / G, h = v - r * G;
-        const E* q = static_cast<const E*>(a.q) + (s.row0 + r) * a.q_row + (g * G + h) * a.q_head;
-#pragma unroll
-        for (int b = 0; b < nb; ++b) q8(q + 32 * b + 8 * tig, x[b]);
+        for (int i = 0; i < 4; ++i) am = fmaxf(am, fmaxf(fabsf(x[b][i].x), fabsf(x[b][i].y)));
       }
-#pragma unroll
-      for (int b = 0; b < nb; ++b)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) am = fmaxf(am, fabsf(x[b][i]));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
       const int e = max(int(__float_as_uint(am) >> 23) - 127, -100);
@@ -509,19 +637,18 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
       for (int b = 0; b < nb; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          qf[j][2 * b + (i >> 1)][i & 1] = pack_half(x[b][2 * i] * f, x[b][2 * i + 1] * f);
+          qf[j][2 * b + (i >> 1)][i & 1] = pack_half(x[b][i].x * f, x[b][i].y * f);
       // back to the thread's score columns: vectors 2 tig and 2 tig + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int ee = __shfl_sync(0xffffffffu, e, (2 * tig + i) * 4);
         qs[j][i] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + ee) << 23);
-        const int c = v0 + 8 * j + 2 * tig + i;
+        const int c = p.v0 + 8 * j + 2 * tig + i;
         lim[j][i] = c < nv ? s.len - s.rows + c / G + 1 : 0;
       }
     }
-    const int all = s.len - s.rows + v0 / G + 1;
+    const int all = s.len - s.rows + p.v0 / G + 1;
 
-    // ---- tiles of the piece, in runs of up to kChunk, dealt over the warps
     Running<D, kNT> w;
     w.top = 29;  // a block of zeros
 #pragma unroll
@@ -531,53 +658,25 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) w.o[j][k][0] = w.o[j][k][1] = w.o[j][k][2] = w.o[j][k][3] = 0.0f;
     }
-    const int run = min(kChunk, (t_hi - t_lo + F::kWarps - 1) / F::kWarps);
-    const int runs = (t_hi - t_lo + run - 1) / run;
-    const int tpp = a.page / kv4::kTile;
-    const int have = (s.len + kv4::kTile - 1) / kv4::kTile;  // tiles with tokens
-    // page id of this lane's tile of a run (loaded one run ahead of its copy)
-    auto page_of = [&](int r) {
-      const int t = t_lo + r * run + lane;
-      return (r < runs && lane < run && t < min(t_hi, have)) ? a.table[seq * a.table_ld + t / tpp] : -1;
-    };
-    auto fill = [&](int r, int id, uint32_t stage) {  // whole warp; r < runs
-      const int t0 = t_lo + r * run;
-      const int n = max(min(min(run, t_hi - t0), have - t0), 0);
-      uint64_t* bar = &s_bar[warp][stage];
-      if (lane == 0) tc::mbar_expect_tx(bar, uint32_t(n) * kv4::tile_bytes(D));
-      __syncwarp();
-      if (lane < n) {
-        if (id < 0 || id >= a.num_pages) {
-          kv4::report(a.err, kv4::kErrPage);
-          id = 0;
-        }
-        const uint8_t* src = a.pool + ((long long)id * a.Hkv + g) * kv4::head_bytes(D, a.page) +
-                             (long long)((t0 + lane) % tpp) * kv4::tile_bytes(D);
-        tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D), src,
-                      kv4::tile_bytes(D), bar);
-      }
-    };
-    uint32_t filled = it;
-    int next = warp, id = page_of(next);
-    for (int k = 0; k < kStages - 1 && next < runs; ++k, ++filled) {
-      fill(next, id, filled % kStages);
-      next += F::kWarps;
-      id = page_of(next);
-    }
     for (int r = warp; r < runs; r += F::kWarps, ++it) {
-      if (next < runs) {
+      if (r + F::kWarps < runs) {
         __syncwarp();  // the stage's last readers are done
-        fill(next, id, filled % kStages);
-        ++filled;
-        next += F::kWarps;
-        id = page_of(next);
+        fill(p, run, r + F::kWarps, id, (it + 1) % kStages);
+        if (r + 2 * F::kWarps < runs) id = page_of(p, run, r + 2 * F::kWarps);
       }
-      const uint32_t stage = it % kStages;
-      tc::mbar_wait(&s_bar[warp][stage], (it / kStages) & 1u, a.err, 1);
-      const int t0 = t_lo + r * run;
-      const int n = min(min(run, t_hi - t0), have - t0);
-      attend_tiles<D, kNT>(w, ring + stage * F::kStageBytes, n, t0 * kv4::kTile, all, s.len, lim, qs,
-                           qf);
+      tc::mbar_wait(&s_bar[warp][it % kStages], (it / kStages) & 1u, a.err, 1);
+      const int t0 = p.t_lo + r * run;
+      const int n = min(min(run, p.t_hi - t0), (s.len + kv4::kTile - 1) / kv4::kTile - t0);
+      attend_tiles<D, kNT>(w, ring + (it % kStages) * F::kStageBytes, n, t0 * kv4::kTile, all, s.len,
+                           lim, qs, qf);
+    }
+    // the next part's first tiles and rows are on their way during the join; the
+    // sums take the place of the stage read last
+    float* sums = reinterpret_cast<float*>(ring + ((it + 1) % kStages) * F::kStageBytes);
+    if (u < hi) {
+      __syncwarp();
+      if (warp * nrun < np.t_hi - np.t_lo) fill(np, nrun, warp, nid, it % kStages);
+      load_q(np, qx);
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
@@ -585,97 +684,82 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
 #pragma unroll
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int off = 4; off <= 16; off <<= 1)
           w.l[j][i] += __shfl_xor_sync(0xffffffffu, w.l[j][i], off);
-    __syncwarp();
-    float* acc = reinterpret_cast<float*>(ring);
-#pragma unroll
-    for (int j = 0; j < kNT; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float* dst = acc + (8 * j + 2 * tig + i) * F::kAcc;
+        float* dst = sums + (8 * j + 2 * tig + i) * F::kAcc;
 #pragma unroll
         for (int b = 0; b < nb; ++b)
           *reinterpret_cast<float4*>(dst + 32 * b + 4 * gid) =
               make_float4(w.o[j][2 * b][i] * unit, w.o[j][2 * b][i + 2] * unit,
                           w.o[j][2 * b + 1][i] * unit, w.o[j][2 * b + 1][i + 2] * unit);
-        if (gid == 0) {
-          dst[D] = w.m[j][i];
-          dst[D + 1] = w.l[j][i];
-        }
+        if (gid == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(w.m[j][i], w.l[j][i]);
       }
+    if (lane == 0) s_sums[warp] = sums;
     __syncthreads();
-    const bool whole = t_lo == 0 && t_hi == tiles;
-    const int slot = t_lo == 0 ? 1 : 0;
-    float* part = slot_of<D, kNT>(a.part, blockIdx.x, slot);
-    const int busy = min(F::kWarps, runs);  // warps that had a run
-    for (int v = warp; v < F::kVec; v += F::kWarps) {
-      float m = -INFINITY;
-      for (int i = 0; i < busy; ++i)
-        m = fmaxf(m, reinterpret_cast<const float*>(smem + i * F::kWarpBytes)[v * F::kAcc + D]);
-      float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int i = 0; i < busy; ++i) {
-        const float* src = reinterpret_cast<const float*>(smem + i * F::kWarpBytes) + v * F::kAcc;
-        const float c = src[D] == -INFINITY ? 0.0f : ex2(src[D] - m);
-        l = fmaf(c, src[D + 1], l);
-        if (4 * lane < D) {
-          const float4 x = *reinterpret_cast<const float4*>(src + 4 * lane);
+    const bool whole = p.t_lo == 0 && p.t_hi == p.tiles;
+    float* part = slot_of<D, kNT>(a.part, blockIdx.x, p.t_lo == 0 ? 1 : 0);
+    constexpr int kPer = D / 4, kRows = 32 / kPer;
+    const int sub = lane / kPer, d0 = (lane % kPer) * 4;
+    // vectors warp * kRows + sub, .. of the sums that the first `busy` warps left
+    auto join_warps = [&](int busy, bool to_part) {
+      for (int v = warp * kRows + sub; v < F::kVec; v += F::kWarps * kRows) {
+        float m = -INFINITY;
+        for (int i = 0; i < busy; ++i) m = fmaxf(m, s_sums[i][v * F::kAcc + D]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < busy; ++i) {
+          const float* src = s_sums[i] + v * F::kAcc;
+          const float c = ex2(src[D] - ref);
+          const float4 x = *reinterpret_cast<const float4*>(src + d0);
+          l = fmaf(c, src[D + 1], l);
           o[0] = fmaf(c, x.x, o[0]);
           o[1] = fmaf(c, x.y, o[1]);
           o[2] = fmaf(c, x.z, o[2]);
           o[3] = fmaf(c, x.w, o[3]);
         }
+        if (to_part) {
+          *reinterpret_cast<float4*>(part + v * F::kAcc + d0) = make_float4(o[0], o[1], o[2], o[3]);
+          if (d0 == 0) *reinterpret_cast<float2*>(part + v * F::kAcc + D) = make_float2(m, l);
+        } else if (p.v0 + v < nv) {
+          store_vector<E>(a, s, p.g, G, p.v0 + v, d0, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+        }
       }
-      if (whole) {
-        if (v0 + v < nv && 4 * lane < D)
-          store_vector<E>(a, s, g, G, v0 + v, lane, o, l == 0.0f ? 0.0f : 1.0f / l, D);
-      } else {
-        if (4 * lane < D)
-          *reinterpret_cast<float4*>(part + v * F::kAcc + 4 * lane) = make_float4(o[0], o[1], o[2], o[3]);
-        if (lane == 0) *reinterpret_cast<float2*>(part + v * F::kAcc + D) = make_float2(m, l);
-      }
-    }
+    };
+    join_warps(min(F::kWarps, runs), !whole);
     if (!whole) {
-      // the piece's last CTA to arrive joins the parts, in the CTAs' order
-      const int c_first = int(((p_lo + 1) * ctas - 1) / U), c_last = int((p_hi * ctas - 1) / U);
+      // the piece's last CTA to arrive joins the parts, in an order that does not depend on arrival
+      const unsigned c_first = cta_of(p.start), c_last = cta_of(p.start + p.tiles - 1);
       __threadfence();
       __syncthreads();
       if (threadIdx.x == 0)
-        s_last = atomicInc(a.counters + c_first, unsigned(c_last - c_first)) == unsigned(c_last - c_first);
+        s_last = atomicInc(a.counters + c_first, c_last - c_first) == c_last - c_first;
       __syncthreads();
       if (s_last) {
         __threadfence();
-        const int parts = c_last - c_first + 1;
-        for (int v = warp; v < F::kVec && v0 + v < nv; v += F::kWarps) {
-          float m = -INFINITY;
-          for (int i = lane; i < parts; i += 32)
-            m = fmaxf(m, __ldcg(slot_of<D, kNT>(a.part, c_first + i, i == 0) + v * F::kAcc + D));
+        const int parts = int(c_last - c_first) + 1;
+        constexpr int kN = F::kVec / kRows;
+        float m[kN], l[kN];
+        float4 o[kN];
+        join_rows<D, kNT>(warp, F::kWarps, parts,
+                          [&](int i) { return slot_of<D, kNT>(a.part, c_first + i, i == 0); }, m, l, o);
 #pragma unroll
-          for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
-          float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-          for (int i = 0; i < parts; ++i) {
-            const float* src = slot_of<D, kNT>(a.part, c_first + i, i == 0) + v * F::kAcc;
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + D));
-            const float4 x = 4 * lane < D ? __ldcg(reinterpret_cast<const float4*>(src + 4 * lane))
-                                          : make_float4(0.f, 0.f, 0.f, 0.f);
-            const float c = ml.x == -INFINITY ? 0.0f : ex2(ml.x - m);
-            l = fmaf(c, ml.y, l);
-            o[0] = fmaf(c, x.x, o[0]);
-            o[1] = fmaf(c, x.y, o[1]);
-            o[2] = fmaf(c, x.z, o[2]);
-            o[3] = fmaf(c, x.w, o[3]);
-          }
-          if (4 * lane < D)
-            store_vector<E>(a, s, g, G, v0 + v, lane, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+        for (int k = 0; k < kN; ++k) {
+          float* dst = sums + (k * kRows + sub) * F::kAcc;
+          *reinterpret_cast<float4*>(dst + d0) = o[k];
+          if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[k], l[k]);
         }
+        __syncthreads();
+        join_warps(min(F::kWarps, parts), false);
       }
     }
-    __syncthreads();  // the warps' sums are read: their memory takes tiles again
-    // the sums were written by ordinary stores, the next tiles by bulk copies
+    if (u >= hi) break;
+    // the sums are read: their memory, written by ordinary stores, takes tiles
+    // from bulk copies again
     tc::fence_proxy_async_smem();
+    __syncthreads();
+    p = np;
   }
   if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], kStages, it);
 }
@@ -742,6 +826,11 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: the workspace must be 256-byte aligned");
   if (workspace_bytes < mfi_kv4_attn_workspace_bytes(n_seq, Hq, Hkv, D, max_q))
     return mfi::set_last_error(MFI_ERR_WORKSPACE, "workspace smaller than the kv4_attn workspace query");
+  // units of work (a tile of a KV head for 8 vectors, at most) are counted in 31 bits
+  const double units = double(n_seq) * Hkv * (double(width) * page / mfi::kv4::kTile + 1) *
+                       (double(max_q) * (Hq / Hkv) / 8 + 1);
+  if (units >= 2147483648.0)
+    return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: more than 2^31 tiles of work in one call");
   mfi::AttnArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head;
   a.pool = pool; a.table = table; a.table_ld = table_ld;
@@ -750,6 +839,11 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   a.T = T; a.max_q = max_q; a.n_seq = n_seq; a.Hq = Hq; a.Hkv = Hkv;
   a.page = page; a.num_pages = num_pages; a.width = width;
   a.scale = scale;
+  const int tpp = page / mfi::kv4::kTile;
+  a.q_vec = !((reinterpret_cast<uintptr_t>(q) | uintptr_t(q_row * 2) | uintptr_t(q_head * 2)) & 15);
+  a.tpp_shift = -1;
+  for (int i = 0; i < 31; ++i)
+    if (tpp == 1 << i) a.tpp_shift = i;
   a.counters = static_cast<unsigned*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + mfi::kCounterBytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
