@@ -70,26 +70,31 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
 //   the blocks joined by their codes: s = sum_b 2^(c_b - 127) S_b
 //   O^T (D x 8 vectors) += V_b^T . P_b,  P_b = p 2^(c_b - 127)
-// The E2M1 values are exact in fp16 and never multiplied by a scale (the codes
-// go to the few scores and weights), and the query rows are scaled by a power of
-// two to a maximum in [2^14, 2^15), which keeps all bits of a bf16 or fp16 row
-// down to 2^-39 of its maximum.  P_b is rounded to fp16 (2^-12) after a factor
-// 2^(14 - top), top the largest value code so far: it keeps all its bits down to
-// 2^-28 and vanishes below 2^-39 of the largest weight times the largest scale.
-// As top is a whole power of two it changes no other bit of P_b.
-constexpr int kChunk = 4;    // tiles of a pipeline stage
+// The E2M1 values are exact in fp16 and never multiplied by a scale: the codes
+// go to the few scores and weights.  A stage's codes are turned into factors by
+// one lane each and read back from shared memory.
+// * The query rows are scaled by a power of two to a maximum in [2^14, 2^15),
+//   which keeps all bits of a bf16 or fp16 row down to 2^-39 of its maximum.
+// * p is rounded to fp16 (2^-12) after a factor 2^10, and multiplied by 2^(c_b -
+//   top + 4), top the largest value code that the warp has seen: exact but for
+//   products below 2^-28 of the largest weight times the largest scale, which
+//   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
 constexpr int kStages = 2;   // one read, one on its way
 constexpr int kCtas = 148;   // one per SM
+constexpr unsigned kSnap = 32;  // tiles
 
 template <int D, int kNT>
 struct Few {
   static constexpr int kWarps = kNT == 1 ? 12 : 8;
+  static constexpr int kChunk = 4;  // tiles of a pipeline stage
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
   static constexpr int kStageBytes = kChunk * kv4::tile_bytes(D);
   static constexpr int kAcc = D + 4;                          // floats of a vector's sum: D, max, sum, pad
   static_assert(kVec * kAcc * 4 <= kStageBytes, "a warp's sums take the place of a stage");
-  static constexpr int kSmem = kWarps * kStages * kStageBytes;
+  static constexpr int kFactors = kChunk * kv4::kTile * (D / 32) * 6;  // key factors fp32, value factors fp16
+  static constexpr int kWarpBytes = kStages * kStageBytes + kFactors;
+  static constexpr int kSmem = kWarps * kWarpBytes;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -124,10 +129,27 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same with sums that start at zero
+__device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                               uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// all ones in the halves of a that are not zero
+__device__ __forceinline__ uint32_t nonzero_half2(uint32_t a) {
+  return __hne2_mask(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0)));
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -158,9 +180,10 @@ __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
 }
 
-// A warp's state: the running maximum and sum of each vector, and O^T times
-// 2^(127 + 14 - top), top the largest value code plus one so far (a code of 255,
-// NaN, counts as 0; two such neighbours may carry one too many).
+// A warp's state: the running maximum (log2 domain) of each vector, the sum of
+// its weights times 2^10, and O^T times 2^(127 + 15 - top), top the largest
+// value code plus one so far (a code of 255, NaN, counts as 0; two such
+// neighbours may carry one too many).
 template <int D, int kNT>
 struct Running {
   uint32_t top;
@@ -168,100 +191,64 @@ struct Running {
   float o[kNT][D / 16][4];
 };
 
-// One stage: n tiles at `base` (shared memory), the first holding token `pos0`.
-// lim: tokens seen by the thread's vectors; tokens below `all` are seen by all,
-// tokens from `len` on by none (their bytes may be anything).
+// What a warp knows of the thread's vectors: tokens that they see (lim), the
+// power of two and scale that their scores lack (qs > 0), the query fragments.
+// Tokens below `all` are seen by all vectors.
 template <int D, int kNT>
-__device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* base, int n,
-                                             int pos0, int all, int len,
-                                             const int (&lim)[kNT][2],
-                                             const float (&qs)[kNT][2],
-                                             const uint32_t (&qf)[kNT][D / 16][2]) {
+struct Query {
+  int all;
+  int lim[kNT][2];
+  float qs[kNT][2];
+  uint32_t f[kNT][D / 16][2];
+};
+
+// kN tiles at `base` (shared memory), the first holding token `pos0`, of which
+// tokens from `end` on count for nothing (their bytes may be anything);
+// `factors`: this warp's place for their factors.
+template <int D, int kNT, int kN>
+__device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, kNT>& q,
+                                             const uint8_t* base, uint8_t* factors, int pos0,
+                                             int end) {
   constexpr int nb = D / 32;
   const int lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   // row r of the score tile is token (r & 1) * 4 + r / 2 (+ 8): the weights'
   // fragment then pairs tokens t and t + 4, so that the four lanes of a quad
   // read neighbouring value rows
   const int tok = (gid & 1) * 4 + (gid >> 1);
-  float s[kChunk][kNT][4];
+  float* kf = reinterpret_cast<float*>(factors);                          // [tile][token][block]
+  uint32_t* vf = reinterpret_cast<uint32_t*>(factors + Few<D, kNT>::kChunk * kv4::kTile * nb * 4);  // [tile][pair][block]
+
+  // ---- codes to factors.  Keys: one word a lane and turn.  Values: lane (tile,
+  // pair) takes tokens t and t + 4, t = 0-3, 8-11
+  __syncwarp();  // the previous tiles' factors are read
+  {
+    constexpr int kWords = kv4::kTile * nb / 4;  // words of a tile's key codes
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    if (i < n) {
-      const uint8_t* tile = base + i * kv4::tile_bytes(D);
-      uint32_t ka[nb], kb[nb];
-      uint32_t cka, ckb;
-      if (D == 128) {
-        const uint4 a = *reinterpret_cast<const uint4*>(tile + tok * 64 + tig * 16);
-        const uint4 b = *reinterpret_cast<const uint4*>(tile + (tok + 8) * 64 + tig * 16);
-        ka[0] = a.x; ka[1] = a.y; ka[nb - 2] = a.z; ka[nb - 1] = a.w;
-        kb[0] = b.x; kb[1] = b.y; kb[nb - 2] = b.z; kb[nb - 1] = b.w;
-        cka = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4);
-        ckb = *reinterpret_cast<const uint32_t*>(tile + 16 * D + tok * 4 + 32);
-      } else {
-        const uint2 a = *reinterpret_cast<const uint2*>(tile + tok * 32 + tig * 8);
-        const uint2 b = *reinterpret_cast<const uint2*>(tile + (tok + 8) * 32 + tig * 8);
-        ka[0] = a.x; ka[1] = a.y;
-        kb[0] = b.x; kb[1] = b.y;
-        cka = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2);
-        ckb = *reinterpret_cast<const uint16_t*>(tile + 16 * D + tok * 2 + 16);
-      }
-      float fa[nb], fb[nb];
-      codes<nb>(cka, fa);
-      codes<nb>(ckb, fb);
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) s[i][j][0] = s[i][j][1] = s[i][j][2] = s[i][j][3] = 0.0f;
-#pragma unroll
-      for (int b = 0; b < nb; ++b) {
-        uint32_t xa[4], xb[4];
-        e2m1x8(ka[b], xa);
-        e2m1x8(kb[b], xb);
-#pragma unroll
-        for (int j = 0; j < kNT; ++j) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma16816(d, xa[0], xb[0], xa[1], xb[1], qf[j][2 * b][0], qf[j][2 * b][1]);
-          mma16816(d, xa[2], xb[2], xa[3], xb[3], qf[j][2 * b + 1][0], qf[j][2 * b + 1][1]);
-          s[i][j][0] = fmaf(d[0], fa[b], s[i][j][0]);
-          s[i][j][1] = fmaf(d[1], fa[b], s[i][j][1]);
-          s[i][j][2] = fmaf(d[2], fb[b], s[i][j][2]);
-          s[i][j][3] = fmaf(d[3], fb[b], s[i][j][3]);
-        }
-      }
-      const int pa = pos0 + i * kv4::kTile + tok, pb = pa + 8;
-#pragma unroll
-      for (int j = 0; j < kNT; ++j) {
-        s[i][j][0] *= qs[j][0];
-        s[i][j][1] *= qs[j][1];
-        s[i][j][2] *= qs[j][0];
-        s[i][j][3] *= qs[j][1];
-      }
-      if (pos0 + (i + 1) * kv4::kTile > all) {  // a tile with tokens that not all vectors see
-#pragma unroll
-        for (int j = 0; j < kNT; ++j) {
-          if (pa >= lim[j][0]) s[i][j][0] = -INFINITY;
-          if (pa >= lim[j][1]) s[i][j][1] = -INFINITY;
-          if (pb >= lim[j][0]) s[i][j][2] = -INFINITY;
-          if (pb >= lim[j][1]) s[i][j][3] = -INFINITY;
-        }
+    for (int k = 0; k < (kN * kWords + 31) / 32; ++k) {
+      const int i = k * (32 / kWords) + lane / kWords, x = lane % kWords;
+      if (kN * kWords % 32 == 0 || i < kN) {
+        float f[4];
+        codes<4>(*reinterpret_cast<const uint32_t*>(base + i * kv4::tile_bytes(D) + 16 * D + 4 * x), f);
+        *reinterpret_cast<float4*>(kf + (i * kWords + x) * 4) = make_float4(f[0], f[1], f[2], f[3]);
       }
     }
   }
-  // the largest value code of the stage's seen tokens, each word read by one lane
-  uint32_t tops = 0;
-  {
-    constexpr int kPer = 128 / D;               // tokens of a word of codes
-    constexpr int kWords = kv4::kTile / kPer;   // words of a tile
-#pragma unroll
-    for (int k = 0; k < (kChunk * kWords + 31) / 32; ++k) {
-      const int i = k * (32 / kWords) + lane / kWords, x = lane % kWords;
-      const int seen = len - pos0 - i * kv4::kTile - x * kPer;  // of the word's tokens
-      if (i < n && seen > 0) {
-        uint32_t c = *reinterpret_cast<const uint32_t*>(base + i * kv4::tile_bytes(D) + 16 * D +
-                                                        D / 2 + 4 * x);
-        if (kPer == 2 && seen == 1) c &= 0xFFFFu;
-        tops = __vmaxu2(tops, (c + 0x00010001u) & 0x00FF00FFu);
-        tops = __vmaxu2(tops, ((c >> 8) + 0x00010001u) & 0x00FF00FFu);
-      }
+  uint32_t ca = 0, cb = 0, tops = 0;
+  const int ti = lane >> 3, pr = lane & 7, ta = pr < 4 ? pr : pr + 4;
+  if (ti < kN) {
+    const uint8_t* c = base + ti * kv4::tile_bytes(D) + 16 * D + D / 2 + ta * nb;
+    if (nb == 4) {
+      ca = *reinterpret_cast<const uint32_t*>(c);
+      cb = *reinterpret_cast<const uint32_t*>(c + 16);
+    } else {
+      ca = *reinterpret_cast<const uint16_t*>(c);
+      cb = *reinterpret_cast<const uint16_t*>(c + 8);
     }
+    if (pos0 + ti * kv4::kTile + ta >= end) ca = 0;
+    if (pos0 + ti * kv4::kTile + ta + 4 >= end) cb = 0;
+    tops = __vmaxu2((ca + 0x00010001u) & 0x00FF00FFu, ((ca >> 8) + 0x00010001u) & 0x00FF00FFu);
+    tops = __vmaxu2(tops, (cb + 0x00010001u) & 0x00FF00FFu);
+    tops = __vmaxu2(tops, ((cb >> 8) + 0x00010001u) & 0x00FF00FFu);
   }
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xFFFFu, tops >> 16));
   if (top > w.top) {
@@ -277,24 +264,99 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
         w.o[j][k][3] *= c;
       }
   }
-  const float unit = __uint_as_float((127 + 127 + 14 - w.top) << 23);  // 2^(127 + 14 - top)
-  // running maximum of the scores (log2 domain), over the stage's tokens
+  if (ti < kN) {
+    const float u = __uint_as_float((127 + 127 + 5 - w.top) << 23);  // 2^(127 + 5 - top)
+    float fa[nb], fb[nb];
+    codes<nb>(ca, fa);
+    codes<nb>(cb, fb);
+    uint32_t h[nb];
+#pragma unroll
+    for (int b = 0; b < nb; ++b) h[b] = pack_half(fa[b] * u, fb[b] * u);
+    uint32_t* dst = vf + (ti * 8 + pr) * nb;
+    if (nb == 4)
+      *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[nb - 2], h[nb - 1]);
+    else
+      *reinterpret_cast<uint2*>(dst) = make_uint2(h[0], h[1]);
+  }
+  __syncwarp();
+
+  // ---- scores, without qs
+  float s[kN][kNT][4];
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+    const uint8_t* tile = base + i * kv4::tile_bytes(D);
+    uint32_t ka[nb], kb[nb];
+    float fa[nb], fb[nb];
+    if (D == 128) {
+      const uint4 a = *reinterpret_cast<const uint4*>(tile + tok * 64 + tig * 16);
+      const uint4 b = *reinterpret_cast<const uint4*>(tile + (tok + 8) * 64 + tig * 16);
+      ka[0] = a.x; ka[1] = a.y; ka[nb - 2] = a.z; ka[nb - 1] = a.w;
+      kb[0] = b.x; kb[1] = b.y; kb[nb - 2] = b.z; kb[nb - 1] = b.w;
+      const float4 x = *reinterpret_cast<const float4*>(kf + (i * kv4::kTile + tok) * nb);
+      const float4 y = *reinterpret_cast<const float4*>(kf + (i * kv4::kTile + tok + 8) * nb);
+      fa[0] = x.x; fa[1] = x.y; fa[nb - 2] = x.z; fa[nb - 1] = x.w;
+      fb[0] = y.x; fb[1] = y.y; fb[nb - 2] = y.z; fb[nb - 1] = y.w;
+    } else {
+      const uint2 a = *reinterpret_cast<const uint2*>(tile + tok * 32 + tig * 8);
+      const uint2 b = *reinterpret_cast<const uint2*>(tile + (tok + 8) * 32 + tig * 8);
+      ka[0] = a.x; ka[1] = a.y;
+      kb[0] = b.x; kb[1] = b.y;
+      const float2 x = *reinterpret_cast<const float2*>(kf + (i * kv4::kTile + tok) * nb);
+      const float2 y = *reinterpret_cast<const float2*>(kf + (i * kv4::kTile + tok + 8) * nb);
+      fa[0] = x.x; fa[1] = x.y;
+      fb[0] = y.x; fb[1] = y.y;
+    }
+#pragma unroll
+    for (int b = 0; b < nb; ++b) {
+      uint32_t xa[4], xb[4];
+      e2m1x8(ka[b], xa);
+      e2m1x8(kb[b], xb);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        float d[4];
+        mma16816_first(d, xa[0], xb[0], xa[1], xb[1], q.f[j][2 * b][0], q.f[j][2 * b][1]);
+        mma16816(d, xa[2], xb[2], xa[3], xb[3], q.f[j][2 * b + 1][0], q.f[j][2 * b + 1][1]);
+        s[i][j][0] = b ? fmaf(d[0], fa[b], s[i][j][0]) : d[0] * fa[b];
+        s[i][j][1] = b ? fmaf(d[1], fa[b], s[i][j][1]) : d[1] * fa[b];
+        s[i][j][2] = b ? fmaf(d[2], fb[b], s[i][j][2]) : d[2] * fb[b];
+        s[i][j][3] = b ? fmaf(d[3], fb[b], s[i][j][3]) : d[3] * fb[b];
+      }
+    }
+  }
+  const bool edge = pos0 + kN * kv4::kTile > min(q.all, end);  // tokens that not all vectors see
+  if (edge) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int pa = pos0 + i * kv4::kTile + tok, pb = pa + 8;
+#pragma unroll
+      for (int j = 0; j < kNT; ++j) {
+        const int l0 = min(q.lim[j][0], end), l1 = min(q.lim[j][1], end);
+        if (pa >= l0) s[i][j][0] = -INFINITY;
+        if (pa >= l1) s[i][j][1] = -INFINITY;
+        if (pb >= l0) s[i][j][2] = -INFINITY;
+        if (pb >= l1) s[i][j][3] = -INFINITY;
+      }
+    }
+  }
+
+  // ---- running maximum over the tiles' tokens
+  float r0[kNT], r1[kNT];
 #pragma unroll
   for (int j = 0; j < kNT; ++j) {
     float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-      if (i < n) {
-        t0 = fmaxf(t0, fmaxf(s[i][j][0], s[i][j][2]));
-        t1 = fmaxf(t1, fmaxf(s[i][j][1], s[i][j][3]));
-      }
+    for (int i = 0; i < kN; ++i) {
+      t0 = fmaxf(t0, fmaxf(s[i][j][0], s[i][j][2]));
+      t1 = fmaxf(t1, fmaxf(s[i][j][1], s[i][j][3]));
     }
 #pragma unroll
     for (int off = 4; off <= 16; off <<= 1) {
       t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, off));
       t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, off));
     }
-    // the reference moves only when it is passed by more than 1 (P_b <= 2^15)
+    t0 *= q.qs[j][0];
+    t1 *= q.qs[j][1];
+    // the reference moves only when it is passed by more than 1 (p <= 2)
     const bool up0 = t0 > w.m[j][0] + 1.0f, up1 = t1 > w.m[j][1] + 1.0f;
     if (__any_sync(0xffffffffu, up0 || up1)) {
       const float m0 = up0 ? t0 : w.m[j][0], m1 = up1 ? t1 : w.m[j][1];
@@ -311,82 +373,80 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const uint8_t* 
         w.o[j][k][3] *= c1;
       }
     }
+    // a vector that has seen nothing keeps m = -inf; its scores are all -inf too
+    r0[j] = (w.m[j][0] == -INFINITY ? 0.0f : w.m[j][0]) - 10.0f;
+    r1[j] = (w.m[j][1] == -INFINITY ? 0.0f : w.m[j][1]) - 10.0f;
   }
+
+  // ---- weights and values
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    if (i < n) {
-      const uint8_t* tile = base + i * kv4::tile_bytes(D);
-      float fa[nb], fb[nb];
-      {
-        const uint8_t* c = tile + 16 * D + D / 2 + tok * nb;
-        codes<nb>(nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c), fa);
-        c += 8 * nb;
-        codes<nb>(nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c), fb);
+  for (int i = 0; i < kN; ++i) {
+    const uint8_t* tile = base + i * kv4::tile_bytes(D);
+    uint32_t pf[kNT][nb][2];  // weights' fragments: tokens tig, tig + 4 (+ 8) of vector gid
+    {
+      uint32_t ga[nb], gb[nb];
+      const uint32_t* src = vf + (i * 8 + tig) * nb;
+      if (nb == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src), y = *reinterpret_cast<const uint4*>(src + 4 * nb);
+        ga[0] = x.x; ga[1] = x.y; ga[nb - 2] = x.z; ga[nb - 1] = x.w;
+        gb[0] = y.x; gb[1] = y.y; gb[nb - 2] = y.z; gb[nb - 1] = y.w;
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(src), y = *reinterpret_cast<const uint2*>(src + 4 * nb);
+        ga[0] = x.x; ga[1] = x.y;
+        gb[0] = y.x; gb[1] = y.y;
       }
-      uint32_t pf[kNT][nb][2];  // weights' fragments: tokens 2tig, 2tig+1 (+8) of vector gid
 #pragma unroll
       for (int j = 0; j < kNT; ++j) {
-        // a vector that has seen nothing keeps m = -inf; its scores are all -inf too
-        const float r0 = w.m[j][0] == -INFINITY ? 0.0f : w.m[j][0];
-        const float r1 = w.m[j][1] == -INFINITY ? 0.0f : w.m[j][1];
-        float p0 = ex2(s[i][j][0] - r0), p1 = ex2(s[i][j][1] - r1);
-        float p2 = ex2(s[i][j][2] - r0), p3 = ex2(s[i][j][3] - r1);
+        const float p0 = ex2(fmaf(s[i][j][0], q.qs[j][0], -r0[j]));
+        const float p1 = ex2(fmaf(s[i][j][1], q.qs[j][1], -r1[j]));
+        const float p2 = ex2(fmaf(s[i][j][2], q.qs[j][0], -r0[j]));
+        const float p3 = ex2(fmaf(s[i][j][3], q.qs[j][1], -r1[j]));
         w.l[j][0] += p0 + p2;
         w.l[j][1] += p1 + p3;
-        p0 *= unit;
-        p1 *= unit;
-        p2 *= unit;
-        p3 *= unit;
-        if (pos0 + (i + 1) * kv4::kTile > all) {
-          // what a vector does not see may hold anything: codes of 255 make no NaN of its zeros
-#pragma unroll
-          for (int b = 0; b < nb; ++b) {
-            pf[j][b][0] = pack_half(s[i][j][0] == -INFINITY ? 0.0f : p0 * fa[b],
-                                    s[i][j][1] == -INFINITY ? 0.0f : p1 * fa[b]);
-            pf[j][b][1] = pack_half(s[i][j][2] == -INFINITY ? 0.0f : p2 * fb[b],
-                                    s[i][j][3] == -INFINITY ? 0.0f : p3 * fb[b]);
-          }
-        } else {
-#pragma unroll
-          for (int b = 0; b < nb; ++b) {
-            pf[j][b][0] = pack_half(p0 * fa[b], p1 * fa[b]);
-            pf[j][b][1] = pack_half(p2 * fb[b], p3 * fb[b]);
-          }
-        }
+        const uint32_t pa = transpose8x8(pack_half(p0, p1)), pb = transpose8x8(pack_half(p2, p3));
 #pragma unroll
         for (int b = 0; b < nb; ++b) {
-          pf[j][b][0] = transpose8x8(pf[j][b][0]);
-          pf[j][b][1] = transpose8x8(pf[j][b][1]);
+          pf[j][b][0] = mul_half2(pa, ga[b]);
+          pf[j][b][1] = mul_half2(pb, gb[b]);
+        }
+        if (edge) {
+          // a token that a vector does not see makes no NaN of its zero, whatever its code
+          const uint32_t ka = nonzero_half2(pa), kb = nonzero_half2(pb);
+#pragma unroll
+          for (int b = 0; b < nb; ++b) {
+            pf[j][b][0] &= ka;
+            pf[j][b][1] &= kb;
+          }
         }
       }
-      // value rows tig, tig + 4, tig + 8, tig + 12: elements 4 gid .. 4 gid + 3 of each block
-      uint32_t v[4][nb / 2];
+    }
+    // value rows tig, tig + 4, tig + 8, tig + 12: elements 4 gid .. 4 gid + 3 of each block
+    uint32_t v[4][nb / 2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const uint8_t* vr = tile + 8 * D + (tig + 4 * r) * (D / 2) + gid * (2 * nb);
-        if (D == 128) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vr);
-          v[r][0] = x.x;
-          v[r][nb / 2 - 1] = x.y;
-        } else {
-          v[r][0] = *reinterpret_cast<const uint32_t*>(vr);
-        }
+    for (int r = 0; r < 4; ++r) {
+      const uint8_t* vr = tile + 8 * D + (tig + 4 * r) * (D / 2) + gid * (2 * nb);
+      if (D == 128) {
+        const uint2 x = *reinterpret_cast<const uint2*>(vr);
+        v[r][0] = x.x;
+        v[r][nb / 2 - 1] = x.y;
+      } else {
+        v[r][0] = *reinterpret_cast<const uint32_t*>(vr);
       }
+    }
 #pragma unroll
-      for (int h = 0; h < nb / 2; ++h) {  // blocks 2h and 2h + 1
-        constexpr uint32_t kLo = 0x0F0F0F0Fu;
-        uint32_t a0[4], a1[4], a2[4], a3[4];
-        e2m1x8((v[0][h] & kLo) | ((v[1][h] << 4) & ~kLo), a0);  // even elements, tokens t, t + 4
-        e2m1x8(((v[0][h] >> 4) & kLo) | (v[1][h] & ~kLo), a1);  // odd elements
-        e2m1x8((v[2][h] & kLo) | ((v[3][h] << 4) & ~kLo), a2);  // tokens t + 8, t + 12
-        e2m1x8(((v[2][h] >> 4) & kLo) | (v[3][h] & ~kLo), a3);
+    for (int h = 0; h < nb / 2; ++h) {  // blocks 2h and 2h + 1
+      constexpr uint32_t kLo = 0x0F0F0F0Fu;
+      uint32_t a0[4], a1[4], a2[4], a3[4];
+      e2m1x8((v[0][h] & kLo) | ((v[1][h] << 4) & ~kLo), a0);  // even elements, tokens t, t + 4
+      e2m1x8(((v[0][h] >> 4) & kLo) | (v[1][h] & ~kLo), a1);  // odd elements
+      e2m1x8((v[2][h] & kLo) | ((v[3][h] << 4) & ~kLo), a2);  // tokens t + 8, t + 12
+      e2m1x8(((v[2][h] >> 4) & kLo) | (v[3][h] & ~kLo), a3);
 #pragma unroll
-        for (int j = 0; j < kNT; ++j)
+      for (int j = 0; j < kNT; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)  // byte k: block 2h + k / 2, elements 2 (k % 2), + 1
-            mma16816(w.o[j][4 * h + k], a0[k], a1[k], a2[k], a3[k], pf[j][2 * h + (k >> 1)][0],
-                     pf[j][2 * h + (k >> 1)][1]);
-      }
+        for (int k = 0; k < 4; ++k)  // byte k: block 2h + k / 2, elements 2 (k % 2), + 1
+          mma16816(w.o[j][4 * h + k], a0[k], a1[k], a2[k], a3[k], pf[j][2 * h + (k >> 1)][0],
+                   pf[j][2 * h + (k >> 1)][1]);
     }
   }
 }
@@ -425,15 +485,15 @@ __device__ __forceinline__ void join_rows(int first, int step, int count, At at,
     l[k] = 0.0f;
     o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
+#pragma unroll 1
   for (int i = first; i < count; i += step) {
-    const float* src = at(i);
+    const float* src = at(i) + sub * F::kAcc;
     float2 ml[kN];
     float4 x[kN];
 #pragma unroll
     for (int k = 0; k < kN; ++k) {
-      const float* v = src + (k * kRows + sub) * F::kAcc;
-      ml[k] = __ldcg(reinterpret_cast<const float2*>(v + D));
-      x[k] = __ldcg(reinterpret_cast<const float4*>(v + d0));
+      ml[k] = __ldcg(reinterpret_cast<const float2*>(src + k * kRows * F::kAcc + D));
+      x[k] = __ldcg(reinterpret_cast<const float4*>(src + k * kRows * F::kAcc + d0));
     }
 #pragma unroll
     for (int k = 0; k < kN; ++k) {
@@ -464,42 +524,26 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   constexpr int nb = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[F::kWarps][kStages];
-  __shared__ unsigned s_scan[F::kWarps];
-  __shared__ unsigned s_start;  // first unit of sequence s_first
-  __shared__ int s_first, s_last;
+  __shared__ int s_last;
   __shared__ float* s_sums[F::kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int G = a.Hq / a.Hkv;
-  uint8_t* ring = smem + warp * (kStages * F::kStageBytes);
+  uint8_t* ring = smem + warp * F::kWarpBytes;
+  uint8_t* factors = ring + kStages * F::kStageBytes;
   if (threadIdx.x == 0) tc::cta_abort_init();
   if (lane == 0)
     for (int i = 0; i < kStages; ++i) tc::mbar_init(&s_bar[warp][i], 1);
   tc::fence_mbar_init();
 
-  // ---- this CTA's share of the work: each thread sums a run of sequences
+  // ---- this CTA's share of the work: every warp sums the sequences' units, 32
+  // at a time, then finds the sequences that hold the share's ends
   auto sets_of = [&](const Seq& s) { return (s.rows * G + F::kVec - 1) / F::kVec; };
   auto units_of = [&](const Seq& s) { return unsigned(seq_tiles(s)) * a.Hkv * sets_of(s); };
-  const int per = (a.n_seq + F::kThreads - 1) / F::kThreads;
-  const int i0 = min(int(threadIdx.x) * per, a.n_seq), i1 = min(i0 + per, a.n_seq);
-  unsigned mine = 0;
-  for (int i = i0; i < i1; ++i) mine += units_of(sequence(a, i));
-  unsigned inc = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const unsigned x = __shfl_up_sync(0xffffffffu, inc, off);
-    if (lane >= off) inc += x;
-  }
-  if (lane == 31) s_scan[warp] = inc;
-  __syncthreads();
-  unsigned U = 0, before = inc - mine;
-#pragma unroll
-  for (int i = 0; i < F::kWarps; ++i) {
-    if (i < warp) before += s_scan[i];
-    U += s_scan[i];
-  }
+  unsigned U = 0;
+  for (int i = lane; i < a.n_seq; i += 32) U += units_of(sequence(a, i));
+  U = __reduce_add_sync(0xffffffffu, U);
   if (U == 0) return;
-  // one tile a warp at least: more CTAs would only add partial sums to join.
-  // CTA c takes `base` units, one more for c < more.
+  // one tile a warp at least.  CTA c takes `base` units, one more for c < more.
   const unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
   if (blockIdx.x >= ctas) return;
   const unsigned base = U / ctas, more = U - base * ctas;
@@ -508,22 +552,51 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     const unsigned x = more * (base + 1);
     return u < x ? u / (base + 1) : more + (u - x) / base;
   };
-  const unsigned lo = first_unit(blockIdx.x), hi = first_unit(blockIdx.x + 1);
-  if (before <= lo && lo < before + mine) {
-    for (int i = i0; i < i1; ++i) {
-      const unsigned n = units_of(sequence(a, i));
-      if (lo < before + n) {
-        s_first = i;
-        s_start = before;
-        break;
+  // An end within kSnap tiles of an end of its piece moves there: what it would
+  // split off costs less than the join.  A piece of up to 2 kSnap is never split.
+  unsigned lo = first_unit(blockIdx.x), hi = first_unit(blockIdx.x + 1), seq_start = 0;
+  int first_seq = 0;
+  {
+    unsigned before = 0, new_lo = lo, new_hi = hi;
+    for (int i0 = 0; i0 < a.n_seq && before < hi; i0 += 32) {
+      const int i = i0 + lane;
+      const Seq s = i < a.n_seq ? sequence(a, i) : Seq{0, 0, 0};
+      const unsigned n = units_of(s), tiles = seq_tiles(s);
+      unsigned start = n;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const unsigned x = __shfl_up_sync(0xffffffffu, start, off);
+        if (lane >= off) start += x;
       }
-      before += n;
+      const unsigned sum = __shfl_sync(0xffffffffu, start, 31);
+      start += before - n;
+      auto moved = [&](unsigned e) {
+        const unsigned in = (e - start) % tiles, out = tiles - in;
+        if (tiles > 2 * kSnap) return in <= kSnap ? e - in : (out <= kSnap ? e + out : e);
+        return in < out ? e - in : e + out;
+      };
+      const unsigned has_lo = __ballot_sync(0xffffffffu, start <= lo && lo < start + n);
+      const unsigned has_hi = __ballot_sync(0xffffffffu, start <= hi && hi < start + n);
+      if (has_lo) {
+        const int src = __ffs(has_lo) - 1;
+        first_seq = i0 + src;
+        seq_start = __shfl_sync(0xffffffffu, start, src);
+        new_lo = __shfl_sync(0xffffffffu, lane == src ? moved(lo) : 0u, src);
+      }
+      if (has_hi) {
+        const int src = __ffs(has_hi) - 1;
+        new_hi = __shfl_sync(0xffffffffu, lane == src ? moved(hi) : 0u, src);
+      }
+      before += sum;
     }
+    // the last end is U and lies in no sequence
+    lo = new_lo;
+    hi = new_hi;
   }
-  __syncthreads();
+  if (lo >= hi) return;
+  __syncthreads();  // the barriers are initialised
 
   // the part that holds unit u, of a sequence at or after p.seq (which starts at unit seq_start)
-  unsigned seq_start = s_start;
   auto part_at = [&](Part& p, unsigned u) {
     unsigned n = units_of(p.s);
     while (u >= seq_start + n) {
@@ -540,32 +613,31 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     p.t_hi = int(min(hi - p.start, unsigned(p.tiles)));
   };
   // tiles go to the warps in runs of up to kChunk
-  auto run_of = [&](const Part& p) { return min(kChunk, (p.t_hi - p.t_lo + F::kWarps - 1) / F::kWarps); };
+  auto run_of = [&](const Part& p) { return min(F::kChunk, (p.t_hi - p.t_lo + F::kWarps - 1) / F::kWarps); };
+  // the part's end in tiles that hold tokens
+  auto end_of = [&](const Part& p) { return min(p.t_hi, (p.s.len + kv4::kTile - 1) / kv4::kTile); };
   const int tpp = a.page / kv4::kTile;
-  // page id of this lane's tile of run r (loaded well before its copy)
-  auto page_of = [&](const Part& p, int run, int r) {
-    const int t = p.t_lo + r * run + lane;
-    const int have = (p.s.len + kv4::kTile - 1) / kv4::kTile;  // tiles with tokens
-    return lane < run && t < min(p.t_hi, have)
-               ? a.table[p.seq * a.table_ld + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp)]
+  const uint64_t page_bytes = uint64_t(a.Hkv) * tpp * kv4::tile_bytes(D);
+  // page id of this lane's tile t of a run, loaded well before its copy; -1: none
+  auto page_of = [&](const Part& p, int run, int t, int end) {
+    return lane < run && t < end
+               ? __ldg(a.table + p.seq * a.table_ld + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp))
                : -1;
   };
-  auto fill = [&](const Part& p, int run, int r, int id, uint32_t stage) {  // whole warp
-    const int t = p.t_lo + r * run + lane;
-    const int have = (p.s.len + kv4::kTile - 1) / kv4::kTile;
-    const int n = max(min(min(run, p.t_hi - t + lane), have - t + lane), 0);
+  // bring a run's tiles (this lane's: t, on page id) into a stage; whole warp
+  auto fill = [&](const Part& p, int run, int t, int end, int id, uint32_t stage) {
     uint64_t* bar = &s_bar[warp][stage];
-    if (lane == 0) tc::mbar_expect_tx(bar, uint32_t(n) * kv4::tile_bytes(D));
+    if (lane == 0)
+      tc::mbar_expect_tx(bar, uint32_t(max(min(run, end - t), 0)) * kv4::tile_bytes(D));
     __syncwarp();
-    if (lane < n) {
-      if (id < 0 || id >= a.num_pages) {
+    if (lane < run && t < end) {
+      if (unsigned(id) >= unsigned(a.num_pages)) {
         kv4::report(a.err, kv4::kErrPage);
         id = 0;
       }
-      const int in = a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp;
-      const uint8_t* src = a.pool + ((uint64_t(uint32_t(id)) * a.Hkv + p.g) * tpp + in) *
-                                        uint64_t(kv4::tile_bytes(D));
-      tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D), src,
+      const int in = p.g * tpp + (a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp);
+      tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D),
+                    a.pool + unsigned(id) * page_bytes + uint64_t(unsigned(in)) * kv4::tile_bytes(D),
                     kv4::tile_bytes(D), bar);
     }
   };
@@ -579,43 +651,47 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
       for (int b = 0; b < nb; ++b) x[j][b] = make_uint4(0u, 0u, 0u, 0u);
       if (v < p.s.rows * G) {
         const int r = v / G, h = v - r * G;
-        const E* q = static_cast<const E*>(a.q) + (p.s.row0 + r) * a.q_row + (p.g * G + h) * a.q_head + 8 * tig;
+        const E* src = static_cast<const E*>(a.q) + (p.s.row0 + r) * a.q_row +
+                       (p.g * G + h) * a.q_head + 8 * tig;
 #pragma unroll
-        for (int b = 0; b < nb; ++b) x[j][b] = q8(q + 32 * b, a.q_vec);
+        for (int b = 0; b < nb; ++b) x[j][b] = q8(src + 32 * b, a.q_vec);
       }
     }
   };
 
   Part p;
-  p.seq = s_first;
+  p.seq = first_seq;
   p.s = sequence(a, p.seq);
   part_at(p, lo);
   uint32_t it = 0;  // stages this warp has taken
   uint4 qx[kNT][nb];
   {
-    const int run = run_of(p);
-    if (warp * run < p.t_hi - p.t_lo) fill(p, run, warp, page_of(p, run, warp), 0);
+    const int run = run_of(p), t = p.t_lo + warp * run + lane, end = end_of(p);
+    const int id = page_of(p, run, t, end);
+    // the rows before the tiles: they would wait behind them
     load_q(p, qx);
+    if (warp * run < p.t_hi - p.t_lo) fill(p, run, t, end, id, 0);
   }
   for (;;) {
-    const int run = run_of(p), runs = (p.t_hi - p.t_lo + run - 1) / run;
-    int id = warp + F::kWarps < runs ? page_of(p, run, warp + F::kWarps) : -1;
+    const int run = run_of(p), runs = (p.t_hi - p.t_lo + run - 1) / run, t_end = end_of(p);
+    int t = p.t_lo + (warp + F::kWarps) * run + lane;  // this lane's tile of the warp's next run
+    int id = page_of(p, run, t, t_end);
     // the part after this one, and its first page
     const unsigned u = p.start + p.t_hi;
     Part np = p;
-    int nrun = 0, nid = -1;
+    int nrun = 0, nid = -1, nt = 0;
     if (u < hi) {
       part_at(np, u);
       nrun = run_of(np);
-      if (warp * nrun < np.t_hi - np.t_lo) nid = page_of(np, nrun, warp);
+      nt = np.t_lo + warp * nrun + lane;
+      nid = page_of(np, nrun, nt, end_of(np));
     }
 
     // ---- query rows to B fragments, scaled to a maximum near 2^15
     const Seq& s = p.s;
     const int nv = s.rows * G;
-    uint32_t qf[kNT][D / 16][2];
-    float qs[kNT][2];
-    int lim[kNT][2];
+    Query<D, kNT> q;
+    q.all = s.len - s.rows + p.v0 / G + 1;
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
       float2 x[nb][4];
@@ -632,22 +708,24 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
       am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
       const int e = max(int(__float_as_uint(am) >> 23) - 127, -100);
-      const float f = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+      // the rows take the scale's sign; with a scale of zero all scores are zero
+      float f = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+      f = a.scale == 0.0f ? 0.0f : copysignf(f, a.scale);
 #pragma unroll
       for (int b = 0; b < nb; ++b)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          qf[j][2 * b + (i >> 1)][i & 1] = pack_half(x[b][i].x * f, x[b][i].y * f);
+          q.f[j][2 * b + (i >> 1)][i & 1] = pack_half(x[b][i].x * f, x[b][i].y * f);
       // back to the thread's score columns: vectors 2 tig and 2 tig + 1
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int ee = __shfl_sync(0xffffffffu, e, (2 * tig + i) * 4);
-        qs[j][i] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + ee) << 23);
+        q.qs[j][i] = fmaxf(fabsf(a.scale) * 1.44269504088896341f *
+                               __uint_as_float(uint32_t(127 - 14 + ee) << 23), 1e-37f);
         const int c = p.v0 + 8 * j + 2 * tig + i;
-        lim[j][i] = c < nv ? s.len - s.rows + c / G + 1 : 0;
+        q.lim[j][i] = c < nv ? s.len - s.rows + c / G + 1 : 0;
       }
     }
-    const int all = s.len - s.rows + p.v0 / G + 1;
 
     Running<D, kNT> w;
     w.top = 29;  // a block of zeros
@@ -661,26 +739,31 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     for (int r = warp; r < runs; r += F::kWarps, ++it) {
       if (r + F::kWarps < runs) {
         __syncwarp();  // the stage's last readers are done
-        fill(p, run, r + F::kWarps, id, (it + 1) % kStages);
-        if (r + 2 * F::kWarps < runs) id = page_of(p, run, r + 2 * F::kWarps);
+        fill(p, run, t, t_end, id, (it + 1) % kStages);
+        t += F::kWarps * run;
+        id = page_of(p, run, t, t_end);
       }
       tc::mbar_wait(&s_bar[warp][it % kStages], (it / kStages) & 1u, a.err, 1);
       const int t0 = p.t_lo + r * run;
-      const int n = min(min(run, p.t_hi - t0), (s.len + kv4::kTile - 1) / kv4::kTile - t0);
-      attend_tiles<D, kNT>(w, ring + (it % kStages) * F::kStageBytes, n, t0 * kv4::kTile, all, s.len,
-                           lim, qs, qf);
+      const int n = min(run, t_end - t0);
+      const uint8_t* stage = ring + (it % kStages) * F::kStageBytes;
+      const int end = min(s.len, (t0 + n) * kv4::kTile);
+      if (n > 1)
+        attend_tiles<D, kNT, F::kChunk>(w, q, stage, factors, t0 * kv4::kTile, end);
+      else if (n == 1)
+        attend_tiles<D, kNT, 1>(w, q, stage, factors, t0 * kv4::kTile, end);
     }
     // the next part's first tiles and rows are on their way during the join; the
     // sums take the place of the stage read last
     float* sums = reinterpret_cast<float*>(ring + ((it + 1) % kStages) * F::kStageBytes);
     if (u < hi) {
-      __syncwarp();
-      if (warp * nrun < np.t_hi - np.t_lo) fill(np, nrun, warp, nid, it % kStages);
       load_q(np, qx);
+      __syncwarp();
+      if (warp * nrun < np.t_hi - np.t_lo) fill(np, nrun, nt, end_of(np), nid, it % kStages);
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
-    const float unit = __uint_as_float((w.top - 14) << 23);  // 2^(top - 127 - 14)
+    const float unit = __uint_as_float((w.top - 5) << 23);  // 2^(top - 127 - 15 + 10)
 #pragma unroll
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
@@ -705,19 +788,29 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     // vectors warp * kRows + sub, .. of the sums that the first `busy` warps left
     auto join_warps = [&](int busy, bool to_part) {
       for (int v = warp * kRows + sub; v < F::kVec; v += F::kWarps * kRows) {
+        const float* src[F::kWarps];
+        float2 ml[F::kWarps];
         float m = -INFINITY;
-        for (int i = 0; i < busy; ++i) m = fmaxf(m, s_sums[i][v * F::kAcc + D]);
+#pragma unroll
+        for (int i = 0; i < F::kWarps; ++i) src[i] = s_sums[i] + v * F::kAcc;
+#pragma unroll
+        for (int i = 0; i < F::kWarps; ++i) {
+          ml[i] = i < busy ? *reinterpret_cast<const float2*>(src[i] + D) : make_float2(-INFINITY, 0.0f);
+          m = fmaxf(m, ml[i].x);
+        }
         const float ref = m == -INFINITY ? 0.0f : m;
         float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < busy; ++i) {
-          const float* src = s_sums[i] + v * F::kAcc;
-          const float c = ex2(src[D] - ref);
-          const float4 x = *reinterpret_cast<const float4*>(src + d0);
-          l = fmaf(c, src[D + 1], l);
-          o[0] = fmaf(c, x.x, o[0]);
-          o[1] = fmaf(c, x.y, o[1]);
-          o[2] = fmaf(c, x.z, o[2]);
-          o[3] = fmaf(c, x.w, o[3]);
+#pragma unroll
+        for (int i = 0; i < F::kWarps; ++i) {
+          if (i < busy) {
+            const float c = ex2(ml[i].x - ref);
+            const float4 x = *reinterpret_cast<const float4*>(src[i] + d0);
+            l = fmaf(c, ml[i].y, l);
+            o[0] = fmaf(c, x.x, o[0]);
+            o[1] = fmaf(c, x.y, o[1]);
+            o[2] = fmaf(c, x.z, o[2]);
+            o[3] = fmaf(c, x.w, o[3]);
+          }
         }
         if (to_part) {
           *reinterpret_cast<float4*>(part + v * F::kAcc + d0) = make_float4(o[0], o[1], o[2], o[3]);
@@ -730,14 +823,16 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     join_warps(min(F::kWarps, runs), !whole);
     if (!whole) {
       // the piece's last CTA to arrive joins the parts, in an order that does not depend on arrival
-      const unsigned c_first = cta_of(p.start), c_last = cta_of(p.start + p.tiles - 1);
-      __threadfence();
+      const unsigned c_first = cta_of(p.start + kSnap), c_last = cta_of(p.start + p.tiles - kSnap - 1);
       __syncthreads();
-      if (threadIdx.x == 0)
+      if (threadIdx.x == 0) {
+        // release of the CTA's part (ordered before by the barrier), acquire of the others'
+        __threadfence();
         s_last = atomicInc(a.counters + c_first, c_last - c_first) == c_last - c_first;
+        __threadfence();
+      }
       __syncthreads();
       if (s_last) {
-        __threadfence();
         const int parts = int(c_last - c_first) + 1;
         constexpr int kN = F::kVec / kRows;
         float m[kN], l[kN];
