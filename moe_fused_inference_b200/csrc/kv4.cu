@@ -12,15 +12,47 @@
 namespace mfi {
 namespace {
 
+// Where a call's tokens are.
+struct Slots {
+  const long long* slots;       // (T,); negative: none
+  int* err;
+  int capacity;                 // tokens of the pool
+  int T, page, page_shift;      // log2 of the page, -1 if that is no power of two
+};
+
 struct WriteArgs {
   const void* x[2];             // keys, values
   long long row[2], head[2];    // strides in elements (the innermost is 1)
   uint8_t* pool;
-  const long long* slots;       // (T,), negative: skip the row
-  int* err;
-  long long capacity;           // tokens of the pool
-  int T, Hkv, page;
+  Slots s;
 };
+
+struct ReadArgs {
+  const uint8_t* pool;
+  void* y[2];                   // keys, values (T, Hkv, D)
+  Slots s;
+};
+
+// Slot of token t, -1 for none.
+__device__ __forceinline__ int slot_of(const Slots& s, int t) {
+  const long long x = s.slots[t];
+  if (x < 0) return -1;
+  if (x >= s.capacity) {
+    kv4::report(s.err, kv4::kErrSlot);
+    return -1;
+  }
+  return int(x);
+}
+
+// Byte offset in the pool of the tile of (slot, head h of Hkv); row: its row there.
+template <int D>
+__device__ __forceinline__ long long tile_of(const Slots& s, int slot, int h, int Hkv, int& row) {
+  const int pg = s.page_shift >= 0 ? slot >> s.page_shift : slot / s.page;
+  const int in = slot - pg * s.page;
+  row = in % kv4::kTile;
+  return ((long long)pg * Hkv + h) * kv4::head_bytes(D, s.page) +
+         (long long)(in / kv4::kTile) * kv4::tile_bytes(D);
+}
 
 template <class E>
 __device__ __forceinline__ float to_float(E x);
@@ -57,29 +89,9 @@ __device__ __forceinline__ void load8(const E* p, float (&v)[8]) {
   }
 }
 
-__device__ __forceinline__ uint8_t* tile_of(uint8_t* pool, long long slot, int h, int Hkv, int page,
-                                            int D) {
-  const long long pg = slot / page;
-  const int in = int(slot - pg * page);
-  return pool + (pg * Hkv + h) * kv4::head_bytes(D, page) +
-         (long long)(in / kv4::kTile) * kv4::tile_bytes(D);
-}
-
-// One lane per 8 elements (a quad per block): lanes run over the elements,
-// then heads, then key / value, then tokens.
-template <class E, int D, bool kVec>
-__global__ void __launch_bounds__(256) kv4_write_kernel(WriteArgs a) {
-  constexpr int kLanes = D / 8, nb = D / 32;
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  const int w = int(i % kLanes);
-  const long long vec = i / kLanes;  // (token, key / value, head)
-  const int h = int(vec % a.Hkv);
-  const int kv = int(vec / a.Hkv) & 1;
-  const long long tok = vec / a.Hkv / 2;
-  const bool live = tok < a.T;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (live)
-    load8<E, kVec>(static_cast<const E*>(a.x[kv]) + tok * a.row[kv] + h * a.head[kv] + 8 * w, v);
+// The quad of lanes that holds a block (lane t: elements 8t .. 8t+7): the
+// lane's 8 nibbles, and the block's code.
+__device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint8_t& code) {
   float am = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; ++j) am = fmax_nan(am, fabsf(v[j]));
@@ -88,75 +100,86 @@ __global__ void __launch_bounds__(256) kv4_write_kernel(WriteArgs a) {
   const bool finite = am <= 3.402823466e38f;
   const int e = block_exp(am);
   const float inv = __uint_as_float(uint32_t(127 - (finite ? e : 0)) << 23);
+  code = finite ? uint8_t(e + 127) : uint8_t(255);
   uint32_t word = 0;
-  if (finite) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)  // the sign of v, not of the scaled value: that may underflow
-      word |= (e2m1_mag(__fmul_rn(v[j], inv)) | (v[j] < 0.0f ? 8u : 0u)) << (4 * j);
-  }
-  if (!live) return;
-  const long long slot = a.slots[tok];
-  if (slot < 0) return;
-  if (slot >= a.capacity) {
-    kv4::report(a.err, kv4::kErrSlot);
-    return;
-  }
-  uint8_t* tile = tile_of(a.pool, slot, h, a.Hkv, a.page, D);
-  const int r = int(slot % kv4::kTile);
-  const int b = w >> 2, t = w & 3;
-  uint8_t* rowp = tile + kv * 8 * D + r * (D / 2);
-  if (kv == 0) {
-    *reinterpret_cast<uint32_t*>(rowp + (t * nb + b) * 4) = word;
-  } else {
-    *reinterpret_cast<uint16_t*>(rowp + ((2 * t) * nb + b) * 2) = uint16_t(word);
-    *reinterpret_cast<uint16_t*>(rowp + ((2 * t + 1) * nb + b) * 2) = uint16_t(word >> 16);
-  }
-  if (t == 0) tile[16 * D + kv * (D / 2) + r * nb + b] = finite ? uint8_t(e + 127) : uint8_t(255);
+  for (int j = 0; j < 8; ++j)  // the sign of v, not of the scaled value: that may underflow
+    word |= (e2m1_mag(__fmul_rn(v[j], inv)) | (v[j] < 0.0f ? 8u : 0u)) << (4 * j);
+  return finite ? word : 0u;
 }
 
-struct ReadArgs {
-  const uint8_t* pool;
-  const long long* slots;
-  void* y[2];                   // keys, values (T, Hkv, D)
-  int* err;
-  long long capacity;
-  int T, Hkv, page;
-};
+// kThreads / (D/8) tokens of one KV head a block: D/8 lanes a token, a quad a
+// block of 32 elements, each lane 8 elements of the key and of the value.  The
+// tokens of a tile are neighbours in memory: a warp writes whole 32-byte
+// sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53 written an element.
+constexpr int kRwThreads = 256;
 
-template <class E, int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(ReadArgs a) {
+template <class E, int D, bool kVec>
+__global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;
-  const long long i = blockIdx.x * 256LL + threadIdx.x;
-  const int w = int(i % kLanes);
-  const long long vec = i / kLanes;
-  const int h = int(vec % a.Hkv);
-  const int kv = int(vec / a.Hkv) & 1;
-  const long long tok = vec / a.Hkv / 2;
-  if (tok >= a.T) return;
-  const long long slot = a.slots[tok];
-  uint32_t word = 0;
-  float s = 1.0f;
-  if (slot >= a.capacity) kv4::report(a.err, kv4::kErrSlot);
-  if (slot >= 0 && slot < a.capacity) {
-    const uint8_t* tile =
-        tile_of(const_cast<uint8_t*>(a.pool), slot, h, a.Hkv, a.page, D);
-    const int r = int(slot % kv4::kTile);
-    const int b = w >> 2, t = w & 3;
-    const uint8_t* rowp = tile + kv * 8 * D + r * (D / 2);
-    if (kv == 0)
-      word = *reinterpret_cast<const uint32_t*>(rowp + (t * nb + b) * 4);
-    else
-      word = uint32_t(*reinterpret_cast<const uint16_t*>(rowp + ((2 * t) * nb + b) * 2)) |
-             uint32_t(*reinterpret_cast<const uint16_t*>(rowp + ((2 * t + 1) * nb + b) * 2)) << 16;
-    s = kv4::code_value(tile[16 * D + kv * (D / 2) + r * nb + b]);
+  const int t = blockIdx.x * (kRwThreads / kLanes) + threadIdx.x / kLanes;
+  const int w = threadIdx.x % kLanes, h = blockIdx.y, Hkv = gridDim.y;
+  float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  int slot = -1;
+  if (t < a.s.T) {
+    slot = slot_of(a.s, t);
+    load8<E, kVec>(static_cast<const E*>(a.x[0]) + t * a.row[0] + h * a.head[0] + 8 * w, k);
+    load8<E, kVec>(static_cast<const E*>(a.x[1]) + t * a.row[1] + h * a.head[1] + 8 * w, v);
   }
+  uint8_t kc, vc;
+  const uint32_t kw = quantise8(k, kc), vw = quantise8(v, vc);
+  // value pieces 2t, 2t+1 of blocks b and b ^ 1 make two words of the row: the
+  // lane of the even block writes the one of pieces 2t, the odd block's 2t+1
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
+  if (slot < 0) return;
+  int r;
+  uint8_t* tile = a.pool + tile_of<D>(a.s, slot, h, Hkv, r);
+  const int b = w >> 2, q = w & 3;
+  *reinterpret_cast<uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4) = kw;
+  const uint32_t word = (b & 1) ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
+  const int piece = 2 * q + (b & 1);
+  *reinterpret_cast<uint32_t*>(tile + 8 * D + r * (D / 2) + (piece * nb + (b & ~1)) * 2) = word;
+  if (q == 0) {
+    tile[16 * D + r * nb + b] = kc;
+    tile[16 * D + D / 2 + r * nb + b] = vc;
+  }
+}
+
+// 8 nibbles times a block's scale, rounded once.
+template <class E>
+__device__ __forceinline__ void store8(E* p, uint32_t w, float s) {
   __align__(16) E out[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) out[j] = from_float<E>(kv4::nibble_value(word >> (4 * j)) * s);
-  E* y = static_cast<E*>(a.y[kv]) + (tok * a.Hkv + h) * D + 8 * w;
+  for (int j = 0; j < 8; ++j) out[j] = from_float<E>(kv4::nibble_value(w >> (4 * j)) * s);
 #pragma unroll
   for (int j = 0; j < int(sizeof(out) / 16); ++j)
-    reinterpret_cast<uint4*>(y)[j] = reinterpret_cast<const uint4*>(out)[j];
+    reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(out)[j];
+}
+
+// The write's shape, the other way round: 0.53 bytes read and 2 written (bf16) an element.
+template <class E, int D>
+__global__ void __launch_bounds__(kRwThreads) kv4_read_kernel(ReadArgs a) {
+  constexpr int kLanes = D / 8, nb = D / 32;
+  const int t = blockIdx.x * (kRwThreads / kLanes) + threadIdx.x / kLanes;
+  const int w = threadIdx.x % kLanes, h = blockIdx.y, Hkv = gridDim.y;
+  if (t >= a.s.T) return;
+  const int slot = slot_of(a.s, t);
+  uint32_t kw = 0, vw = 0;
+  float ks = 1.0f, vs = 1.0f;
+  if (slot >= 0) {
+    int r;
+    const uint8_t* tile = a.pool + tile_of<D>(a.s, slot, h, Hkv, r);
+    const int b = w >> 2, q = w & 3;
+    const uint8_t* vr = tile + 8 * D + r * (D / 2);
+    kw = __ldg(reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4));
+    vw = uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + (2 * q * nb + b) * 2))) |
+         uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + ((2 * q + 1) * nb + b) * 2))) << 16;
+    ks = kv4::code_value(__ldg(tile + 16 * D + r * nb + b));
+    vs = kv4::code_value(__ldg(tile + 16 * D + D / 2 + r * nb + b));
+  }
+  const long long at = ((long long)t * Hkv + h) * D + 8 * w;
+  store8(static_cast<E*>(a.y[0]) + at, kw, ks);
+  store8(static_cast<E*>(a.y[1]) + at, vw, vs);
 }
 
 int check_pool(const void* pool, int Hkv, int D, int page, int num_pages) {
@@ -165,6 +188,8 @@ int check_pool(const void* pool, int Hkv, int D, int page, int num_pages) {
   if (page <= 0 || page % kv4::kTile != 0)
     return set_last_error(MFI_ERR_ARG, "kv4: the page must be a positive multiple of 16 tokens");
   if (num_pages <= 0) return set_last_error(MFI_ERR_ARG, "kv4: the pool has no pages");
+  if ((long long)num_pages * page > 0x7FFFFFFFLL)
+    return set_last_error(MFI_ERR_ARG, "kv4: the pool has more than 2^31 - 1 tokens");
   if (!pool) return set_last_error(MFI_ERR_ARG, "null pointer");
   if (reinterpret_cast<uintptr_t>(pool) & 15)
     return set_last_error(MFI_ERR_ARG, "kv4: the pool must be 16-byte aligned");
@@ -177,20 +202,38 @@ int launched(const char*) {
 }
 
 template <class E>
-void launch_write(const WriteArgs& a, int D, bool vec, unsigned blocks, cudaStream_t s) {
+void launch_write(const WriteArgs& a, int D, bool vec, dim3 grid, cudaStream_t s) {
   if (D == 128) {
-    if (vec) kv4_write_kernel<E, 128, true><<<blocks, 256, 0, s>>>(a);
-    else kv4_write_kernel<E, 128, false><<<blocks, 256, 0, s>>>(a);
+    if (vec) kv4_write_kernel<E, 128, true><<<grid, kRwThreads, 0, s>>>(a);
+    else kv4_write_kernel<E, 128, false><<<grid, kRwThreads, 0, s>>>(a);
   } else {
-    if (vec) kv4_write_kernel<E, 64, true><<<blocks, 256, 0, s>>>(a);
-    else kv4_write_kernel<E, 64, false><<<blocks, 256, 0, s>>>(a);
+    if (vec) kv4_write_kernel<E, 64, true><<<grid, kRwThreads, 0, s>>>(a);
+    else kv4_write_kernel<E, 64, false><<<grid, kRwThreads, 0, s>>>(a);
   }
 }
 
 template <class E>
-void launch_read(const ReadArgs& a, int D, unsigned blocks, cudaStream_t s) {
-  if (D == 128) kv4_read_kernel<E, 128><<<blocks, 256, 0, s>>>(a);
-  else kv4_read_kernel<E, 64><<<blocks, 256, 0, s>>>(a);
+void launch_read(const ReadArgs& a, int D, dim3 grid, cudaStream_t s) {
+  if (D == 128) kv4_read_kernel<E, 128><<<grid, kRwThreads, 0, s>>>(a);
+  else kv4_read_kernel<E, 64><<<grid, kRwThreads, 0, s>>>(a);
+}
+
+Slots make_slots(const int64_t* slots, int T, int page, int num_pages) {
+  Slots s{};
+  s.slots = reinterpret_cast<const long long*>(slots);
+  s.err = device_error_flag();
+  s.capacity = num_pages * page;
+  s.T = T;
+  s.page = page;
+  s.page_shift = -1;
+  for (int i = 4; i < 31; ++i)
+    if (page == 1 << i) s.page_shift = i;
+  return s;
+}
+
+dim3 rw_grid(int T, int Hkv, int D) {
+  const int per = kRwThreads / (D / 8);
+  return dim3(unsigned((T + per - 1) / per), unsigned(Hkv));
 }
 
 }  // namespace
@@ -223,23 +266,18 @@ extern "C" int mfi_kv4_write(const void* k, long long k_row, long long k_head, c
   a.row[0] = k_row; a.row[1] = v_row;
   a.head[0] = k_head; a.head[1] = v_head;
   a.pool = pool;
-  a.slots = reinterpret_cast<const long long*>(slots);
-  a.err = mfi::device_error_flag();
-  a.capacity = (long long)num_pages * page;
-  a.T = T; a.Hkv = Hkv; a.page = page;
+  a.s = mfi::make_slots(slots, T, page, num_pages);
   // 16-byte loads where every vector starts on a 16-byte boundary
   const int size = dtype == MFI_F32 ? 4 : 2;
   bool vec = true;
   for (int i = 0; i < 2; ++i)
     vec = vec && !((reinterpret_cast<uintptr_t>(a.x[i]) | uintptr_t(a.row[i] * size) |
                     uintptr_t(a.head[i] * size)) & 15);
-  const long long lanes = (long long)T * 2 * Hkv * (D / 8);
-  const long long blocks = (lanes + 255) / 256;
-  if (blocks > 0x7FFFFFFFLL) return mfi::set_last_error(MFI_ERR_ARG, "kv4_write: too many rows");
+  const dim3 grid = mfi::rw_grid(T, Hkv, D);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == MFI_F32) mfi::launch_write<float>(a, D, vec, unsigned(blocks), s);
-  else if (dtype == MFI_F16) mfi::launch_write<__half>(a, D, vec, unsigned(blocks), s);
-  else mfi::launch_write<__nv_bfloat16>(a, D, vec, unsigned(blocks), s);
+  if (dtype == MFI_F32) mfi::launch_write<float>(a, D, vec, grid, s);
+  else if (dtype == MFI_F16) mfi::launch_write<__half>(a, D, vec, grid, s);
+  else mfi::launch_write<__nv_bfloat16>(a, D, vec, grid, s);
   return mfi::launched("kv4_write");
 }
 
@@ -256,17 +294,12 @@ extern "C" int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, 
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: k and v must be 16-byte aligned");
   mfi::ReadArgs a{};
   a.pool = pool;
-  a.slots = reinterpret_cast<const long long*>(slots);
   a.y[0] = k; a.y[1] = v;
-  a.err = mfi::device_error_flag();
-  a.capacity = (long long)num_pages * page;
-  a.T = T; a.Hkv = Hkv; a.page = page;
-  const long long lanes = (long long)T * 2 * Hkv * (D / 8);
-  const long long blocks = (lanes + 255) / 256;
-  if (blocks > 0x7FFFFFFFLL) return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: too many rows");
+  a.s = mfi::make_slots(slots, T, page, num_pages);
+  const dim3 grid = mfi::rw_grid(T, Hkv, D);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == MFI_F32) mfi::launch_read<float>(a, D, unsigned(blocks), s);
-  else if (dtype == MFI_F16) mfi::launch_read<__half>(a, D, unsigned(blocks), s);
-  else mfi::launch_read<__nv_bfloat16>(a, D, unsigned(blocks), s);
+  if (dtype == MFI_F32) mfi::launch_read<float>(a, D, grid, s);
+  else if (dtype == MFI_F16) mfi::launch_read<__half>(a, D, grid, s);
+  else mfi::launch_read<__nv_bfloat16>(a, D, grid, s);
   return mfi::launched("kv4_read");
 }

@@ -18,7 +18,6 @@ buffer (runtime/model_runner_v2.py:39, src/ext/mxfp4_decode.cu:352-490).
 
 from __future__ import annotations
 
-import math
 from typing import Optional
 
 import torch
@@ -28,6 +27,7 @@ from . import _lib
 __all__ = ["KV4Cache", "kv4_write", "kv4_read", "kv4_attention", "attention_workspace"]
 
 _DT = {torch.float32: _lib.MFI_F32, torch.float16: _lib.MFI_F16, torch.bfloat16: _lib.MFI_BF16}
+_QT = (torch.bfloat16, torch.float16)
 TILE = 16
 
 
@@ -36,8 +36,10 @@ def _check(cond: bool, msg: str) -> None:
         raise RuntimeError(msg)
 
 
-def _stream(dev) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+def _stream(index: int) -> int:
+    """The current stream of a device, without making a Stream object (these
+    calls are a few microseconds of host time in all, 2 of them for that)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class KV4Cache:
@@ -65,6 +67,8 @@ class KV4Cache:
 
     def _set(self, data):
         self.data = data
+        self.device = data.device
+        self.vector = (data.shape[1], data.shape[3] // 17)   # of a token: heads, elements
         self.num_pages, self.kv_heads = data.shape[0], data.shape[1]
         self.page, self.head_dim = data.shape[2] * TILE, data.shape[3] // 17
 
@@ -75,10 +79,9 @@ class KV4Cache:
 
 
 def _check_slots(slots, T, cache):
-    _check(slots.is_cuda and slots.device == cache.data.device and slots.dtype == torch.int64
+    _check(slots.is_cuda and slots.device == cache.device and slots.dtype == torch.int64
            and slots.dim() == 1, "slots must be a 1-D int64 tensor on the cache's device")
     _check(slots.shape[0] == T, "slots must have one entry per token")
-    return slots.contiguous()
 
 
 def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
@@ -89,25 +92,34 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
     and heads may have any stride, elements are contiguous.  A block with a
     value that is not finite reads back as NaN."""
     lib = _lib.load()
-    _check(k.is_cuda and v.is_cuda and cache.data.is_cuda, "tensors must be cuda")
-    _check(k.device == cache.data.device and v.device == cache.data.device,
-           "k and v must be on the cache's device")
-    _check(k.dtype in _DT and v.dtype == k.dtype, "k and v must both be bfloat16, float16 or float32")
-    _check(k.dim() == 3 and v.shape == k.shape and
-           k.shape[1:] == (cache.kv_heads, cache.head_dim),
-           "k and v must be (T, kv_heads, head_dim) of the cache")
-    T = k.shape[0]
-    slots = _check_slots(slots, T, cache)
+    dev, shape = cache.device, k.shape
+    if not (k.is_cuda and k.device == dev and v.device == dev and slots.device == dev
+            and k.dtype in _DT and v.dtype == k.dtype and len(shape) == 3 and v.shape == shape
+            and shape[1:] == cache.vector and slots.dtype == torch.int64
+            and slots.shape == shape[:1]):
+        _check(k.is_cuda and v.is_cuda and cache.data.is_cuda, "tensors must be cuda")
+        _check(k.device == dev and v.device == dev, "k and v must be on the cache's device")
+        _check(k.dtype in _DT and v.dtype == k.dtype, "k and v must both be bfloat16, float16 or float32")
+        _check(len(shape) == 3 and v.shape == shape and shape[1:] == cache.vector,
+               "k and v must be (T, kv_heads, head_dim) of the cache")
+        _check_slots(slots, shape[0], cache)
+    T = shape[0]
     if T == 0:
         return
-    if k.stride(2) != 1:
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1:
         k = k.contiguous()
-    if v.stride(2) != 1:
+        ks = k.stride()
+    if vs[2] != 1:
         v = v.contiguous()
-    _lib.check(lib.mfi_kv4_write(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        _DT[k.dtype], cache.data.data_ptr(), slots.data_ptr(), T, cache.kv_heads, cache.head_dim,
-        cache.page, cache.num_pages, _stream(k.device)), "kv4_write")
+        vs = v.stride()
+    if not slots.is_contiguous():
+        slots = slots.contiguous()
+    st = lib.mfi_kv4_write(
+        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _DT[k.dtype],
+        cache.data.data_ptr(), slots.data_ptr(), T, cache.kv_heads, cache.head_dim, cache.page,
+        cache.num_pages, _stream(dev.index))
+    _lib.check(st, "kv4_write")
 
 
 def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bfloat16):
@@ -116,17 +128,23 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bf
     negative slot gives zeros; so does one past the pool, which is reported
     through the device error flag."""
     lib = _lib.load()
-    _check(cache.data.is_cuda, "tensors must be cuda")
-    _check(dtype in _DT, "dtype must be bfloat16, float16 or float32")
-    T = slots.shape[0] if slots.dim() == 1 else -1
-    slots = _check_slots(slots, T, cache)
-    out = torch.empty((2, T, cache.kv_heads, cache.head_dim), dtype=dtype, device=slots.device)
+    dev = cache.device
+    if not (slots.is_cuda and slots.device == dev and slots.dtype == torch.int64
+            and slots.dim() == 1 and dtype in _DT):
+        _check(cache.data.is_cuda, "tensors must be cuda")
+        _check(dtype in _DT, "dtype must be bfloat16, float16 or float32")
+        _check_slots(slots, slots.shape[0] if slots.dim() else 0, cache)
+    T = slots.shape[0]
+    out = slots.new_empty((2, T, *cache.vector), dtype=dtype)
     if T:
-        _lib.check(lib.mfi_kv4_read(
-            cache.data.data_ptr(), slots.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
-            _DT[dtype], T, cache.kv_heads, cache.head_dim, cache.page, cache.num_pages,
-            _stream(slots.device)), "kv4_read")
-    return out[0], out[1]
+        if not slots.is_contiguous():
+            slots = slots.contiguous()
+        k = out.data_ptr()
+        st = lib.mfi_kv4_read(
+            cache.data.data_ptr(), slots.data_ptr(), k, k + out.nbytes // 2, _DT[dtype], T,
+            cache.kv_heads, cache.head_dim, cache.page, cache.num_pages, _stream(dev.index))
+        _lib.check(st, "kv4_read")
+    return out.unbind(0)
 
 
 def attention_workspace(num_seqs: int, heads: int, cache: KV4Cache, max_q: int = 1) -> torch.Tensor:
@@ -139,7 +157,7 @@ def attention_workspace(num_seqs: int, heads: int, cache: KV4Cache, max_q: int =
     _check(n > 0, "num_seqs and max_q must be positive and heads a positive multiple of kv_heads")
     dev = cache.data.device
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _lib.check(lib.mfi_kv4_attn_init_workspace(ws.data_ptr(), n, _stream(dev)),
+    _lib.check(lib.mfi_kv4_attn_init_workspace(ws.data_ptr(), n, _stream(ws.device.index)),
                "kv4_attn_init_workspace")
     return ws
 
@@ -165,50 +183,60 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
     as page 0, cut to the table, or left out).  ``workspace``: from
     ``attention_workspace``; made for this call if not given."""
     lib = _lib.load()
-    _check(q.is_cuda and cache.data.is_cuda and page_table.is_cuda and kv_lens.is_cuda,
-           "tensors must be cuda")
-    dev = q.device
-    _check(cache.data.device == dev and page_table.device == dev and kv_lens.device == dev,
-           "tensors must be on one device")
-    _check(q.dtype in (torch.bfloat16, torch.float16), "q must be bfloat16 or float16")
-    _check(q.dim() == 3 and q.shape[2] == cache.head_dim, "q must be (T, heads, head_dim) of the cache")
-    T, heads, D = q.shape
-    _check(heads > 0 and heads % cache.kv_heads == 0, "heads must be a positive multiple of kv_heads")
-    _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 (n, pages)")
+    dev, shape = cache.device, q.shape
+    if not (q.is_cuda and q.device == dev and page_table.device == dev and kv_lens.device == dev
+            and q.dtype in _QT and len(shape) == 3 and shape[2] == cache.head_dim
+            and shape[1] > 0 and shape[1] % cache.kv_heads == 0 and page_table.dtype == torch.int32
+            and page_table.dim() == 2 and kv_lens.dtype == torch.int32
+            and kv_lens.shape == page_table.shape[:1]):
+        _check(q.is_cuda and cache.data.is_cuda and page_table.is_cuda and kv_lens.is_cuda,
+               "tensors must be cuda")
+        _check(q.device == dev and page_table.device == dev and kv_lens.device == dev,
+               "tensors must be on one device")
+        _check(q.dtype in _QT, "q must be bfloat16 or float16")
+        _check(len(shape) == 3 and shape[2] == cache.head_dim, "q must be (T, heads, head_dim) of the cache")
+        _check(shape[1] > 0 and shape[1] % cache.kv_heads == 0,
+               "heads must be a positive multiple of kv_heads")
+        _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 (n, pages)")
+        _check(False, "kv_lens must be int32 (n,)")
+    T, heads, D = shape
     n, width = page_table.shape
-    _check(kv_lens.dtype == torch.int32 and kv_lens.shape == (n,), "kv_lens must be int32 (n,)")
     if cu_q is None:
         _check(T % n == 0 if n else T == 0, "without cu_q every sequence has the same count of rows")
         max_q = T // n if n else 0
     else:
         _check(cu_q.device == dev and cu_q.dtype == torch.int32 and cu_q.shape == (n + 1,),
                "cu_q must be int32 (n + 1,) on q's device")
-        cu_q = cu_q.contiguous()
+        if not cu_q.is_contiguous():
+            cu_q = cu_q.contiguous()
         max_q = T if max_q is None else min(int(max_q), T)
         _check(max_q >= 0, "max_q must not be negative")
     if out is None:
-        out = torch.empty((T, heads, D), dtype=q.dtype, device=dev)
+        out = q.new_empty(shape)
     else:
-        _check(out.shape == q.shape and out.dtype == q.dtype and out.device == dev
+        _check(out.shape == shape and out.dtype == q.dtype and out.device == dev
                and out.is_contiguous(), "out must be a contiguous tensor of q's shape, type and device")
     if T == 0 or n == 0 or max_q == 0:
         return out
-    if q.stride(2) != 1:
+    qs = q.stride()
+    if qs[2] != 1:
         q = q.contiguous()
+        qs = q.stride()
     if page_table.stride(1) != 1:
         page_table = page_table.contiguous()
-    kv_lens = kv_lens.contiguous()
+    if not kv_lens.is_contiguous():
+        kv_lens = kv_lens.contiguous()
     if workspace is None:
         workspace = attention_workspace(n, heads, cache, max_q)
     else:
-        _check(workspace.is_cuda and workspace.device == dev and workspace.dtype == torch.uint8
+        _check(workspace.device == dev and workspace.dtype == torch.uint8
                and workspace.is_contiguous(), "workspace must be a uint8 tensor on q's device")
     if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    _lib.check(lib.mfi_kv4_attn(
-        q.data_ptr(), _DT[q.dtype], q.stride(0), q.stride(1), cache.data.data_ptr(),
-        page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(),
-        0 if cu_q is None else cu_q.data_ptr(), out.data_ptr(), T, max_q, n, heads, cache.kv_heads,
-        D, cache.page, cache.num_pages, width, float(scale), workspace.data_ptr(),
-        workspace.numel(), _stream(dev)), "kv4_attn")
+        scale = D ** -0.5
+    st = lib.mfi_kv4_attn(
+        q.data_ptr(), _DT[q.dtype], qs[0], qs[1], cache.data.data_ptr(), page_table.data_ptr(),
+        page_table.stride(0), kv_lens.data_ptr(), 0 if cu_q is None else cu_q.data_ptr(),
+        out.data_ptr(), T, max_q, n, heads, cache.kv_heads, D, cache.page, cache.num_pages, width,
+        scale, workspace.data_ptr(), workspace.numel(), _stream(dev.index))
+    _lib.check(st, "kv4_attn")
     return out
