@@ -17,7 +17,8 @@ struct Slots {
   const long long* slots;       // (T,); negative: none
   int* err;
   int capacity;                 // tokens of the pool
-  int T, page, page_shift;      // log2 of the page, -1 if that is no power of two
+  int T, Hkv, page;
+  int page_shift;               // log2 of the page, -1 if that is no power of two
 };
 
 struct WriteArgs {
@@ -108,17 +109,20 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint8_t& code
   return finite ? word : 0u;
 }
 
-// kThreads / (D/8) tokens of one KV head a block: D/8 lanes a token, a quad a
-// block of 32 elements, each lane 8 elements of the key and of the value.  The
-// tokens of a tile are neighbours in memory: a warp writes whole 32-byte
-// sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53 written an element.
-constexpr int kRwThreads = 256;
+// A block takes kRwThreads / (D/8) tokens of one KV head, its neighbours the other
+// heads of the same tokens, so that the rows (T, Hkv, D) are met in order: D/8
+// lanes a token, a quad a block of 32 elements, each lane 8 elements of the key
+// and of the value.  The tokens of a tile are neighbours in memory: a warp
+// writes whole 32-byte sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53
+// written an element.  More tokens a thread cost more than they hide (2 of them:
+// 16384 tokens 30 -> 33 us with their read-back, 1021 fp32 tokens 4.9 -> 8.5 us).
+constexpr int kRwThreads = 128;
 
 template <class E, int D, bool kVec>
 __global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;
-  const int t = blockIdx.x * (kRwThreads / kLanes) + threadIdx.x / kLanes;
-  const int w = threadIdx.x % kLanes, h = blockIdx.y, Hkv = gridDim.y;
+  const int Hkv = a.s.Hkv, run = blockIdx.x / Hkv, h = blockIdx.x - run * Hkv;
+  const int t = run * (kRwThreads / kLanes) + threadIdx.x / kLanes, w = threadIdx.x % kLanes;
   float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   int slot = -1;
   if (t < a.s.T) {
@@ -128,8 +132,8 @@ __global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
   }
   uint8_t kc, vc;
   const uint32_t kw = quantise8(k, kc), vw = quantise8(v, vc);
-  // value pieces 2t, 2t+1 of blocks b and b ^ 1 make two words of the row: the
-  // lane of the even block writes the one of pieces 2t, the odd block's 2t+1
+  // value pieces 2q, 2q+1 of blocks b and b ^ 1 make two words of the row: the
+  // lane of the even block writes the one of pieces 2q, the odd block's 2q+1
   const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
   if (slot < 0) return;
   int r;
@@ -148,24 +152,34 @@ __global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
 // 8 nibbles times a block's scale, rounded once.
 template <class E>
 __device__ __forceinline__ void store8(E* p, uint32_t w, float s) {
+  uint32_t h[4];
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
   __align__(16) E out[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) out[j] = from_float<E>(kv4::nibble_value(w >> (4 * j)) * s);
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+    out[2 * j] = from_float<E>(f.x * s);
+    out[2 * j + 1] = from_float<E>(f.y * s);
+  }
 #pragma unroll
   for (int j = 0; j < int(sizeof(out) / 16); ++j)
     reinterpret_cast<uint4*>(p)[j] = reinterpret_cast<const uint4*>(out)[j];
 }
 
-// The write's shape, the other way round: 0.53 bytes read and 2 written (bf16) an element.
+// The write's shape, the other way round: 0.53 bytes read and 2 written (bf16) an
+// element.  131072 tokens of 4 heads of 128: 71 us, 4.8 TB/s.
 template <class E, int D>
 __global__ void __launch_bounds__(kRwThreads) kv4_read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;
-  const int t = blockIdx.x * (kRwThreads / kLanes) + threadIdx.x / kLanes;
-  const int w = threadIdx.x % kLanes, h = blockIdx.y, Hkv = gridDim.y;
+  const int Hkv = a.s.Hkv, run = blockIdx.x / Hkv, h = blockIdx.x - run * Hkv;
+  const int t = run * (kRwThreads / kLanes) + threadIdx.x / kLanes, w = threadIdx.x % kLanes;
   if (t >= a.s.T) return;
   const int slot = slot_of(a.s, t);
-  uint32_t kw = 0, vw = 0;
-  float ks = 1.0f, vs = 1.0f;
+  uint32_t kw = 0u, vw = 0u, kc = 127u, vc = 127u;
   if (slot >= 0) {
     int r;
     const uint8_t* tile = a.pool + tile_of<D>(a.s, slot, h, Hkv, r);
@@ -174,12 +188,12 @@ __global__ void __launch_bounds__(kRwThreads) kv4_read_kernel(ReadArgs a) {
     kw = __ldg(reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4));
     vw = uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + (2 * q * nb + b) * 2))) |
          uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + ((2 * q + 1) * nb + b) * 2))) << 16;
-    ks = kv4::code_value(__ldg(tile + 16 * D + r * nb + b));
-    vs = kv4::code_value(__ldg(tile + 16 * D + D / 2 + r * nb + b));
+    kc = __ldg(tile + 16 * D + r * nb + b);
+    vc = __ldg(tile + 16 * D + D / 2 + r * nb + b);
   }
   const long long at = ((long long)t * Hkv + h) * D + 8 * w;
-  store8(static_cast<E*>(a.y[0]) + at, kw, ks);
-  store8(static_cast<E*>(a.y[1]) + at, vw, vs);
+  store8(static_cast<E*>(a.y[0]) + at, kw, kv4::code_value(kc));
+  store8(static_cast<E*>(a.y[1]) + at, vw, kv4::code_value(vc));
 }
 
 int check_pool(const void* pool, int Hkv, int D, int page, int num_pages) {
@@ -202,7 +216,7 @@ int launched(const char*) {
 }
 
 template <class E>
-void launch_write(const WriteArgs& a, int D, bool vec, dim3 grid, cudaStream_t s) {
+void launch_write(const WriteArgs& a, int D, bool vec, unsigned grid, cudaStream_t s) {
   if (D == 128) {
     if (vec) kv4_write_kernel<E, 128, true><<<grid, kRwThreads, 0, s>>>(a);
     else kv4_write_kernel<E, 128, false><<<grid, kRwThreads, 0, s>>>(a);
@@ -213,17 +227,18 @@ void launch_write(const WriteArgs& a, int D, bool vec, dim3 grid, cudaStream_t s
 }
 
 template <class E>
-void launch_read(const ReadArgs& a, int D, dim3 grid, cudaStream_t s) {
+void launch_read(const ReadArgs& a, int D, unsigned grid, cudaStream_t s) {
   if (D == 128) kv4_read_kernel<E, 128><<<grid, kRwThreads, 0, s>>>(a);
   else kv4_read_kernel<E, 64><<<grid, kRwThreads, 0, s>>>(a);
 }
 
-Slots make_slots(const int64_t* slots, int T, int page, int num_pages) {
+Slots make_slots(const int64_t* slots, int T, int Hkv, int page, int num_pages) {
   Slots s{};
   s.slots = reinterpret_cast<const long long*>(slots);
   s.err = device_error_flag();
   s.capacity = num_pages * page;
   s.T = T;
+  s.Hkv = Hkv;
   s.page = page;
   s.page_shift = -1;
   for (int i = 4; i < 31; ++i)
@@ -231,9 +246,11 @@ Slots make_slots(const int64_t* slots, int T, int page, int num_pages) {
   return s;
 }
 
-dim3 rw_grid(int T, int Hkv, int D) {
+// Blocks of a call; 0: more than a grid holds.
+unsigned rw_grid(int T, int Hkv, int D) {
   const int per = kRwThreads / (D / 8);
-  return dim3(unsigned((T + per - 1) / per), unsigned(Hkv));
+  const long long n = ((long long)T + per - 1) / per * Hkv;
+  return n > 0x7FFFFFFFLL ? 0u : unsigned(n);
 }
 
 }  // namespace
@@ -266,14 +283,15 @@ extern "C" int mfi_kv4_write(const void* k, long long k_row, long long k_head, c
   a.row[0] = k_row; a.row[1] = v_row;
   a.head[0] = k_head; a.head[1] = v_head;
   a.pool = pool;
-  a.s = mfi::make_slots(slots, T, page, num_pages);
+  a.s = mfi::make_slots(slots, T, Hkv, page, num_pages);
   // 16-byte loads where every vector starts on a 16-byte boundary
   const int size = dtype == MFI_F32 ? 4 : 2;
   bool vec = true;
   for (int i = 0; i < 2; ++i)
     vec = vec && !((reinterpret_cast<uintptr_t>(a.x[i]) | uintptr_t(a.row[i] * size) |
                     uintptr_t(a.head[i] * size)) & 15);
-  const dim3 grid = mfi::rw_grid(T, Hkv, D);
+  const unsigned grid = mfi::rw_grid(T, Hkv, D);
+  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_write: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == MFI_F32) mfi::launch_write<float>(a, D, vec, grid, s);
   else if (dtype == MFI_F16) mfi::launch_write<__half>(a, D, vec, grid, s);
@@ -295,8 +313,9 @@ extern "C" int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, 
   mfi::ReadArgs a{};
   a.pool = pool;
   a.y[0] = k; a.y[1] = v;
-  a.s = mfi::make_slots(slots, T, page, num_pages);
-  const dim3 grid = mfi::rw_grid(T, Hkv, D);
+  a.s = mfi::make_slots(slots, T, Hkv, page, num_pages);
+  const unsigned grid = mfi::rw_grid(T, Hkv, D);
+  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == MFI_F32) mfi::launch_read<float>(a, D, grid, s);
   else if (dtype == MFI_F16) mfi::launch_read<__half>(a, D, grid, s);
