@@ -7,8 +7,10 @@
 // and zeros for a row that sees no token.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "../../include/moe_fp4.h"
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 #include "tc_ptx.cuh"
 #include "tmap.cuh"
 #include "work.cuh"
@@ -19,45 +21,7 @@ int kv4_check_pool(const void* pool, int Hkv, int D, int page, int num_pages);
 
 namespace {
 
-struct AttnArgs {
-  const void* q;
-  long long q_row, q_head;   // strides in elements
-  const uint8_t* pool;
-  const int* table;          // (n_seq, width)
-  long long table_ld;
-  const int* kv_lens;
-  const int* cu_q;           // (n_seq + 1) or null: max_q rows each
-  void* out;                 // (T, Hq, D)
-  int* err;
-  unsigned* counters;        // one per CTA, zero between calls
-  float* part;               // two slots per CTA
-  int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
-  bool q_vec;                // every query row starts on a 16-byte boundary
-  int tpp_shift;             // log2 of the tiles of a page, -1 if that is no power of two
-  float scale;
-};
-
-// Rows and tokens of sequence i, clamped to the query rows and the table.
-struct Seq {
-  int row0, rows, len;
-};
-__device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
-  Seq s;
-  s.row0 = a.cu_q ? a.cu_q[i] : i * a.max_q;
-  const int end = a.cu_q ? a.cu_q[i + 1] : s.row0 + a.max_q;
-  s.rows = end - s.row0;
-  s.len = a.kv_lens[i];
-  const long long room = (long long)a.width * a.page;
-  if (s.row0 < 0 || s.rows < 0 || end > a.T || s.rows > a.max_q) {
-    kv4::report(a.err, kv4::kErrPage);
-    s.rows = 0;
-  }
-  if (s.len > room || s.len < 0) {
-    kv4::report(a.err, kv4::kErrPage);
-    s.len = s.len < 0 ? 0 : int(room);
-  }
-  return s;
-}
+using namespace kv4;
 
 // ---- few rows: vectors of a group on the legacy tensor path --------------------
 // A vector is one row of one query head; the R G vectors of a sequence and KV
@@ -80,7 +44,6 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
 constexpr int kStages = 2;   // one read, one on its way
-constexpr int kCtas = 148;   // one per SM
 constexpr unsigned kSnap = 32;  // tiles
 
 template <int D, int kNT>
@@ -97,30 +60,6 @@ struct Few {
   static constexpr int kSmem = kWarps * kWarpBytes;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// The four bytes of w, each two E2M1 values, to fp16x2 (low nibble: low half).
-__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {
-  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
-      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
-      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-      : "r"(w));
-}
-// E8M0 codes (nb bytes) to fp32; 255 gives NaN.
-template <int nb>
-__device__ __forceinline__ void codes(uint32_t w, float (&f)[nb]) {
-#pragma unroll
-  for (int i = 0; i < nb / 2; ++i) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(uint16_t(i ? w >> 16 : w)));
-    f[2 * i] = __uint_as_float(r << 16);
-    f[2 * i + 1] = __uint_as_float(r & 0xFFFF0000u);
-  }
-}
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -143,38 +82,10 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
 // all ones in the halves of a that are not zero
 __device__ __forceinline__ uint32_t nonzero_half2(uint32_t a) {
   return __hne2_mask(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0)));
 }
-__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// 8 elements of a query row as they are; vec: p is 16-byte aligned.
-template <class E>
-__device__ __forceinline__ uint4 q8(const E* p, bool vec) {
-  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
-  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-  return make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16,
-                    h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
-}
-template <class E>
-__device__ __forceinline__ float2 two_floats(uint32_t w);
-template <>
-__device__ __forceinline__ float2 two_floats<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <>
-__device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
-}
-
 // Tiles of sequence s's pieces and their count of sets.
 __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
@@ -538,7 +449,9 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   // ---- this CTA's share of the work: every warp sums the sequences' units, 32
   // at a time, then finds the sequences that hold the share's ends
   auto sets_of = [&](const Seq& s) { return (s.rows * G + F::kVec - 1) / F::kVec; };
-  auto units_of = [&](const Seq& s) { return unsigned(seq_tiles(s)) * a.Hkv * sets_of(s); };
+  auto units_of = [&](const Seq& s) {
+    return s.rows * G > a.few ? 0u : unsigned(seq_tiles(s)) * a.Hkv * sets_of(s);
+  };
   unsigned U = 0;
   for (int i = lane; i < a.n_seq; i += 32) U += units_of(sequence(a, i));
   U = __reduce_add_sync(0xffffffffu, U);
@@ -870,15 +783,19 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
 }
 
 // 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
-// are then read and decoded half as often), else 8.
-template <class E, int D>
-cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
-  const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
-  return vectors <= 8 ? launch_few<E, D, 1>(a, s) : launch_few<E, D, 2>(a, s);
-}
+// are then read and decoded half as often), else 8.  Sequences of more than
+// kFew vectors go to the kernel for many rows, whose tile is 256 vectors.
+constexpr int kFew = 64;
 
-constexpr size_t kCounterBytes = 1024;  // one counter per CTA
-static_assert(kCounterBytes >= kCtas * sizeof(unsigned), "a counter per CTA");
+template <class E, int D>
+cudaError_t launch(AttnArgs& a, cudaStream_t s) {
+  const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
+  a.few = kFew;
+  cudaError_t e = vectors <= 8 ? launch_few<E, D, 1>(a, s) : launch_few<E, D, 2>(a, s);
+  if (e == cudaSuccess && vectors > kFew)
+    e = launch_kv4_prefill(a, std::is_same<E, __nv_bfloat16>::value, D, s);
+  return e;
+}
 
 }  // namespace
 }  // namespace mfi
@@ -886,7 +803,7 @@ static_assert(kCounterBytes >= kCtas * sizeof(unsigned), "a counter per CTA");
 extern "C" size_t mfi_kv4_attn_workspace_bytes(int n_seq, int Hq, int Hkv, int D, int max_q) {
   if (n_seq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_q <= 0)
     return 0;
-  return mfi::kCounterBytes + size_t(mfi::kCtas) * 2 * 16 * (D + 4) * sizeof(float);
+  return mfi::kv4::kCounterBytes + size_t(mfi::kv4::kCtas) * 2 * 16 * (D + 4) * sizeof(float);
 }
 
 extern "C" int mfi_kv4_attn_init_workspace(void* workspace, size_t workspace_bytes, void* stream) {
@@ -926,7 +843,7 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
                        (double(max_q) * (Hq / Hkv) / 8 + 1);
   if (units >= 2147483648.0)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: more than 2^31 tiles of work in one call");
-  mfi::AttnArgs a{};
+  mfi::kv4::AttnArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head;
   a.pool = pool; a.table = table; a.table_ld = table_ld;
   a.kv_lens = kv_lens; a.cu_q = cu_q; a.out = out;
@@ -940,7 +857,7 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   for (int i = 0; i < 31; ++i)
     if (tpp == 1 << i) a.tpp_shift = i;
   a.counters = static_cast<unsigned*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + mfi::kCounterBytes);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + mfi::kv4::kCounterBytes);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
   if (dtype == MFI_BF16)

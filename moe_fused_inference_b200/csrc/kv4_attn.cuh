@@ -1,0 +1,112 @@
+// kv4_attn.cuh — what the two attention kernels over the paged 4-bit KV cache
+// share (kv4_attn.cu: few rows; kv4_prefill.cu: many).
+#pragma once
+#include "kv4.cuh"
+
+namespace mfi {
+namespace kv4 {
+
+struct AttnArgs {
+  const void* q;
+  long long q_row, q_head;   // strides in elements
+  const uint8_t* pool;
+  const int* table;          // (n_seq, width)
+  long long table_ld;
+  const int* kv_lens;
+  const int* cu_q;           // (n_seq + 1) or null: max_q rows each
+  void* out;                 // (T, Hq, D)
+  int* err;
+  unsigned* counters;        // kCounters words, zero between calls
+  float* part;               // two slots per CTA
+  int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
+  int few;                   // sequences of up to this many vectors (rows x heads of a group) are `few`
+  bool q_vec;                // every query row starts on a 16-byte boundary
+  int tpp_shift;             // log2 of the tiles of a page, -1 if that is no power of two
+  float scale;
+};
+
+// Rows and tokens of sequence i, clamped to the query rows and the table.
+struct Seq {
+  int row0, rows, len;
+};
+__device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
+  Seq s;
+  s.row0 = a.cu_q ? a.cu_q[i] : i * a.max_q;
+  const int end = a.cu_q ? a.cu_q[i + 1] : s.row0 + a.max_q;
+  s.rows = end - s.row0;
+  s.len = a.kv_lens[i];
+  const long long room = (long long)a.width * a.page;
+  if (s.row0 < 0 || s.rows < 0 || end > a.T || s.rows > a.max_q) {
+    report(a.err, kv4::kErrPage);
+    s.rows = 0;
+  }
+  if (s.len > room || s.len < 0) {
+    report(a.err, kv4::kErrPage);
+    s.len = s.len < 0 ? 0 : int(room);
+  }
+  return s;
+}
+
+
+constexpr int kCtas = 148;                 // one per SM
+constexpr size_t kCounterBytes = 1024;
+constexpr int kItemCounter = kCtas, kDoneCounter = kCtas + 1;  // of the kernel for many rows
+static_assert(kCounterBytes >= (kCtas + 2) * sizeof(unsigned), "a counter per CTA and two more");
+
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// The four bytes of w, each two E2M1 values, to fp16x2 (low nibble: low half).
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
+}
+// E8M0 codes (nb bytes) to fp32; 255 gives NaN.
+template <int nb>
+__device__ __forceinline__ void codes(uint32_t w, float (&f)[nb]) {
+#pragma unroll
+  for (int i = 0; i < nb / 2; ++i) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.ue8m0x2 %0, %1;" : "=r"(r) : "h"(uint16_t(i ? w >> 16 : w)));
+    f[2 * i] = __uint_as_float(r << 16);
+    f[2 * i + 1] = __uint_as_float(r & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// 8 elements of a query row as they are; vec: p is 16-byte aligned.
+template <class E>
+__device__ __forceinline__ uint4 q8(const E* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  return make_uint4(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16,
+                    h[4] | uint32_t(h[5]) << 16, h[6] | uint32_t(h[7]) << 16);
+}
+template <class E>
+__device__ __forceinline__ float2 two_floats(uint32_t w);
+template <>
+__device__ __forceinline__ float2 two_floats<__half>(uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+
+}  // namespace kv4
+
+// Launch the kernel for many rows on the sequences of more than a.few vectors.
+cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, bool bf16, int D, cudaStream_t s);
+
+}  // namespace mfi

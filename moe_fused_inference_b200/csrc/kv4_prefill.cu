@@ -1,0 +1,633 @@
+// kv4_prefill.cu — attention over the paged 4-bit KV cache for many rows
+// (prompts and their chunks) on the tcgen05 tensor cores.  Semantics and
+// arguments: kv4_attn.cu; layout: kv4.cuh.
+//
+// A vector is one row of one query head; an item is 256 vectors (two tiles of
+// 128) of a sequence and KV head, against the tokens that the last of them sees,
+// 128 at a time.  One persistent CTA per SM takes items from a counter, the
+// longest of a sequence first.  Its roles:
+//   warp 13      finds the next item, brings the tokens' tiles in by bulk copies
+//   warps 8-11   decode them to fp16 operands in shared memory (128-byte swizzle)
+//   warp 12      issues S_i = Q_i K^T and O_i += P_i V for both tiles i; while the
+//                tensor cores work for one tile the other is in its softmax
+//   warps 0-7    softmax, one thread a vector: S from TMEM, P as fp16 back into
+//                its place, O rescaled in TMEM when the maximum has moved, O out
+// TMEM: S_0, S_1 (128 columns each, P in the first 64), O_0, O_1.
+//
+// The operands are fp16: a query row times a power of two that brings its
+// maximum to [2^14, 2^15), a key or value element times 2^(c - ref + 12) with
+// ref the largest code (of the keys' 128 tokens, of the item's values so far):
+// exact unless 2^-36 below it.
+// P is rounded to fp16 after a factor 2^8; the maximum that it refers to moves
+// when it is passed by 2^4, the value scale that O refers to when passed by 2^3,
+// so P stays below 2^15.  l and O are fp32.
+#include <cuda_fp16.h>
+
+#include <atomic>
+
+#include "../../include/moe_fp4.h"
+#include "kv4_attn.cuh"
+#include "tc_ptx.cuh"
+#include "tmap.cuh"
+#include "work.cuh"
+
+namespace mfi {
+namespace {
+
+using namespace kv4;
+
+constexpr int kTok = 128;                  // tokens of a step
+constexpr int kRows = 128;                 // vectors of a tile
+constexpr int kThreads = 512;
+constexpr int kRegsSoftmax = 192, kRegsDecode = 80, kRegsOther = 48;
+static_assert(2 * kRegsSoftmax + kRegsDecode + kRegsOther <= 512, "registers of the launch: 128 a thread");
+constexpr float kLazy = 4.0f, kShift = 8.0f;  // log2: the maximum's slack, the weights' factor
+constexpr int kVSlack = 3;                    // log2: the value scale's slack
+constexpr int kUp = 12;                       // log2: the elements' factor
+
+template <int D>
+struct Many {
+  static constexpr int kOperand = kTok * D * 2;              // Q tile, K or V of a step
+  static constexpr int kRaw = kTok / kTile * tile_bytes(D);  // a step's tiles
+  static constexpr int kOffQ = 0, kOffK = 2 * kOperand, kOffV = 4 * kOperand, kOffRaw = 6 * kOperand;
+  static constexpr int kSmem = kOffRaw + 2 * kRaw;
+};
+
+struct Item {
+  int valid, seq, row0, rows, len, g, v0, steps;
+};
+
+// Byte offset of 16-byte chunk c (8 elements) of row r of an operand: halves of
+// 64 elements, each 128 rows of 128 bytes in the 128-byte swizzle.
+__device__ __forceinline__ uint32_t operand_at(int r, int c) {
+  return uint32_t(c >> 3) * (kTok * 128) + uint32_t(r) * 128 + (uint32_t((c & 7) ^ (r & 7)) << 4);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+// (a.x, a.y) * b + c, each half on its own
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n"
+      " add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+
+struct Bars {
+  uint64_t item_full[2], item_empty[2];  // the next item's description
+  uint64_t raw_full[2], raw_empty[2];    // a step's tiles
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t q_full[2];                    // of tile i: query rows written,
+  uint64_t s_full[2], p_full[2];         // scores there, weights there,
+  uint64_t o_full[2];                    // an item's last sum there
+  uint64_t drain;
+};
+
+template <class E, int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) {
+  using M = Many<D>;
+  constexpr int nb = D / 32;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ Bars bar;
+  __shared__ Item s_item[2];
+  __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN
+  __shared__ uint32_t s_ref[4][2];  // of a step: the key and value codes that its operands refer to
+  __shared__ uint32_t s_tmem;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = a.Hq / a.Hkv;
+
+  if (threadIdx.x == 0) {
+    tc::cta_abort_init();
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(&bar.item_full[i], 1);
+      tc::mbar_init(&bar.item_empty[i], 8 + 4 + 1);  // a lane of each warp that reads it
+      tc::mbar_init(&bar.raw_full[i], 1);
+      tc::mbar_init(&bar.raw_empty[i], 4);
+      tc::mbar_init(&bar.k_full[i], 4);
+      tc::mbar_init(&bar.k_empty[i], 1);
+      tc::mbar_init(&bar.v_full[i], 4);
+      tc::mbar_init(&bar.v_empty[i], 1);
+      tc::mbar_init(&bar.q_full[i], 4);
+      tc::mbar_init(&bar.s_full[i], 1);
+      tc::mbar_init(&bar.p_full[i], 4);
+      tc::mbar_init(&bar.o_full[i], 1);
+    }
+    tc::mbar_init(&bar.drain, 1);
+    tc::fence_mbar_init();
+  }
+  if (warp == 12) tc::tmem_alloc(&s_tmem, 512);
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  int* err = a.err;
+
+  // wait for the n-th completion (from 0) of a barrier
+  auto wait_one = [&](uint64_t* b, uint32_t n, int code) { return tc::mbar_wait(b, n & 1u, err, code); };
+  // the same for a whole warp, which goes on or gives up as one
+  auto wait = [&](uint64_t* b, uint32_t n, int code) {
+    return __all_sync(0xffffffffu, tc::mbar_wait(b, n & 1u, err, code)) != 0;
+  };
+
+  if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == 13) {
+      // ---- items and their tiles
+      const int tpp = a.page / kTile;
+      const uint64_t page_bytes = uint64_t(a.Hkv) * tpp * tile_bytes(D);
+      uint32_t step = 0, filled = 0;
+      for (uint32_t n = 0;; ++n) {
+        unsigned idx = 0;
+        if (lane == 0) idx = atomicAdd(a.counters + kItemCounter, 1u);
+        idx = __shfl_sync(0xffffffffu, idx, 0);
+        Item it{};
+        unsigned before = 0;
+        for (int i0 = 0; i0 < a.n_seq; i0 += 32) {
+          const int i = i0 + lane;
+          const Seq s = i < a.n_seq ? sequence(a, i) : Seq{0, 0, 0};
+          const unsigned items =
+              s.rows * G > a.few ? unsigned((s.rows * G + 2 * kRows - 1) / (2 * kRows)) * a.Hkv : 0u;
+          unsigned start = items;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const unsigned x = __shfl_up_sync(0xffffffffu, start, off);
+            if (lane >= off) start += x;
+          }
+          const unsigned sum = __shfl_sync(0xffffffffu, start, 31);
+          start += before - items;
+          const unsigned has = __ballot_sync(0xffffffffu, start <= idx && idx < start + items);
+          if (has) {
+            const int src = __ffs(has) - 1;
+            it.valid = 1;
+            it.seq = i0 + src;
+            it.row0 = __shfl_sync(0xffffffffu, s.row0, src);
+            it.rows = __shfl_sync(0xffffffffu, s.rows, src);
+            it.len = __shfl_sync(0xffffffffu, s.len, src);
+            const unsigned in = idx - __shfl_sync(0xffffffffu, start, src);
+            const unsigned pairs = __shfl_sync(0xffffffffu, items, src) / a.Hkv;
+            it.g = int(in % a.Hkv);
+            it.v0 = int(pairs - 1 - in / a.Hkv) * 2 * kRows;  // the rows that see most first
+            const int last = min(it.v0 + 2 * kRows, it.rows * G) - 1;
+            it.steps = max(1, (it.len - it.rows + last / G + 1 + kTok - 1) / kTok);
+            break;
+          }
+          before += sum;
+        }
+        const uint32_t slot = n & 1u;
+        if (n >= 2 && !wait(&bar.item_empty[slot], (n >> 1) - 1, 1)) break;
+        if (lane == 0) {
+          s_item[slot] = it;
+          for (int b = 0; b < 4; ++b) s_nan[slot][b] = 0x7FFFFFFF;
+          tc::mbar_arrive(&bar.item_full[slot]);
+        }
+        if (!it.valid) break;
+        const int have = (it.len + kTile - 1) / kTile;
+        const int* row = a.table + it.seq * a.table_ld;
+        auto page_of = [&](int t) {
+          return lane < kTok / kTile && t < have ? __ldg(row + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp))
+                                                 : -1;
+        };
+        int t = lane, id = page_of(t);
+        bool ok = true;
+        for (int j = 0; j < it.steps; ++j, ++step) {
+          const uint32_t st = step & 1u;
+          ok = step < 2 || wait(&bar.raw_empty[st], (step >> 1) - 1, 1);
+          if (!ok) break;
+          if (lane == 0)
+            tc::mbar_expect_tx(&bar.raw_full[st],
+                               uint32_t(max(min(kTok / kTile, have - t), 0)) * tile_bytes(D));
+          __syncwarp();
+          filled = step + 1;
+          if (lane < kTok / kTile && t < have) {
+            if (unsigned(id) >= unsigned(a.num_pages)) {
+              report(err, kErrPage);
+              id = 0;
+            }
+            const int in = it.g * tpp + (a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp);
+            tc::bulk_load(smem + M::kOffRaw + st * M::kRaw + lane * tile_bytes(D),
+                          a.pool + unsigned(id) * page_bytes + uint64_t(unsigned(in)) * tile_bytes(D),
+                          tile_bytes(D), &bar.raw_full[st]);
+          }
+          t += kTok / kTile;
+          id = page_of(t);
+        }
+        if (!ok) break;
+      }
+      if (tc::cta_aborted()) tc::drain_ring(bar.raw_full, 2, filled);
+      // the last CTA to see no item left resets the counter for the next call
+      if (lane == 0 && atomicInc(a.counters + kDoneCounter, gridDim.x - 1) == gridDim.x - 1)
+        atomicExch(a.counters + kItemCounter, 0u);
+    } else if (warp == 12 && lane == 0) {
+      // ---- MMA issue
+      constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(kTok >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+      constexpr uint32_t kIdescPV =  // B (values) with the elements along N contiguous
+          (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
+      const uint32_t base = tc::smem_u32(smem);
+      auto scores = [&](int i, uint32_t slot) {
+        tc::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = uint32_t(k >> 2) * (kTok * 128) + (k & 3) * 32;
+          mma_ss(tmem + i * 128, tc::make_sdesc(base + M::kOffQ + i * M::kOperand + off, 16, 1024, tc::kLayoutSW128),
+                 tc::make_sdesc(base + M::kOffK + slot * M::kOperand + off, 16, 1024, tc::kLayoutSW128),
+                 kIdesc, k != 0);
+        }
+        tc::tc_commit(&bar.s_full[i]);
+      };
+      auto values = [&](int i, uint32_t slot, bool add) {
+        tc::tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < kTok / 16; ++k)
+          mma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
+                 tc::make_sdesc(base + M::kOffV + slot * M::kOperand + k * 2048, kTok * 128, 1024,
+                                tc::kLayoutSW128),
+                 kIdescPV, add || k != 0);
+      };
+      uint32_t step = 0;
+      bool ok = true;
+      for (uint32_t n = 0; ok; ++n) {
+        const uint32_t slot = n & 1u;
+        if (!wait_one(&bar.item_full[slot], n >> 1, 2)) break;
+        const Item it = s_item[slot];
+        tc::mbar_arrive(&bar.item_empty[slot]);
+        if (!it.valid) break;
+        ok = wait_one(&bar.k_full[step & 1u], step >> 1, 2);
+        for (int i = 0; i < 2 && ok; ++i) {
+          ok = wait_one(&bar.q_full[i], n, 2);
+          if (ok) scores(i, step & 1u);
+        }
+        if (!ok) break;
+        tc::tc_commit(&bar.k_empty[step & 1u]);
+        uint32_t pn = step;  // completions of p_full so far
+        for (int j = 0; j < it.steps && ok; ++j, ++step, ++pn) {
+          const uint32_t st = step & 1u, nst = (step + 1) & 1u;
+          const bool more = j + 1 < it.steps;
+          ok = wait_one(&bar.v_full[st], step >> 1, 2);
+          for (int i = 0; i < 2 && ok; ++i) {
+            ok = wait_one(&bar.p_full[i], pn, 2);
+            if (!ok) break;
+            values(i, st, j != 0);
+            if (!more) {
+              tc::tc_commit(&bar.o_full[i]);
+            } else {
+              if (i == 0) ok = wait_one(&bar.k_full[nst], (step + 1) >> 1, 2);
+              if (ok) scores(i, nst);
+            }
+          }
+          if (!ok) break;
+          tc::tc_commit(&bar.v_empty[st]);
+          if (more) tc::tc_commit(&bar.k_empty[nst]);
+        }
+      }
+      if (tc::cta_aborted()) tc::drain_mma(&bar.drain);
+    }
+  } else if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDecode));
+    // ---- decode: lane (row, quarter t of the row) of 8 rows at a time, rows r
+    // and r + 4 side by side: their swizzled chunks share no banks
+    const int dw = warp - 8, t = lane & 3, r8 = ((lane >> 2) & 1) * 4 + (lane >> 3);
+    uint32_t step = 0;
+    for (uint32_t n = 0;; ++n) {
+      const uint32_t slot = n & 1u;
+      if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
+      const int len = s_item[slot].len, steps = s_item[slot].steps, valid = s_item[slot].valid;
+      bool ok = true;
+      uint32_t vtop = 28u;
+      if (valid) {
+        for (int j = 0; j < steps; ++j, ++step) {
+          const uint32_t st = step & 1u;
+          ok = wait(&bar.raw_full[st], step >> 1, 1);
+          if (!ok) break;
+          const uint8_t* raw = smem + M::kOffRaw + st * M::kRaw;
+          const int pos0 = j * kTok;
+          // the largest codes (255, NaN, not counted) of the step's keys and of the
+          // item's values so far, by every warp
+          uint32_t ref[2];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int x = 0; x < kTok / 32; ++x) {
+              const int tok = x * 32 + lane;
+              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
+              uint32_t w = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+              if (pos0 + tok >= len) w = 0;
+              w &= ~__vcmpeq4(w, 0xFFFFFFFFu);
+              m = __vmaxu4(m, w);
+            }
+            m = max(max(m & 0xFFu, (m >> 8) & 0xFFu), max((m >> 16) & 0xFFu, m >> 24));
+            ref[kv] = max(__reduce_max_sync(0xffffffffu, m), 28u);
+          }
+          ref[1] = vtop = max(ref[1], vtop);
+          if (dw == 0 && lane == 0) {
+            s_ref[step & 3u][0] = ref[0];
+            s_ref[step & 3u][1] = ref[1];
+          }
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            uint64_t* empty = kv ? &bar.v_empty[st] : &bar.k_empty[st];
+            ok = step < 2 || wait(empty, (step >> 1) - 1, 1);
+            if (!ok) break;
+            uint8_t* dst = smem + (kv ? M::kOffV : M::kOffK) + st * M::kOperand;
+            const float u = __uint_as_float((127 + 127 + kUp - ref[kv]) << 23);  // 2^(127 + kUp - ref)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int row = dw * 32 + x * 8 + r8, in = row % kTile;
+              const uint8_t* tile = raw + (row / kTile) * tile_bytes(D);
+              const uint8_t* c = tile + 16 * D + kv * (D / 2) + in * nb;
+              uint32_t cw = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+              uint32_t w[nb];
+              const uint8_t* src = tile + kv * 8 * D + in * (D / 2) + t * (4 * nb);
+              if (nb == 4) {
+                const uint4 y = *reinterpret_cast<const uint4*>(src);
+                w[0] = y.x; w[1] = y.y; w[nb - 2] = y.z; w[nb - 1] = y.w;
+              } else {
+                const uint2 y = *reinterpret_cast<const uint2*>(src);
+                w[0] = y.x; w[1] = y.y;
+              }
+              if (pos0 + row >= len) cw = 0;
+              if (kv) {
+                // pieces 2t and 2t + 1 of the blocks to the blocks' 8 elements
+                uint32_t y[nb];
+#pragma unroll
+                for (int b = 0; b < nb; ++b)
+                  y[b] = __byte_perm(w[b / 2], w[nb / 2 + b / 2], b % 2 ? 0x7632 : 0x5410);
+#pragma unroll
+                for (int b = 0; b < nb; ++b) w[b] = y[b];
+                // a NaN block counts for the rows that see it only: noted here,
+                // written at the end, and zero in the product
+                const uint32_t bad = __vcmpeq4(cw, 0xFFFFFFFFu);
+                if (bad) {
+                  for (int b = 0; b < nb; ++b)
+                    if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[slot][b], pos0 + row);
+                  cw &= ~bad;
+                }
+              }
+              float f[nb];
+              codes<nb>(cw, f);
+#pragma unroll
+              for (int b = 0; b < nb; ++b) {
+                const uint32_t h = pack_half(f[b] * u, f[b] * u);
+                uint32_t o[4];
+                e2m1x8(w[b], o);
+                *reinterpret_cast<uint4*>(dst + operand_at(row, 4 * b + t)) =
+                    make_uint4(mul_half2(o[0], h), mul_half2(o[1], h), mul_half2(o[2], h), mul_half2(o[3], h));
+              }
+            }
+            tc::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(kv ? &bar.v_full[st] : &bar.k_full[st]);
+          }
+          if (!ok) break;
+          if (lane == 0) tc::mbar_arrive(&bar.raw_empty[st]);
+        }
+      }
+      if (lane == 0) tc::mbar_arrive(&bar.item_empty[slot]);
+      if (!ok || !valid) break;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    // ---- softmax of tile i: thread = vector
+    const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * 128;
+    // load the item's query row, scaled to a maximum near 2^15; its scores lack qs
+    auto load_q = [&](const Item& it) {
+      const int v = it.v0 + i * kRows + r;
+      uint4 x[D / 8];
+      float am = 0.0f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) x[c] = make_uint4(0u, 0u, 0u, 0u);
+      if (v < it.rows * G) {
+        const int row = v / G, h = v - row * G;
+        const E* q = static_cast<const E*>(a.q) + (it.row0 + row) * a.q_row + (it.g * G + h) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) x[c] = q8(q + 8 * c, a.q_vec);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = two_floats<E>(w[k]);
+          am = fmaxf(am, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+      }
+      const int e = max(int(__float_as_uint(am) >> 23) - 127, -100);
+      // the rows take the scale's sign; with a scale of zero all scores are zero
+      float f = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+      f = a.scale == 0.0f ? 0.0f : copysignf(f, a.scale);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+        uint32_t h[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 y = two_floats<E>(w[k]);
+          h[k] = pack_half(y.x * f, y.y * f);
+        }
+        *reinterpret_cast<uint4*>(smem + M::kOffQ + i * M::kOperand + operand_at(r, c)) =
+            make_uint4(h[0], h[1], h[2], h[3]);
+      }
+      tc::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.q_full[i]);
+      return fmaxf(fabsf(a.scale) * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + e) << 23), 1e-37f);
+    };
+    uint32_t step = 0;
+    Item it{};
+    float qs = 0.0f;
+    bool ok = wait(&bar.item_full[0], 0, 3);
+    if (ok) {
+      it = s_item[0];
+      if (it.valid) qs = load_q(it);
+    }
+    for (uint32_t n = 0; ok && it.valid; ++n) {
+      const int v = it.v0 + i * kRows + r, nv = it.rows * G;
+      const int lim = v < nv ? it.len - it.rows + v / G + 1 : 0;     // tokens that this vector sees
+      const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1;  // that all of the tile see
+      float m = -INFINITY, l = 0.0f;
+      uint32_t vrun = 0;  // the value code that O refers to
+      for (int j = 0; j < it.steps; ++j, ++step) {
+        ok = wait(&bar.s_full[i], step, 3);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint32_t kref = s_ref[step & 3u][0], vref = s_ref[step & 3u][1];
+        const float sc = qs * __uint_as_float((127 + kref - 127 - kUp) << 23);
+        uint32_t s[kTok];
+#pragma unroll
+        for (int c = 0; c < kTok / 32; ++c)
+          tc::tmem_ld_32x32b_x32(ts + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+        tc::tmem_ld_wait();
+        if ((j + 1) * kTok > all) {
+          const int keep = lim - j * kTok;
+#pragma unroll
+          for (int c = 0; c < kTok; ++c)
+            if (c >= keep) s[c] = 0xFF800000u;
+        }
+        float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kTok; c += 4) {
+          t0 = fmaxf(fmaxf(t0, __uint_as_float(s[c])), __uint_as_float(s[c + 1]));
+          t1 = fmaxf(fmaxf(t1, __uint_as_float(s[c + 2])), __uint_as_float(s[c + 3]));
+        }
+        const float top = fmaxf(t0, t1) * sc;
+        const bool up = top > m + kLazy;
+        const bool vup = j == 0 || int(vref) > int(vrun) + kVSlack;
+        if (__any_sync(0xffffffffu, up) || vup) {
+          float c = up ? ex2(m - top) : 1.0f;
+          if (up) m = top;
+          l *= c;
+          if (vup) {
+            c *= j == 0 ? 0.0f : __uint_as_float(uint32_t(max(127 + int(vrun) - int(vref), 0)) << 23);
+            vrun = vref;
+          }
+          if (j > 0) {  // the products of the steps before are complete: their successor's scores are
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+              uint32_t o[32];
+              tc::tmem_ld_32x32b_x32(to + 32 * x, o);
+              tc::tmem_ld_wait();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c);
+              tmem_st_x32(to + 32 * x, o);
+            }
+          }
+        }
+        // p 2^(kShift + vref - vrun), l without the latter
+        const int dv = int(vref) - int(vrun);
+        const float down = __uint_as_float(uint32_t(127 - dv) << 23);  // 2^-dv, dv = 0 .. kVSlack
+        const float b0 = kShift + float(dv) - (m == -INFINITY ? 0.0f : m);
+        const float2 sc2 = make_float2(sc, sc), b2 = make_float2(b0, b0);
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            float2 x = make_float2(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1]));
+            x = fma2(x, sc2, b2);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            if (c & 1) sum1 = add2(sum1, x);
+            else sum0 = add2(sum0, x);
+            p[c] = pack_half(x.x, x.y);
+          }
+          tmem_st_x32(ts + 32 * h, p);
+        }
+        sum0 = add2(sum0, sum1);
+        l = fmaf(sum0.x + sum0.y, down, l);
+        tmem_st_wait();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bar.p_full[i]);
+      }
+      if (!ok) break;
+      // the next item's rows before this one's sums: its scores can begin
+      Item nx{};
+      float nqs = 0.0f;
+      ok = wait(&bar.item_full[(n + 1) & 1u], (n + 1) >> 1, 3);
+      if (!ok) break;
+      nx = s_item[(n + 1) & 1u];
+      if (nx.valid) nqs = load_q(nx);
+      ok = wait(&bar.o_full[i], n, 3);
+      if (!ok) break;
+      tc::tc_fence_after();
+      // O 2^(vrun - 127 - kUp) / l
+      const float inv = l == 0.0f ? 0.0f : __uint_as_float((vrun - kUp) << 23) / l;
+      E* out = static_cast<E*>(a.out) +
+               ((long long)(it.row0 + v / G) * a.Hq + it.g * G + v % G) * D;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        uint32_t o[32];
+        tc::tmem_ld_32x32b_x32(to + 32 * x, o);
+        tc::tmem_ld_wait();
+        const bool bad = lim > s_nan[n & 1u][x];
+        if (v < nv) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            __align__(16) E y[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              y[k] = E(bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[8 * c + k]) * inv);
+            *reinterpret_cast<uint4*>(out + 32 * x + 8 * c) = *reinterpret_cast<const uint4*>(y);
+          }
+        }
+      }
+      tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&bar.item_empty[n & 1u]);
+      it = nx;
+      qs = nqs;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 12) tc::tmem_dealloc(tmem, 512);
+}
+
+template <class E, int D>
+cudaError_t launch(const AttnArgs& a, cudaStream_t s) {
+  const void* fn = reinterpret_cast<const void*>(kv4_attn_many_kernel<E, D>);
+  cudaError_t e = ensure_dynamic_smem(fn, Many<D>::kSmem);
+  if (e != cudaSuccess) return e;
+  // the roles' registers come out of the launch's: never ask for more than it has
+  static std::atomic<int> regs{0};
+  int have = regs.load(std::memory_order_relaxed);
+  if (have == 0) {
+    cudaFuncAttributes at;
+    e = cudaFuncGetAttributes(&at, fn);
+    if (e != cudaSuccess) return e;
+    have = (at.numRegs + 7) / 8 * 8;
+    regs.store(have, std::memory_order_relaxed);
+  }
+  if (4 * have < 2 * kRegsSoftmax + kRegsDecode + kRegsOther) return cudaErrorLaunchOutOfResources;
+  kv4_attn_many_kernel<E, D><<<kCtas, kThreads, Many<D>::kSmem, s>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_kv4_prefill(const kv4::AttnArgs& a, bool bf16, int D, cudaStream_t s) {
+  if (bf16)
+    return D == 128 ? launch<__nv_bfloat16, 128>(a, s) : launch<__nv_bfloat16, 64>(a, s);
+  return D == 128 ? launch<__half, 128>(a, s) : launch<__half, 64>(a, s);
+}
+
+}  // namespace mfi
