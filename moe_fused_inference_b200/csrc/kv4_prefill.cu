@@ -39,7 +39,7 @@ using namespace kv4;
 constexpr int kTok = 128;                  // tokens of a step
 constexpr int kRows = 128;                 // vectors of a tile
 constexpr int kThreads = 512;
-constexpr int kRegsSoftmax = 192, kRegsDecode = 80, kRegsOther = 48;
+constexpr int kRegsSoftmax = 184, kRegsDecode = 88, kRegsOther = 56;
 static_assert(2 * kRegsSoftmax + kRegsDecode + kRegsOther <= 512, "registers of the launch: 128 a thread");
 constexpr float kLazy = 4.0f, kShift = 8.0f;  // log2: the maximum's slack, the weights' factor
 constexpr int kVSlack = 3;                    // log2: the value scale's slack
@@ -77,14 +77,12 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "r"(a), "l"(b), "r"(idesc), "r"(uint32_t(add))
       : "memory");
 }
-__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
+      "%15,%16};" ::"r"(taddr),
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-      "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-      "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() {
@@ -518,14 +516,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             vrun = vref;
           }
           if (j > 0) {  // the products of the steps before are complete: their successor's scores are
-#pragma unroll
-            for (int x = 0; x < D / 32; ++x) {
-              uint32_t o[32];
-              tc::tmem_ld_32x32b_x32(to + 32 * x, o);
+#pragma unroll 1
+            for (int x = 0; x < D / 16; ++x) {
+              uint32_t o[16];
+              tc::tmem_ld_32x32b_x16(to + 16 * x, o);
               tc::tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c);
-              tmem_st_x32(to + 32 * x, o);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c);
+              tmem_st_x16(to + 16 * x, o);
             }
           }
         }
@@ -536,11 +534,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         const float2 sc2 = make_float2(sc, sc), b2 = make_float2(b0, b0);
         float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t p[32];
+        for (int h = 0; h < kTok / 32; ++h) {
+          uint32_t p[16];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            float2 x = make_float2(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1]));
+          for (int c = 0; c < 16; ++c) {
+            float2 x = make_float2(__uint_as_float(s[32 * h + 2 * c]), __uint_as_float(s[32 * h + 2 * c + 1]));
             x = fma2(x, sc2, b2);
             x.x = ex2(x.x);
             x.y = ex2(x.y);
@@ -548,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             else sum0 = add2(sum0, x);
             p[c] = pack_half(x.x, x.y);
           }
-          tmem_st_x32(ts + 32 * h, p);
+          tmem_st_x16(ts + 16 * h, p);
         }
         sum0 = add2(sum0, sum1);
         l = fmaf(sum0.x + sum0.y, down, l);
