@@ -18,8 +18,8 @@
 // maximum to [2^14, 2^15), a key or value element times 2^(c - ref + 12) with
 // ref the largest code (of the keys' 128 tokens, of the item's values so far):
 // exact unless 2^-36 below it.
-// P is rounded to fp16 after a factor 2^8; the maximum that it refers to moves
-// when it is passed by 2^4, the value scale that O refers to when passed by 2^3,
+// P is rounded to fp16 after a factor 2^5; the maximum that it refers to moves
+// when it is passed by 2^7, the value scale that O refers to when passed by 2^3,
 // so P stays below 2^15.  l and O are fp32.
 #include <cuda_fp16.h>
 
@@ -41,7 +41,7 @@ constexpr int kRows = 128;                 // vectors of a tile
 constexpr int kThreads = 512;
 constexpr int kRegsSoftmax = 184, kRegsDecode = 88, kRegsOther = 56;
 static_assert(2 * kRegsSoftmax + kRegsDecode + kRegsOther <= 512, "registers of the launch: 128 a thread");
-constexpr float kLazy = 4.0f, kShift = 8.0f;  // log2: the maximum's slack, the weights' factor
+constexpr float kLazy = 7.0f, kShift = 5.0f;  // log2: the maximum's slack, the weights' factor
 constexpr int kVSlack = 3;                    // log2: the value scale's slack
 constexpr int kUp = 12;                       // log2: the elements' factor
 
@@ -106,6 +106,27 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
+// tc::mbar_wait with a long suspend hint: the softmax warps wait for much of the
+// time, and polls would take issue slots from the others.
+__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err, int code) {
+  const uint64_t t0 = tc::globaltimer_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(tc::smem_u32(bar)), "r"(parity), "r"(1000000u)
+        : "memory");
+    if (ok) return true;
+    if (tc::cta_aborted()) return false;
+    if (tc::globaltimer_ns() - t0 > tc::kWaitLimitNs) {
+      tc::cta_fail(err, code);
+      return false;
+    }
+  }
+}
+
 struct Bars {
   uint64_t item_full[2], item_empty[2];  // the next item's description
   uint64_t raw_full[2], raw_empty[2];    // a step's tiles
@@ -156,10 +177,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   int* err = a.err;
 
   // wait for the n-th completion (from 0) of a barrier
-  auto wait_one = [&](uint64_t* b, uint32_t n, int code) { return tc::mbar_wait(b, n & 1u, err, code); };
+  auto wait_one = [&](uint64_t* b, uint32_t n, int code) { return wait_asleep(b, n & 1u, err, code); };
   // the same for a whole warp, which goes on or gives up as one
   auto wait = [&](uint64_t* b, uint32_t n, int code) {
-    return __all_sync(0xffffffffu, tc::mbar_wait(b, n & 1u, err, code)) != 0;
+    return __all_sync(0xffffffffu, wait_asleep(b, n & 1u, err, code)) != 0;
   };
 
   if (warp >= 12) {
@@ -319,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     // ---- decode: lane (row, quarter t of the row) of 8 rows at a time, rows r
     // and r + 4 side by side: their swizzled chunks share no banks
     const int dw = warp - 8, t = lane & 3, r8 = ((lane >> 2) & 1) * 4 + (lane >> 3);
+    const int at = (dw * 32 + r8) * 128 + ((t ^ r8) << 4);  // operand_at(dw * 32 + r8, t)
     uint32_t step = 0;
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
@@ -336,20 +358,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           // the largest codes (255, NaN, not counted) of the step's keys and of the
           // item's values so far, by every warp
           uint32_t ref[2];
+          bool nan[2];
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
+            auto code_word = [&](int x) {
+              const int tok = x * 32 + lane;
+              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
+              const uint32_t w = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+              return pos0 + tok < len ? w : 0u;
+            };
             uint32_t m = 0;
 #pragma unroll
             for (int x = 0; x < kTok / 32; ++x) {
-              const int tok = x * 32 + lane;
-              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
-              uint32_t w = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-              if (pos0 + tok >= len) w = 0;
-              w &= ~__vcmpeq4(w, 0xFFFFFFFFu);
-              m = __vmaxu4(m, w);
+              const uint32_t w = code_word(x);
+              m = __vmaxu2(__vmaxu2(m, w & 0x00FF00FFu), (w >> 8) & 0x00FF00FFu);
             }
-            m = max(max(m & 0xFFu, (m >> 8) & 0xFFu), max((m >> 16) & 0xFFu, m >> 24));
-            ref[kv] = max(__reduce_max_sync(0xffffffffu, m), 28u);
+            m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+            nan[kv] = m == 255u;
+            if (nan[kv]) {  // rare: once more without them
+              m = 0;
+#pragma unroll 1
+              for (int x = 0; x < kTok / 32; ++x) {
+                uint32_t w = code_word(x);
+                w &= ~__vcmpeq4(w, 0xFFFFFFFFu);
+                m = __vmaxu2(__vmaxu2(m, w & 0x00FF00FFu), (w >> 8) & 0x00FF00FFu);
+              }
+              m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+            }
+            ref[kv] = max(m, 28u);
           }
           ref[1] = vtop = max(ref[1], vtop);
           if (dw == 0 && lane == 0) {
@@ -365,8 +401,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             const float u = __uint_as_float((127 + 127 + kUp - ref[kv]) << 23);  // 2^(127 + kUp - ref)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int row = dw * 32 + x * 8 + r8, in = row % kTile;
-              const uint8_t* tile = raw + (row / kTile) * tile_bytes(D);
+              const int row = dw * 32 + x * 8 + r8;
+              const uint8_t* tile = raw + (dw * 2 + x / 2) * tile_bytes(D);
+              const int in = (x % 2) * 8 + r8;  // row in the tile
               const uint8_t* c = tile + 16 * D + kv * (D / 2) + in * nb;
               uint32_t cw = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
               uint32_t w[nb];
@@ -387,10 +424,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
                   y[b] = __byte_perm(w[b / 2], w[nb / 2 + b / 2], b % 2 ? 0x7632 : 0x5410);
 #pragma unroll
                 for (int b = 0; b < nb; ++b) w[b] = y[b];
-                // a NaN block counts for the rows that see it only: noted here,
-                // written at the end, and zero in the product
-                const uint32_t bad = __vcmpeq4(cw, 0xFFFFFFFFu);
-                if (bad) {
+                if (nan[1]) {
+                  // a NaN block counts for the rows that see it only: noted here,
+                  // written at the end, and zero in the product
+                  const uint32_t bad = __vcmpeq4(cw, 0xFFFFFFFFu);
                   for (int b = 0; b < nb; ++b)
                     if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[slot][b], pos0 + row);
                   cw &= ~bad;
@@ -403,7 +440,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
                 const uint32_t h = pack_half(f[b] * u, f[b] * u);
                 uint32_t o[4];
                 e2m1x8(w[b], o);
-                *reinterpret_cast<uint4*>(dst + operand_at(row, 4 * b + t)) =
+                // chunk 4b + t of the row
+                *reinterpret_cast<uint4*>(dst + (b / 2) * (kTok * 128) + x * 1024 + (b % 2 ? at ^ 64 : at)) =
                     make_uint4(mul_half2(o[0], h), mul_half2(o[1], h), mul_half2(o[2], h), mul_half2(o[3], h));
               }
             }
