@@ -176,9 +176,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   const uint32_t tmem = s_tmem;
   int* err = a.err;
 
-  // wait for the n-th completion (from 0) of a barrier
-  auto wait_one = [&](uint64_t* b, uint32_t n, int code) { return wait_asleep(b, n & 1u, err, code); };
-  // the same for a whole warp, which goes on or gives up as one
+  // wait for the n-th completion (from 0) of a barrier; the warp goes on or gives
+  // up as one
   auto wait = [&](uint64_t* b, uint32_t n, int code) {
     return __all_sync(0xffffffffu, wait_asleep(b, n & 1u, err, code)) != 0;
   };
@@ -271,69 +270,80 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       // the last CTA to see no item left resets the counter for the next call
       if (lane == 0 && atomicInc(a.counters + kDoneCounter, gridDim.x - 1) == gridDim.x - 1)
         atomicExch(a.counters + kItemCounter, 0u);
-    } else if (warp == 12 && lane == 0) {
-      // ---- MMA issue
+    } else if (warp == 12) {
+      // ---- MMA issue: the whole warp goes along, so that the descriptors stay in
+      // uniform registers, one lane issues.  Descriptors are advanced by adding to
+      // their address field (bytes / 16).
       constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(kTok >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       constexpr uint32_t kIdescPV =  // B (values) with the elements along N contiguous
           (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       const uint32_t base = tc::smem_u32(smem);
+      const uint64_t dq = tc::make_sdesc(base + M::kOffQ, 16, 1024, tc::kLayoutSW128);
+      const uint64_t dk = tc::make_sdesc(base + M::kOffK, 16, 1024, tc::kLayoutSW128);
+      const uint64_t dv = tc::make_sdesc(base + M::kOffV, kTok * 128, 1024, tc::kLayoutSW128);
+      const bool leader = tc::elect_one();
+      auto commit = [&](uint64_t* bar) {
+        if (leader) tc::tc_commit(bar);
+      };
       auto scores = [&](int i, uint32_t slot) {
         tc::tc_fence_after();
+        const uint64_t q = dq + uint32_t(i) * (M::kOperand >> 4), k = dk + slot * (M::kOperand >> 4);
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = uint32_t(k >> 2) * (kTok * 128) + (k & 3) * 32;
-          mma_ss(tmem + i * 128, tc::make_sdesc(base + M::kOffQ + i * M::kOperand + off, 16, 1024, tc::kLayoutSW128),
-                 tc::make_sdesc(base + M::kOffK + slot * M::kOperand + off, 16, 1024, tc::kLayoutSW128),
-                 kIdesc, k != 0);
+          for (int x = 0; x < D / 16; ++x) {
+            const uint32_t off = ((x >> 2) * (kTok * 128) + (x & 3) * 32) >> 4;
+            mma_ss(tmem + i * 128, q + off, k + off, kIdesc, x != 0);
+          }
+          tc::tc_commit(&bar.s_full[i]);
         }
-        tc::tc_commit(&bar.s_full[i]);
       };
       auto values = [&](int i, uint32_t slot, bool add) {
         tc::tc_fence_after();
+        const uint64_t v = dv + slot * (M::kOperand >> 4);
+        if (leader) {
 #pragma unroll
-        for (int k = 0; k < kTok / 16; ++k)
-          mma_ts(tmem + 256 + i * 128, tmem + i * 128 + k * 8,
-                 tc::make_sdesc(base + M::kOffV + slot * M::kOperand + k * 2048, kTok * 128, 1024,
-                                tc::kLayoutSW128),
-                 kIdescPV, add || k != 0);
+          for (int x = 0; x < kTok / 16; ++x)
+            mma_ts(tmem + 256 + i * 128, tmem + i * 128 + x * 8, v + x * (2048 >> 4), kIdescPV, add || x != 0);
+        }
       };
       uint32_t step = 0;
       bool ok = true;
       for (uint32_t n = 0; ok; ++n) {
         const uint32_t slot = n & 1u;
-        if (!wait_one(&bar.item_full[slot], n >> 1, 2)) break;
+        if (!wait(&bar.item_full[slot], n >> 1, 2)) break;
         const Item it = s_item[slot];
-        tc::mbar_arrive(&bar.item_empty[slot]);
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&bar.item_empty[slot]);
         if (!it.valid) break;
-        ok = wait_one(&bar.k_full[step & 1u], step >> 1, 2);
+        ok = wait(&bar.k_full[step & 1u], step >> 1, 2);
         for (int i = 0; i < 2 && ok; ++i) {
-          ok = wait_one(&bar.q_full[i], n, 2);
+          ok = wait(&bar.q_full[i], n, 2);
           if (ok) scores(i, step & 1u);
         }
         if (!ok) break;
-        tc::tc_commit(&bar.k_empty[step & 1u]);
+        commit(&bar.k_empty[step & 1u]);
         uint32_t pn = step;  // completions of p_full so far
         for (int j = 0; j < it.steps && ok; ++j, ++step, ++pn) {
           const uint32_t st = step & 1u, nst = (step + 1) & 1u;
           const bool more = j + 1 < it.steps;
-          ok = wait_one(&bar.v_full[st], step >> 1, 2);
+          ok = wait(&bar.v_full[st], step >> 1, 2);
           for (int i = 0; i < 2 && ok; ++i) {
-            ok = wait_one(&bar.p_full[i], pn, 2);
+            ok = wait(&bar.p_full[i], pn, 2);
             if (!ok) break;
             values(i, st, j != 0);
             if (!more) {
-              tc::tc_commit(&bar.o_full[i]);
+              commit(&bar.o_full[i]);
             } else {
-              if (i == 0) ok = wait_one(&bar.k_full[nst], (step + 1) >> 1, 2);
+              if (i == 0) ok = wait(&bar.k_full[nst], (step + 1) >> 1, 2);
               if (ok) scores(i, nst);
             }
           }
           if (!ok) break;
-          tc::tc_commit(&bar.v_empty[st]);
-          if (more) tc::tc_commit(&bar.k_empty[nst]);
+          commit(&bar.v_empty[st]);
+          if (more) commit(&bar.k_empty[nst]);
         }
       }
-      if (tc::cta_aborted()) tc::drain_mma(&bar.drain);
+      if (tc::cta_aborted() && leader) tc::drain_mma(&bar.drain);
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDecode));
