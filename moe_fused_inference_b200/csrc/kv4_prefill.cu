@@ -4,19 +4,23 @@
 //
 // A vector is one row of one query head; an item is 256 vectors (two tiles of
 // 128) of a sequence and KV head, against the tokens that the last of them sees,
-// 128 at a time.  One persistent CTA per SM takes items from a counter, the
-// longest of a sequence first.  Its roles:
+// 64 a step.  One persistent CTA per SM takes items from a counter, the longest
+// of a sequence first.  Its roles:
 //   warp 13      finds the next item, brings the tokens' tiles in by bulk copies
 //   warps 8-11   decode them to fp16 operands in shared memory (128-byte swizzle)
-//   warp 12      issues S_i = Q_i K^T and O_i += P_i V for both tiles i; while the
-//                tensor cores work for one tile the other is in its softmax
+//   warps 12, 14 issue S_i = Q_i K^T of step s + 2 and O_i += P_i V of step s, one
+//                warp a tile i: while one waits the other's products run
 //   warps 0-7    softmax, one thread a vector: S from TMEM, P as fp16 back into
 //                its place, O rescaled in TMEM when the maximum has moved, O out
-// TMEM: S_0, S_1 (128 columns each, P in the first 64), O_0, O_1.
+// TMEM: of each tile two S of 64 columns (P in the first half of its S), then O_0
+// and O_1.  Two S a tile keep the softmax supplied while the tensor cores are at
+// the step before; with one S of 128 tokens a tile its warps and the tensor cores
+// waited for each other (16384 rows: 1.98 ms), although a product of 64 columns
+// takes 50 clocks and one of 128 takes 65 (both operands from shared memory).
 //
 // The operands are fp16: a query row times a power of two that brings its
 // maximum to [2^14, 2^15), a key or value element times 2^(c - ref + 12) with
-// ref the largest code (of the keys' 128 tokens, of the item's values so far):
+// ref the largest code (of the keys' 64 tokens, of the item's values so far):
 // exact unless 2^-36 below it.
 // P is rounded to fp16 after a factor 2^5; the maximum that it refers to moves
 // when it is passed by 2^7, the value scale that O refers to when passed by 2^3,
@@ -36,10 +40,11 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kTok = 128;                  // tokens of a step
+constexpr int kTok = 64;                   // tokens of a step
+constexpr int kSlots = 4;                  // steps on their way
 constexpr int kRows = 128;                 // vectors of a tile
 constexpr int kThreads = 512;
-constexpr int kRegsSoftmax = 184, kRegsDecode = 88, kRegsOther = 56;
+constexpr int kRegsSoftmax = 168, kRegsDecode = 112, kRegsOther = 64;
 static_assert(2 * kRegsSoftmax + kRegsDecode + kRegsOther <= 512, "registers of the launch: 128 a thread");
 constexpr float kLazy = 7.0f, kShift = 5.0f;  // log2: the maximum's slack, the weights' factor
 constexpr int kVSlack = 3;                    // log2: the value scale's slack
@@ -47,20 +52,23 @@ constexpr int kUp = 12;                       // log2: the elements' factor
 
 template <int D>
 struct Many {
-  static constexpr int kOperand = kTok * D * 2;              // Q tile, K or V of a step
+  static constexpr int kQ = kRows * D * 2;                   // a tile's query rows
+  static constexpr int kOperand = kTok * D * 2;              // K or V of a step
   static constexpr int kRaw = kTok / kTile * tile_bytes(D);  // a step's tiles
-  static constexpr int kOffQ = 0, kOffK = 2 * kOperand, kOffV = 4 * kOperand, kOffRaw = 6 * kOperand;
-  static constexpr int kSmem = kOffRaw + 2 * kRaw;
+  static constexpr int kOffK = 2 * kQ, kOffV = kOffK + kSlots * kOperand;
+  static constexpr int kOffRaw = kOffV + kSlots * kOperand;
+  static constexpr int kSmem = kOffRaw + kSlots * kRaw;
 };
 
 struct Item {
   int valid, seq, row0, rows, len, g, v0, steps;
 };
 
-// Byte offset of 16-byte chunk c (8 elements) of row r of an operand: halves of
-// 64 elements, each 128 rows of 128 bytes in the 128-byte swizzle.
+// An operand of R rows: halves of 64 elements, each R rows of 128 bytes in the
+// 128-byte swizzle.  Byte offset of 16-byte chunk c (8 elements) of row r:
+template <int R>
 __device__ __forceinline__ uint32_t operand_at(int r, int c) {
-  return uint32_t(c >> 3) * (kTok * 128) + uint32_t(r) * 128 + (uint32_t((c & 7) ^ (r & 7)) << 4);
+  return uint32_t(c >> 3) * (R * 128) + uint32_t(r) * 128 + (uint32_t((c & 7) ^ (r & 7)) << 4);
 }
 
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
@@ -106,35 +114,32 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// tc::mbar_wait with a long suspend hint: the softmax warps wait for much of the
-// time, and polls would take issue slots from the others.
-__device__ __forceinline__ bool wait_asleep(uint64_t* bar, uint32_t parity, int* err, int code) {
-  const uint64_t t0 = tc::globaltimer_ns();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(tc::smem_u32(bar)), "r"(parity), "r"(1000000u)
-        : "memory");
-    if (ok) return true;
-    if (tc::cta_aborted()) return false;
-    if (tc::globaltimer_ns() - t0 > tc::kWaitLimitNs) {
-      tc::cta_fail(err, code);
-      return false;
-    }
-  }
+// tc::mbar_wait for a warp that must stay uniform to the compiler (descriptors in
+// uniform registers): the polls are a loop inside the instruction block.  A poll
+// sleeps in hardware; the limit on their count is above the others' limit in time.
+__device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity, int* err, int code) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+      " add.u32 n, n, 1;\n setp.lt.u32 q, n, 4000000;\n @q bra AGAIN;\n"
+      "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  const bool all = __all_sync(0xffffffffu, ok != 0) != 0;
+  if (!all) tc::cta_fail(err, code);
+  return all;
 }
 
 struct Bars {
-  uint64_t item_full[2], item_empty[2];  // the next item's description
-  uint64_t raw_full[2], raw_empty[2];    // a step's tiles
-  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-  uint64_t q_full[2];                    // of tile i: query rows written,
-  uint64_t s_full[2], p_full[2];         // scores there, weights there,
-  uint64_t o_full[2];                    // an item's last sum there
-  uint64_t drain;
+  uint64_t item_full[2], item_empty[2];            // the next item's description
+  uint64_t raw_full[kSlots], raw_empty[kSlots];    // a step's tiles, operands
+  uint64_t k_full[kSlots], k_empty[kSlots], v_full[kSlots], v_empty[kSlots];
+  uint64_t q_full[2];                              // of tile i: query rows written,
+  uint64_t s_full[2][2], p_full[2][2];             // scores there, weights there (by step & 1),
+  uint64_t o_done[2][2];                           // products added (by step & 1)
+  uint64_t drain[2];
 };
 
 template <class E, int D>
@@ -145,42 +150,49 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   __shared__ Bars bar;
   __shared__ Item s_item[2];
   __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN
-  __shared__ uint32_t s_ref[4][2];  // of a step: the key and value codes that its operands refer to
+  __shared__ uint32_t s_ref[8][2];  // of a step: the key and value codes that its operands refer to
   __shared__ uint32_t s_tmem;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (from lane 0: the roles' branches are then known to be uniform)
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int G = a.Hq / a.Hkv;
 
   if (threadIdx.x == 0) {
     tc::cta_abort_init();
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&bar.item_full[i], 1);
-      tc::mbar_init(&bar.item_empty[i], 8 + 4 + 1);  // a lane of each warp that reads it
+      tc::mbar_init(&bar.item_empty[i], 8 + 4 + 64);  // a lane of each warp that reads it, all of warps 12 and 14
+      tc::mbar_init(&bar.drain[i], 1);
+      tc::mbar_init(&bar.q_full[i], 4);
+      for (int b = 0; b < 2; ++b) {
+        tc::mbar_init(&bar.s_full[i][b], 1);
+        tc::mbar_init(&bar.p_full[i][b], 4);
+        tc::mbar_init(&bar.o_done[i][b], 1);
+      }
+    }
+    for (int i = 0; i < kSlots; ++i) {
       tc::mbar_init(&bar.raw_full[i], 1);
       tc::mbar_init(&bar.raw_empty[i], 4);
       tc::mbar_init(&bar.k_full[i], 4);
-      tc::mbar_init(&bar.k_empty[i], 1);
+      tc::mbar_init(&bar.k_empty[i], 2);
       tc::mbar_init(&bar.v_full[i], 4);
-      tc::mbar_init(&bar.v_empty[i], 1);
-      tc::mbar_init(&bar.q_full[i], 4);
-      tc::mbar_init(&bar.s_full[i], 1);
-      tc::mbar_init(&bar.p_full[i], 4);
-      tc::mbar_init(&bar.o_full[i], 1);
+      tc::mbar_init(&bar.v_empty[i], 2);
     }
-    tc::mbar_init(&bar.drain, 1);
     tc::fence_mbar_init();
   }
   if (warp == 12) tc::tmem_alloc(&s_tmem, 512);
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
   int* err = a.err;
 
   // wait for the n-th completion (from 0) of a barrier; the warp goes on or gives
   // up as one
   auto wait = [&](uint64_t* b, uint32_t n, int code) {
-    return __all_sync(0xffffffffu, wait_asleep(b, n & 1u, err, code)) != 0;
+    return __all_sync(0xffffffffu, tc::mbar_wait(b, n & 1u, err, code)) != 0;
   };
+  // the n-th completion of the barrier of step n's slot
+  auto wait_slot = [&](uint64_t* b, uint32_t n, int code) { return wait(b + n % kSlots, n / kSlots, code); };
 
   if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -243,8 +255,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         int t = lane, id = page_of(t);
         bool ok = true;
         for (int j = 0; j < it.steps; ++j, ++step) {
-          const uint32_t st = step & 1u;
-          ok = step < 2 || wait(&bar.raw_empty[st], (step >> 1) - 1, 1);
+          const uint32_t st = step % kSlots;
+          ok = step < kSlots || wait_slot(bar.raw_empty, step - kSlots, 1);
           if (!ok) break;
           if (lane == 0)
             tc::mbar_expect_tx(&bar.raw_full[st],
@@ -266,91 +278,91 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         }
         if (!ok) break;
       }
-      if (tc::cta_aborted()) tc::drain_ring(bar.raw_full, 2, filled);
+      if (tc::cta_aborted()) tc::drain_ring(bar.raw_full, kSlots, filled);
       // the last CTA to see no item left resets the counter for the next call
       if (lane == 0 && atomicInc(a.counters + kDoneCounter, gridDim.x - 1) == gridDim.x - 1)
         atomicExch(a.counters + kItemCounter, 0u);
-    } else if (warp == 12) {
-      // ---- MMA issue: the whole warp goes along, so that the descriptors stay in
+    } else if (warp == 12 || warp == 14) {
+      // ---- MMA issue of tile i: the whole warp goes along, so that the descriptors stay in
       // uniform registers, one lane issues.  Descriptors are advanced by adding to
       // their address field (bytes / 16).
       constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(kTok >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       constexpr uint32_t kIdescPV =  // B (values) with the elements along N contiguous
           (1u << 4) | (1u << 16) | (uint32_t(D >> 3) << 17) | (uint32_t(kRows >> 4) << 24);
       const uint32_t base = tc::smem_u32(smem);
-      const uint64_t dq = tc::make_sdesc(base + M::kOffQ, 16, 1024, tc::kLayoutSW128);
+      const uint64_t dq = tc::make_sdesc(base, 16, 1024, tc::kLayoutSW128);
       const uint64_t dk = tc::make_sdesc(base + M::kOffK, 16, 1024, tc::kLayoutSW128);
       const uint64_t dv = tc::make_sdesc(base + M::kOffV, kTok * 128, 1024, tc::kLayoutSW128);
+      const int i = (warp - 12) >> 1;
       const bool leader = tc::elect_one();
-      auto commit = [&](uint64_t* bar) {
-        if (leader) tc::tc_commit(bar);
+      auto wait1 = [&](uint64_t* b, uint32_t n) { return wait_uniform(tc::smem_u32(b), n & 1u, err, 2); };
+      auto wait1_slot = [&](uint64_t* b, uint32_t n) { return wait1(b + n % kSlots, n / kSlots); };
+      auto commit = [&](uint64_t* b) {
+        if (leader) tc::tc_commit(b);
       };
-      auto scores = [&](int i, uint32_t slot) {
+      auto scores = [&](uint32_t g) {  // of step g
         tc::tc_fence_after();
-        const uint64_t q = dq + uint32_t(i) * (M::kOperand >> 4), k = dk + slot * (M::kOperand >> 4);
+        const uint64_t q = dq + uint32_t(i) * (M::kQ >> 4), k = dk + (g % kSlots) * (M::kOperand >> 4);
+        const uint32_t d = tmem + i * 128 + (g & 1u) * 64;
         if (leader) {
 #pragma unroll
-          for (int x = 0; x < D / 16; ++x) {
-            const uint32_t off = ((x >> 2) * (kTok * 128) + (x & 3) * 32) >> 4;
-            mma_ss(tmem + i * 128, q + off, k + off, kIdesc, x != 0);
-          }
-          tc::tc_commit(&bar.s_full[i]);
+          for (int x = 0; x < D / 16; ++x)
+            mma_ss(d, q + (((x >> 2) * (kRows * 128) + (x & 3) * 32) >> 4),
+                   k + (((x >> 2) * (kTok * 128) + (x & 3) * 32) >> 4), kIdesc, x != 0);
+          tc::tc_commit(&bar.s_full[i][g & 1u]);
         }
       };
-      auto values = [&](int i, uint32_t slot, bool add) {
+      auto values = [&](uint32_t g, bool add) {
         tc::tc_fence_after();
-        const uint64_t v = dv + slot * (M::kOperand >> 4);
+        const uint64_t v = dv + (g % kSlots) * (M::kOperand >> 4);
+        const uint32_t p = tmem + i * 128 + (g & 1u) * 64;
         if (leader) {
 #pragma unroll
           for (int x = 0; x < kTok / 16; ++x)
-            mma_ts(tmem + 256 + i * 128, tmem + i * 128 + x * 8, v + x * (2048 >> 4), kIdescPV, add || x != 0);
+            mma_ts(tmem + 256 + i * 128, p + x * 8, v + x * (2048 >> 4), kIdescPV, add || x != 0);
+          tc::tc_commit(&bar.o_done[i][g & 1u]);
         }
       };
-      uint32_t step = 0;
+      uint32_t g = 0;  // steps of all items
       bool ok = true;
       for (uint32_t n = 0; ok; ++n) {
         const uint32_t slot = n & 1u;
-        if (!wait(&bar.item_full[slot], n >> 1, 2)) break;
-        const Item it = s_item[slot];
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bar.item_empty[slot]);
-        if (!it.valid) break;
-        ok = wait(&bar.k_full[step & 1u], step >> 1, 2);
-        for (int i = 0; i < 2 && ok; ++i) {
-          ok = wait(&bar.q_full[i], n, 2);
-          if (ok) scores(i, step & 1u);
-        }
-        if (!ok) break;
-        commit(&bar.k_empty[step & 1u]);
-        uint32_t pn = step;  // completions of p_full so far
-        for (int j = 0; j < it.steps && ok; ++j, ++step, ++pn) {
-          const uint32_t st = step & 1u, nst = (step + 1) & 1u;
-          const bool more = j + 1 < it.steps;
-          ok = wait(&bar.v_full[st], step >> 1, 2);
-          for (int i = 0; i < 2 && ok; ++i) {
-            ok = wait(&bar.p_full[i], pn, 2);
-            if (!ok) break;
-            values(i, st, j != 0);
-            if (!more) {
-              commit(&bar.o_full[i]);
-            } else {
-              if (i == 0) ok = wait(&bar.k_full[nst], (step + 1) >> 1, 2);
-              if (ok) scores(i, nst);
-            }
-          }
+        if (!wait1(&bar.item_full[slot], n >> 1)) break;
+        const int valid = __shfl_sync(0xffffffffu, s_item[slot].valid, 0);
+        const int steps = __shfl_sync(0xffffffffu, s_item[slot].steps, 0);
+        tc::mbar_arrive(&bar.item_empty[slot]);
+        if (!valid) break;
+        ok = wait1(&bar.q_full[i], n);
+        // the scores run two steps ahead of the products
+        for (int j = 0; j < 2 && j < steps && ok; ++j) {
+          ok = wait1_slot(bar.k_full, g + j);
           if (!ok) break;
-          commit(&bar.v_empty[st]);
-          if (more) commit(&bar.k_empty[nst]);
+          scores(g + j);
+          commit(&bar.k_empty[(g + j) % kSlots]);
+        }
+        for (int j = 0; j < steps && ok; ++j, ++g) {
+          const bool more = j + 2 < steps;
+          ok = wait1_slot(bar.v_full, g) && wait1(&bar.p_full[i][g & 1u], g >> 1);
+          if (!ok) break;
+          values(g, j != 0);
+          commit(&bar.v_empty[g % kSlots]);
+          if (more) {
+            ok = wait1_slot(bar.k_full, g + 2);
+            if (!ok) break;
+            scores(g + 2);
+            commit(&bar.k_empty[(g + 2) % kSlots]);
+          }
         }
       }
-      if (tc::cta_aborted() && leader) tc::drain_mma(&bar.drain);
+      if (tc::cta_aborted() && leader) tc::drain_mma(&bar.drain[i]);
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDecode));
     // ---- decode: lane (row, quarter t of the row) of 8 rows at a time, rows r
     // and r + 4 side by side: their swizzled chunks share no banks
     const int dw = warp - 8, t = lane & 3, r8 = ((lane >> 2) & 1) * 4 + (lane >> 3);
-    const int at = (dw * 32 + r8) * 128 + ((t ^ r8) << 4);  // operand_at(dw * 32 + r8, t)
+    constexpr int kMine = kTok / 4;                             // a warp's tokens: one tile
+    const int at = (dw * kMine + r8) * 128 + ((t ^ r8) << 4);  // operand_at(dw * kMine + r8, t)
     uint32_t step = 0;
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
@@ -360,8 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       uint32_t vtop = 28u;
       if (valid) {
         for (int j = 0; j < steps; ++j, ++step) {
-          const uint32_t st = step & 1u;
-          ok = wait(&bar.raw_full[st], step >> 1, 1);
+          const uint32_t st = step % kSlots;
+          ok = wait_slot(bar.raw_full, step, 1);
           if (!ok) break;
           const uint8_t* raw = smem + M::kOffRaw + st * M::kRaw;
           const int pos0 = j * kTok;
@@ -399,21 +411,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           }
           ref[1] = vtop = max(ref[1], vtop);
           if (dw == 0 && lane == 0) {
-            s_ref[step & 3u][0] = ref[0];
-            s_ref[step & 3u][1] = ref[1];
+            s_ref[step & 7u][0] = ref[0];
+            s_ref[step & 7u][1] = ref[1];
           }
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            uint64_t* empty = kv ? &bar.v_empty[st] : &bar.k_empty[st];
-            ok = step < 2 || wait(empty, (step >> 1) - 1, 1);
+            ok = step < kSlots || wait_slot(kv ? bar.v_empty : bar.k_empty, step - kSlots, 1);
             if (!ok) break;
             uint8_t* dst = smem + (kv ? M::kOffV : M::kOffK) + st * M::kOperand;
             const float u = __uint_as_float((127 + 127 + kUp - ref[kv]) << 23);  // 2^(127 + kUp - ref)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const int row = dw * 32 + x * 8 + r8;
-              const uint8_t* tile = raw + (dw * 2 + x / 2) * tile_bytes(D);
-              const int in = (x % 2) * 8 + r8;  // row in the tile
+            for (int x = 0; x < kMine / 8; ++x) {
+              const int row = dw * kMine + x * 8 + r8, in = x * 8 + r8;  // token of the step, of the tile
+              const uint8_t* tile = raw + dw * tile_bytes(D);
               const uint8_t* c = tile + 16 * D + kv * (D / 2) + in * nb;
               uint32_t cw = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
               uint32_t w[nb];
@@ -507,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           const float2 y = two_floats<E>(w[k]);
           h[k] = pack_half(y.x * f, y.y * f);
         }
-        *reinterpret_cast<uint4*>(smem + M::kOffQ + i * M::kOperand + operand_at(r, c)) =
+        *reinterpret_cast<uint4*>(smem + i * M::kQ + operand_at<kRows>(r, c)) =
             make_uint4(h[0], h[1], h[2], h[3]);
       }
       tc::fence_proxy_async_smem();
@@ -530,15 +540,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       float m = -INFINITY, l = 0.0f;
       uint32_t vrun = 0;  // the value code that O refers to
       for (int j = 0; j < it.steps; ++j, ++step) {
-        ok = wait(&bar.s_full[i], step, 3);
+        const uint32_t buf = step & 1u, tb = ts + buf * 64;
+        ok = wait(&bar.s_full[i][buf], step >> 1, 3);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t kref = s_ref[step & 3u][0], vref = s_ref[step & 3u][1];
+        const uint32_t kref = s_ref[step & 7u][0], vref = s_ref[step & 7u][1];
         const float sc = qs * __uint_as_float((127 + kref - 127 - kUp) << 23);
         uint32_t s[kTok];
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c)
-          tc::tmem_ld_32x32b_x32(ts + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
+          tc::tmem_ld_32x32b_x32(tb + 32 * c, reinterpret_cast<uint32_t(&)[32]>(s[32 * c]));
         tc::tmem_ld_wait();
         if ((j + 1) * kTok > all) {
           const int keep = lim - j * kTok;
@@ -563,7 +574,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             c *= j == 0 ? 0.0f : __uint_as_float(uint32_t(max(127 + int(vrun) - int(vref), 0)) << 23);
             vrun = vref;
           }
-          if (j > 0) {  // the products of the steps before are complete: their successor's scores are
+          if (j > 0) {
+            // the products of the step before (those before that are complete: these
+            // scores came after them)
+            ok = wait(&bar.o_done[i][buf ^ 1u], (step - 1) >> 1, 3);
+            if (!ok) break;
+            tc::tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < D / 16; ++x) {
               uint32_t o[16];
@@ -594,14 +610,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             else sum0 = add2(sum0, x);
             p[c] = pack_half(x.x, x.y);
           }
-          tmem_st_x16(ts + 16 * h, p);
+          tmem_st_x16(tb + 16 * h, p);
         }
         sum0 = add2(sum0, sum1);
         l = fmaf(sum0.x + sum0.y, down, l);
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(&bar.p_full[i]);
+        if (lane == 0) tc::mbar_arrive(&bar.p_full[i][buf]);
       }
       if (!ok) break;
       // the next item's rows before this one's sums: its scores can begin
@@ -611,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       if (!ok) break;
       nx = s_item[(n + 1) & 1u];
       if (nx.valid) nqs = load_q(nx);
-      ok = wait(&bar.o_full[i], n, 3);
+      ok = wait(&bar.o_done[i][(step - 1) & 1u], (step - 1) >> 1, 3);
       if (!ok) break;
       tc::tc_fence_after();
       // O 2^(vrun - 127 - kUp) / l
