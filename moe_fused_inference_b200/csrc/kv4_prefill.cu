@@ -114,9 +114,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// tc::mbar_wait for a warp that must stay uniform to the compiler (descriptors in
-// uniform registers): the polls are a loop inside the instruction block.  A poll
-// sleeps in hardware; the limit on their count is above the others' limit in time.
+// Wait for a phase of a barrier, as a whole warp.  The polls are a loop inside the
+// instruction block: few instructions (they take issue slots from the other
+// roles), and no divergence in the compiler's eyes (the issuing warps' descriptors
+// stay in uniform registers).  A poll sleeps in hardware; the count limits them to
+// seconds.
 __device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity, int* err, int code) {
   uint32_t ok;
   asm volatile(
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   // wait for the n-th completion (from 0) of a barrier; the warp goes on or gives
   // up as one
   auto wait = [&](uint64_t* b, uint32_t n, int code) {
-    return __all_sync(0xffffffffu, tc::mbar_wait(b, n & 1u, err, code)) != 0;
+    return wait_uniform(tc::smem_u32(b), n & 1u, err, code);
   };
   // the n-th completion of the barrier of step n's slot
   auto wait_slot = [&](uint64_t* b, uint32_t n, int code) { return wait(b + n % kSlots, n / kSlots, code); };
@@ -295,8 +297,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const uint64_t dv = tc::make_sdesc(base + M::kOffV, kTok * 128, 1024, tc::kLayoutSW128);
       const int i = (warp - 12) >> 1;
       const bool leader = tc::elect_one();
-      auto wait1 = [&](uint64_t* b, uint32_t n) { return wait_uniform(tc::smem_u32(b), n & 1u, err, 2); };
-      auto wait1_slot = [&](uint64_t* b, uint32_t n) { return wait1(b + n % kSlots, n / kSlots); };
       auto commit = [&](uint64_t* b) {
         if (leader) tc::tc_commit(b);
       };
@@ -327,27 +327,27 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       bool ok = true;
       for (uint32_t n = 0; ok; ++n) {
         const uint32_t slot = n & 1u;
-        if (!wait1(&bar.item_full[slot], n >> 1)) break;
+        if (!wait(&bar.item_full[slot], n >> 1, 2)) break;
         const int valid = __shfl_sync(0xffffffffu, s_item[slot].valid, 0);
         const int steps = __shfl_sync(0xffffffffu, s_item[slot].steps, 0);
         tc::mbar_arrive(&bar.item_empty[slot]);
         if (!valid) break;
-        ok = wait1(&bar.q_full[i], n);
+        ok = wait(&bar.q_full[i], n, 2);
         // the scores run two steps ahead of the products
         for (int j = 0; j < 2 && j < steps && ok; ++j) {
-          ok = wait1_slot(bar.k_full, g + j);
+          ok = wait_slot(bar.k_full, g + j, 2);
           if (!ok) break;
           scores(g + j);
           commit(&bar.k_empty[(g + j) % kSlots]);
         }
         for (int j = 0; j < steps && ok; ++j, ++g) {
           const bool more = j + 2 < steps;
-          ok = wait1_slot(bar.v_full, g) && wait1(&bar.p_full[i][g & 1u], g >> 1);
+          ok = wait_slot(bar.v_full, g, 2) && wait(&bar.p_full[i][g & 1u], g >> 1, 2);
           if (!ok) break;
           values(g, j != 0);
           commit(&bar.v_empty[g % kSlots]);
           if (more) {
-            ok = wait1_slot(bar.k_full, g + 2);
+            ok = wait_slot(bar.k_full, g + 2, 2);
             if (!ok) break;
             scores(g + 2);
             commit(&bar.k_empty[(g + 2) % kSlots]);
