@@ -7,7 +7,8 @@
 // 64 a step.  One persistent CTA per SM takes items from a counter, the longest
 // of a sequence first.  Its roles:
 //   warp 13      finds the next item, brings the tokens' tiles in by bulk copies
-//   warps 8-11   decode them to fp16 operands in shared memory (128-byte swizzle)
+//   warp 15      finds the largest codes of a step
+//   warps 8-11   decode its tiles to fp16 operands in shared memory (128-byte swizzle)
 //   warps 12, 14 issue S_i = Q_i K^T of step s + 2 and O_i += P_i V of step s, one
 //                warp a tile i: while one waits the other's products run
 //   warps 0-7    softmax, one thread a vector: S from TMEM, P as fp16 back into
@@ -136,8 +137,9 @@ __device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity, int*
 
 struct Bars {
   uint64_t item_full[2], item_empty[2];            // the next item's description
-  uint64_t raw_full[kSlots], raw_empty[kSlots];    // a step's tiles, operands
-  uint64_t k_full[kSlots], k_empty[kSlots], v_full[kSlots], v_empty[kSlots];
+  uint64_t raw_full[kSlots], raw_empty[kSlots];    // a step's tiles,
+  uint64_t ref_full[kSlots];                       // its codes' references,
+  uint64_t kv_full[kSlots], kv_empty[kSlots];      // its operands
   uint64_t q_full[2];                              // of tile i: query rows written,
   uint64_t s_full[2][2], p_full[2][2];             // scores there, weights there (by step & 1),
   uint64_t o_done[2][2];                           // products added (by step & 1)
@@ -152,7 +154,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   __shared__ Bars bar;
   __shared__ Item s_item[2];
   __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN
-  __shared__ uint32_t s_ref[8][2];  // of a step: the key and value codes that its operands refer to
+  // of a step: the key and value codes that its operands refer to, whether there
+  // are NaN values.  Its writer is at most 2 kSlots steps ahead of its last reader.
+  __shared__ uint4 s_ref[4 * kSlots];
   __shared__ uint32_t s_tmem;
   // (from lane 0: the roles' branches are then known to be uniform)
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     tc::cta_abort_init();
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(&bar.item_full[i], 1);
-      tc::mbar_init(&bar.item_empty[i], 8 + 4 + 64);  // a lane of each warp that reads it, all of warps 12 and 14
+      tc::mbar_init(&bar.item_empty[i], 8 + 4 + 1 + 64);  // a lane of each warp that reads it, all of warps 12 and 14
       tc::mbar_init(&bar.drain[i], 1);
       tc::mbar_init(&bar.q_full[i], 4);
       for (int b = 0; b < 2; ++b) {
@@ -174,10 +178,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     for (int i = 0; i < kSlots; ++i) {
       tc::mbar_init(&bar.raw_full[i], 1);
       tc::mbar_init(&bar.raw_empty[i], 4);
-      tc::mbar_init(&bar.k_full[i], 4);
-      tc::mbar_init(&bar.k_empty[i], 2);
-      tc::mbar_init(&bar.v_full[i], 4);
-      tc::mbar_init(&bar.v_empty[i], 2);
+      tc::mbar_init(&bar.ref_full[i], 1);
+      tc::mbar_init(&bar.kv_full[i], 4);
+      tc::mbar_init(&bar.kv_empty[i], 2);
     }
     tc::fence_mbar_init();
   }
@@ -335,142 +338,149 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         ok = wait(&bar.q_full[i], n, 2);
         // the scores run two steps ahead of the products
         for (int j = 0; j < 2 && j < steps && ok; ++j) {
-          ok = wait_slot(bar.k_full, g + j, 2);
+          ok = wait_slot(bar.kv_full, g + j, 2);
           if (!ok) break;
           scores(g + j);
-          commit(&bar.k_empty[(g + j) % kSlots]);
         }
         for (int j = 0; j < steps && ok; ++j, ++g) {
           const bool more = j + 2 < steps;
-          ok = wait_slot(bar.v_full, g, 2) && wait(&bar.p_full[i][g & 1u], g >> 1, 2);
+          ok = wait(&bar.p_full[i][g & 1u], g >> 1, 2);
           if (!ok) break;
           values(g, j != 0);
-          commit(&bar.v_empty[g % kSlots]);
+          commit(&bar.kv_empty[g % kSlots]);  // of its keys too: their scores came before
           if (more) {
-            ok = wait_slot(bar.k_full, g + 2, 2);
+            ok = wait_slot(bar.kv_full, g + 2, 2);
             if (!ok) break;
             scores(g + 2);
-            commit(&bar.k_empty[(g + 2) % kSlots]);
           }
         }
       }
       if (tc::cta_aborted() && leader) tc::drain_mma(&bar.drain[i]);
+    } else if (warp == 15) {
+      // ---- the largest codes (255, NaN, not counted): of the step's keys, of the
+      // item's values so far
+      uint32_t step = 0;
+      bool ok = true;
+      for (uint32_t n = 0; ok; ++n) {
+        const uint32_t slot = n & 1u;
+        if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
+        const int len = s_item[slot].len, valid = s_item[slot].valid;
+        const int steps = s_item[slot].steps;
+        uint32_t vtop = 28u;  // a block of zeros
+        for (int j = 0; valid && j < steps; ++j, ++step) {
+          ok = wait_slot(bar.raw_full, step, 1);
+          if (!ok) break;
+          const uint8_t* raw = smem + M::kOffRaw + (step % kSlots) * M::kRaw;
+          uint32_t ref[2];
+          bool nan[2];
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            uint32_t w[kTok / 32], m = 0;  // codes of tokens lane, lane + 32
+#pragma unroll
+            for (int x = 0; x < kTok / 32; ++x) {
+              const int tok = x * 32 + lane;
+              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
+              w[x] = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+              if (j * kTok + tok >= len) w[x] = 0u;
+              m = __vmaxu2(__vmaxu2(m, w[x] & 0x00FF00FFu), (w[x] >> 8) & 0x00FF00FFu);
+            }
+            m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+            nan[kv] = m == 255u;
+            if (nan[kv]) {  // rare: once more without them
+              m = 0;
+#pragma unroll
+              for (int x = 0; x < kTok / 32; ++x) {
+                const uint32_t bad = __vcmpeq4(w[x], 0xFFFFFFFFu);
+                // a NaN value block counts for the rows that see it only: noted here,
+                // written at the end, and zero in the product
+                for (int b = 0; b < nb; ++b)
+                  if (kv && ((bad >> (8 * b)) & 1u)) atomicMin(&s_nan[slot][b], j * kTok + x * 32 + lane);
+                w[x] &= ~bad;
+                m = __vmaxu2(__vmaxu2(m, w[x] & 0x00FF00FFu), (w[x] >> 8) & 0x00FF00FFu);
+              }
+              m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+            }
+            ref[kv] = max(m, 28u);
+          }
+          vtop = max(vtop, ref[1]);
+          __syncwarp();
+          if (lane == 0) {
+            s_ref[step % (4 * kSlots)] = make_uint4(ref[0], vtop, nan[1], 0u);
+            tc::mbar_arrive(&bar.ref_full[step % kSlots]);
+          }
+        }
+        if (lane == 0) tc::mbar_arrive(&bar.item_empty[slot]);
+        if (!valid) break;
+      }
     }
   } else if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsDecode));
-    // ---- decode: lane (row, quarter t of the row) of 8 rows at a time, rows r
-    // and r + 4 side by side: their swizzled chunks share no banks
+    // ---- decode: a warp a tile; lane (row, quarter t of the row) of 8 rows at a
+    // time, rows r and r + 4 side by side: their swizzled chunks share no banks
+    constexpr int kMine = kTok / 4;
+    static_assert(kMine == kTile, "a tile a warp");
     const int dw = warp - 8, t = lane & 3, r8 = ((lane >> 2) & 1) * 4 + (lane >> 3);
-    constexpr int kMine = kTok / 4;                             // a warp's tokens: one tile
-    const int at = (dw * kMine + r8) * 128 + ((t ^ r8) << 4);  // operand_at(dw * kMine + r8, t)
+    const int at = (dw * kMine + r8) * 128 + ((t ^ r8) << 4);  // of the row's chunk t
     uint32_t step = 0;
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
       if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
       const int len = s_item[slot].len, steps = s_item[slot].steps, valid = s_item[slot].valid;
       bool ok = true;
-      uint32_t vtop = 28u;
-      if (valid) {
-        for (int j = 0; j < steps; ++j, ++step) {
-          const uint32_t st = step % kSlots;
-          ok = wait_slot(bar.raw_full, step, 1);
-          if (!ok) break;
-          const uint8_t* raw = smem + M::kOffRaw + st * M::kRaw;
-          const int pos0 = j * kTok;
-          // the largest codes (255, NaN, not counted) of the step's keys and of the
-          // item's values so far, by every warp
-          uint32_t ref[2];
-          bool nan[2];
+      for (int j = 0; valid && j < steps; ++j, ++step) {
+        const uint32_t st = step % kSlots;
+        ok = wait(&bar.ref_full[st], step / kSlots, 1);
+        if (!ok) break;
+        const uint4 ref = s_ref[step % (4 * kSlots)];
+        const uint8_t* tile = smem + M::kOffRaw + st * M::kRaw + dw * tile_bytes(D);
+        uint32_t w[2][2][nb], cw[2][2];  // of key and value rows r8, r8 + 8
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            auto code_word = [&](int x) {
-              const int tok = x * 32 + lane;
-              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
-              const uint32_t w = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-              return pos0 + tok < len ? w : 0u;
-            };
-            uint32_t m = 0;
+        for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
-            for (int x = 0; x < kTok / 32; ++x) {
-              const uint32_t w = code_word(x);
-              m = __vmaxu2(__vmaxu2(m, w & 0x00FF00FFu), (w >> 8) & 0x00FF00FFu);
+          for (int x = 0; x < 2; ++x) {
+            const int in = x * 8 + r8;
+            const uint8_t* c = tile + 16 * D + kv * (D / 2) + in * nb;
+            cw[kv][x] = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+            if (j * kTok + dw * kMine + in >= len) cw[kv][x] = 0;
+            const uint8_t* src = tile + kv * 8 * D + in * (D / 2) + t * (4 * nb);
+            if (nb == 4) {
+              const uint4 y = *reinterpret_cast<const uint4*>(src);
+              w[kv][x][0] = y.x; w[kv][x][1] = y.y; w[kv][x][nb - 2] = y.z; w[kv][x][nb - 1] = y.w;
+            } else {
+              const uint2 y = *reinterpret_cast<const uint2*>(src);
+              w[kv][x][0] = y.x; w[kv][x][1] = y.y;
             }
-            m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
-            nan[kv] = m == 255u;
-            if (nan[kv]) {  // rare: once more without them
-              m = 0;
-#pragma unroll 1
-              for (int x = 0; x < kTok / 32; ++x) {
-                uint32_t w = code_word(x);
-                w &= ~__vcmpeq4(w, 0xFFFFFFFFu);
-                m = __vmaxu2(__vmaxu2(m, w & 0x00FF00FFu), (w >> 8) & 0x00FF00FFu);
-              }
-              m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+          }
+        ok = step < kSlots || wait_slot(bar.kv_empty, step - kSlots, 1);
+        if (!ok) break;
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const uint32_t dst = (kv ? M::kOffV : M::kOffK) + st * M::kOperand + at;
+          const float u = __uint_as_float((127 + 127 + kUp - (kv ? ref.y : ref.x)) << 23);  // 2^(127 + kUp - ref)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (kv && ref.z) cw[kv][x] &= ~__vcmpeq4(cw[kv][x], 0xFFFFFFFFu);
+            float f[nb];
+            codes<nb>(cw[kv][x], f);
+#pragma unroll
+            for (int b = 0; b < nb; ++b) {
+              const uint32_t h = pack_half(f[b] * u, f[b] * u);
+              // values: pieces 2t and 2t + 1 of a block make its 8 elements
+              const uint32_t e = kv ? __byte_perm(w[kv][x][b / 2], w[kv][x][nb / 2 + b / 2], b % 2 ? 0x7632 : 0x5410)
+                                    : w[kv][x][b];
+              uint32_t o[4];
+              e2m1x8(e, o);
+              // chunk 4b + t of the row
+              *reinterpret_cast<uint4*>(smem + (b % 2 ? dst ^ 64u : dst) + (b / 2) * (kTok * 128) + x * 1024) =
+                  make_uint4(mul_half2(o[0], h), mul_half2(o[1], h), mul_half2(o[2], h), mul_half2(o[3], h));
             }
-            ref[kv] = max(m, 28u);
           }
-          ref[1] = vtop = max(ref[1], vtop);
-          if (dw == 0 && lane == 0) {
-            s_ref[step & 7u][0] = ref[0];
-            s_ref[step & 7u][1] = ref[1];
-          }
-#pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            ok = step < kSlots || wait_slot(kv ? bar.v_empty : bar.k_empty, step - kSlots, 1);
-            if (!ok) break;
-            uint8_t* dst = smem + (kv ? M::kOffV : M::kOffK) + st * M::kOperand;
-            const float u = __uint_as_float((127 + 127 + kUp - ref[kv]) << 23);  // 2^(127 + kUp - ref)
-#pragma unroll
-            for (int x = 0; x < kMine / 8; ++x) {
-              const int row = dw * kMine + x * 8 + r8, in = x * 8 + r8;  // token of the step, of the tile
-              const uint8_t* tile = raw + dw * tile_bytes(D);
-              const uint8_t* c = tile + 16 * D + kv * (D / 2) + in * nb;
-              uint32_t cw = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-              uint32_t w[nb];
-              const uint8_t* src = tile + kv * 8 * D + in * (D / 2) + t * (4 * nb);
-              if (nb == 4) {
-                const uint4 y = *reinterpret_cast<const uint4*>(src);
-                w[0] = y.x; w[1] = y.y; w[nb - 2] = y.z; w[nb - 1] = y.w;
-              } else {
-                const uint2 y = *reinterpret_cast<const uint2*>(src);
-                w[0] = y.x; w[1] = y.y;
-              }
-              if (pos0 + row >= len) cw = 0;
-              if (kv) {
-                // pieces 2t and 2t + 1 of the blocks to the blocks' 8 elements
-                uint32_t y[nb];
-#pragma unroll
-                for (int b = 0; b < nb; ++b)
-                  y[b] = __byte_perm(w[b / 2], w[nb / 2 + b / 2], b % 2 ? 0x7632 : 0x5410);
-#pragma unroll
-                for (int b = 0; b < nb; ++b) w[b] = y[b];
-                if (nan[1]) {
-                  // a NaN block counts for the rows that see it only: noted here,
-                  // written at the end, and zero in the product
-                  const uint32_t bad = __vcmpeq4(cw, 0xFFFFFFFFu);
-                  for (int b = 0; b < nb; ++b)
-                    if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[slot][b], pos0 + row);
-                  cw &= ~bad;
-                }
-              }
-              float f[nb];
-              codes<nb>(cw, f);
-#pragma unroll
-              for (int b = 0; b < nb; ++b) {
-                const uint32_t h = pack_half(f[b] * u, f[b] * u);
-                uint32_t o[4];
-                e2m1x8(w[b], o);
-                // chunk 4b + t of the row
-                *reinterpret_cast<uint4*>(dst + (b / 2) * (kTok * 128) + x * 1024 + (b % 2 ? at ^ 64 : at)) =
-                    make_uint4(mul_half2(o[0], h), mul_half2(o[1], h), mul_half2(o[2], h), mul_half2(o[3], h));
-              }
-            }
-            tc::fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(kv ? &bar.v_full[st] : &bar.k_full[st]);
-          }
-          if (!ok) break;
-          if (lane == 0) tc::mbar_arrive(&bar.raw_empty[st]);
+        }
+        tc::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tc::mbar_arrive(&bar.kv_full[st]);
+          tc::mbar_arrive(&bar.raw_empty[st]);
         }
       }
       if (lane == 0) tc::mbar_arrive(&bar.item_empty[slot]);
@@ -544,7 +554,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         ok = wait(&bar.s_full[i][buf], step >> 1, 3);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t kref = s_ref[step & 7u][0], vref = s_ref[step & 7u][1];
+        const uint32_t kref = s_ref[step % (4 * kSlots)].x, vref = s_ref[step % (4 * kSlots)].y;
         const float sc = qs * __uint_as_float((127 + kref - 127 - kUp) << 23);
         uint32_t s[kTok];
 #pragma unroll
