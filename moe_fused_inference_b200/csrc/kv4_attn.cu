@@ -785,8 +785,6 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
 // 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
 // are then read and decoded half as often), else 8.  Sequences of more than
 // kFew vectors go to the kernel for many rows, whose tile is 256 vectors.
-constexpr int kFew = 64;
-
 template <class E, int D>
 cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
@@ -803,7 +801,8 @@ cudaError_t launch(AttnArgs& a, cudaStream_t s) {
 extern "C" size_t mfi_kv4_attn_workspace_bytes(int n_seq, int Hq, int Hkv, int D, int max_q) {
   if (n_seq <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128) || max_q <= 0)
     return 0;
-  return mfi::kv4::kCounterBytes + size_t(mfi::kv4::kCtas) * 2 * 16 * (D + 4) * sizeof(float);
+  const bool many = (long long)max_q * (Hq / Hkv) > mfi::kv4::kFew;
+  return mfi::kv4::kCounterBytes + (many ? mfi::kv4::many_bytes(D) : mfi::kv4::few_bytes(D));
 }
 
 extern "C" int mfi_kv4_attn_init_workspace(void* workspace, size_t workspace_bytes, void* stream) {

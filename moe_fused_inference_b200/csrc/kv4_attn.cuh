@@ -16,8 +16,8 @@ struct AttnArgs {
   const int* cu_q;           // (n_seq + 1) or null: max_q rows each
   void* out;                 // (T, Hq, D)
   int* err;
-  unsigned* counters;        // kCounters words, zero between calls
-  float* part;               // two slots per CTA
+  unsigned* counters;        // kCounterBytes, zero between calls
+  float* part;               // few_bytes or many_bytes
   int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
   int few;                   // sequences of up to this many vectors (rows x heads of a group) are `few`
   bool q_vec;                // every query row starts on a 16-byte boundary
@@ -49,9 +49,16 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 
 
 constexpr int kCtas = 148;                 // one per SM
-constexpr size_t kCounterBytes = 1024;
-constexpr int kItemCounter = kCtas, kDoneCounter = kCtas + 1;  // of the kernel for many rows
-static_assert(kCounterBytes >= (kCtas + 2) * sizeof(unsigned), "a counter per CTA and two more");
+// Words of the workspace's head, zero between calls: one per CTA (few rows); for
+// many rows the next item, the CTAs that are done, and one per part and warp.
+constexpr int kItemCounter = kCtas, kDoneCounter = kCtas + 1, kPartCounters = kCtas + 2;
+constexpr size_t kCounterBytes = 8192;
+static_assert(kCounterBytes >= (kPartCounters + 8 * kCtas) * sizeof(unsigned), "room for the counters");
+constexpr int kFew = 64;                   // vectors of a sequence and KV head that are few rows
+
+// Bytes of the sums that parts of a piece or item leave for each other.
+constexpr size_t few_bytes(int D) { return size_t(kCtas) * 2 * 16 * (D + 4) * sizeof(float); }
+constexpr size_t many_bytes(int D) { return size_t(kCtas) * 256 * (D + 2) * sizeof(float); }
 
 __device__ __forceinline__ float ex2(float x) {
   float r;

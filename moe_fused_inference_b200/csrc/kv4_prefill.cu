@@ -5,7 +5,8 @@
 // A vector is one row of one query head; an item is 256 vectors (two tiles of
 // 128) of a sequence and KV head, against the tokens that the last of them sees,
 // 64 a step.  One persistent CTA per SM takes items from a counter, the longest
-// of a sequence first.  Its roles:
+// of a sequence first.  With fewer items than CTAs the tokens of each are split
+// into parts, whose sums the last part's warps join.  A CTA's roles:
 //   warp 13      finds the next item, brings the tokens' tiles in by bulk copies
 //   warp 15      finds the largest codes of a step
 //   warps 8-11   decode its tiles to fp16 operands in shared memory (128-byte swizzle)
@@ -63,8 +64,15 @@ struct Many {
 };
 
 struct Item {
-  int valid, seq, row0, rows, len, g, v0, steps;
+  int valid, seq, row0, rows, len, g, v0;
+  int step0, steps;         // of this part
+  int part, parts, index;   // the part's index among all parts of the call
 };
+
+// Parts of an item: no more than the CTAs allow, of at least kMinSteps steps (a
+// part starts in about 5 us, 8 steps take about as long), at most kMaxParts (they
+// are joined by one CTA's warps).
+constexpr int kMinSteps = 8, kMaxParts = 12;
 
 // An operand of R rows: halves of 64 elements, each R rows of 128 bytes in the
 // 128-byte swizzle.  Byte offset of 16-byte chunk c (8 elements) of row r:
@@ -207,6 +215,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const int tpp = a.page / kTile;
       const uint64_t page_bytes = uint64_t(a.Hkv) * tpp * tile_bytes(D);
       uint32_t step = 0, filled = 0;
+      auto items_of = [&](const Seq& s) {
+        return s.rows * G > a.few ? unsigned((s.rows * G + 2 * kRows - 1) / (2 * kRows)) * a.Hkv : 0u;
+      };
+      unsigned all_items = 0;
+      for (int i = lane; i < a.n_seq; i += 32) all_items += items_of(sequence(a, i));
+      all_items = __reduce_add_sync(0xffffffffu, all_items);
+      const int most = all_items ? min(kMaxParts, int(gridDim.x / all_items)) : 0;
+      // the same for all items of a sequence; none is left without a step: the item
+      // of the first rows sees len - rows + 1 tokens at least
+      auto parts_of = [&](const Seq& s) {
+        const int few_steps = (s.len - s.rows) / kTok;
+        return unsigned(max(1, min(most, few_steps / kMinSteps)));
+      };
       for (uint32_t n = 0;; ++n) {
         unsigned idx = 0;
         if (lane == 0) idx = atomicAdd(a.counters + kItemCounter, 1u);
@@ -216,8 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         for (int i0 = 0; i0 < a.n_seq; i0 += 32) {
           const int i = i0 + lane;
           const Seq s = i < a.n_seq ? sequence(a, i) : Seq{0, 0, 0};
-          const unsigned items =
-              s.rows * G > a.few ? unsigned((s.rows * G + 2 * kRows - 1) / (2 * kRows)) * a.Hkv : 0u;
+          const unsigned parts = parts_of(s), items = items_of(s) * parts;
           unsigned start = items;
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) {
@@ -234,12 +254,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             it.row0 = __shfl_sync(0xffffffffu, s.row0, src);
             it.rows = __shfl_sync(0xffffffffu, s.rows, src);
             it.len = __shfl_sync(0xffffffffu, s.len, src);
+            it.parts = int(__shfl_sync(0xffffffffu, parts, src));
+            const unsigned all = __shfl_sync(0xffffffffu, items, src) / it.parts;
             const unsigned in = idx - __shfl_sync(0xffffffffu, start, src);
-            const unsigned pairs = __shfl_sync(0xffffffffu, items, src) / a.Hkv;
-            it.g = int(in % a.Hkv);
-            it.v0 = int(pairs - 1 - in / a.Hkv) * 2 * kRows;  // the rows that see most first
+            it.part = int(in % it.parts);
+            it.index = int(idx);
+            const unsigned item = in / it.parts;
+            it.g = int(item % a.Hkv);
+            it.v0 = int(all / a.Hkv - 1 - item / a.Hkv) * 2 * kRows;  // the rows that see most first
             const int last = min(it.v0 + 2 * kRows, it.rows * G) - 1;
-            it.steps = max(1, (it.len - it.rows + last / G + 1 + kTok - 1) / kTok);
+            const int steps = max(1, (it.len - it.rows + last / G + 1 + kTok - 1) / kTok);
+            it.step0 = int((long long)steps * it.part / it.parts);
+            it.steps = int((long long)steps * (it.part + 1) / it.parts) - it.step0;
             break;
           }
           before += sum;
@@ -258,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           return lane < kTok / kTile && t < have ? __ldg(row + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp))
                                                  : -1;
         };
-        int t = lane, id = page_of(t);
+        int t = it.step0 * (kTok / kTile) + lane, id = page_of(t);
         bool ok = true;
         for (int j = 0; j < it.steps; ++j, ++step) {
           const uint32_t st = step % kSlots;
@@ -365,8 +391,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       for (uint32_t n = 0; ok; ++n) {
         const uint32_t slot = n & 1u;
         if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
-        const int len = s_item[slot].len, valid = s_item[slot].valid;
-        const int steps = s_item[slot].steps;
+        const int valid = s_item[slot].valid, steps = s_item[slot].steps;
+        const int pos = s_item[slot].step0 * kTok, len = s_item[slot].len - pos;  // of the part
         uint32_t vtop = 28u;  // a block of zeros
         for (int j = 0; valid && j < steps; ++j, ++step) {
           ok = wait_slot(bar.raw_full, step, 1);
@@ -395,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
                 // a NaN value block counts for the rows that see it only: noted here,
                 // written at the end, and zero in the product
                 for (int b = 0; b < nb; ++b)
-                  if (kv && ((bad >> (8 * b)) & 1u)) atomicMin(&s_nan[slot][b], j * kTok + x * 32 + lane);
+                  if (kv && ((bad >> (8 * b)) & 1u)) atomicMin(&s_nan[slot][b], pos + j * kTok + x * 32 + lane);
                 w[x] &= ~bad;
                 m = __vmaxu2(__vmaxu2(m, w[x] & 0x00FF00FFu), (w[x] >> 8) & 0x00FF00FFu);
               }
@@ -426,7 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     for (uint32_t n = 0;; ++n) {
       const uint32_t slot = n & 1u;
       if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
-      const int len = s_item[slot].len, steps = s_item[slot].steps, valid = s_item[slot].valid;
+      const int steps = s_item[slot].steps, valid = s_item[slot].valid;
+      const int len = s_item[slot].len - s_item[slot].step0 * kTok;  // of the part on
       bool ok = true;
       for (int j = 0; valid && j < steps; ++j, ++step) {
         const uint32_t st = step % kSlots;
@@ -546,8 +573,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     }
     for (uint32_t n = 0; ok && it.valid; ++n) {
       const int v = it.v0 + i * kRows + r, nv = it.rows * G;
-      const int lim = v < nv ? it.len - it.rows + v / G + 1 : 0;     // tokens that this vector sees
-      const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1;  // that all of the tile see
+      // tokens, from the part's first on, that this vector sees, that all of the tile see
+      const int pos = it.step0 * kTok;
+      const int lim = v < nv ? it.len - it.rows + v / G + 1 - pos : 0;
+      const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1 - pos;
       float m = -INFINITY, l = 0.0f;
       uint32_t vrun = 0;  // the value code that O refers to
       for (int j = 0; j < it.steps; ++j, ++step) {
@@ -641,24 +670,76 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       ok = wait(&bar.o_done[i][(step - 1) & 1u], (step - 1) >> 1, 3);
       if (!ok) break;
       tc::tc_fence_after();
-      // O 2^(vrun - 127 - kUp) / l
-      const float inv = l == 0.0f ? 0.0f : __uint_as_float((vrun - kUp) << 23) / l;
+      const float unit = __uint_as_float((vrun - kUp) << 23);  // O's: 2^(vrun - 127 - kUp)
+      const float nan = __uint_as_float(0x7FC00000u);
       E* out = static_cast<E*>(a.out) +
                ((long long)(it.row0 + v / G) * a.Hq + it.g * G + v % G) * D;
+      // a part leaves [D + 2][256 vectors] sums
+      float* sums = a.part + size_t(it.index) * (256 * (D + 2)) + i * kRows + r;
+      const float inv = it.parts > 1 ? unit : (l == 0.0f ? 0.0f : unit / l);
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
         tc::tmem_ld_32x32b_x32(to + 32 * x, o);
         tc::tmem_ld_wait();
-        const bool bad = lim > s_nan[n & 1u][x];
-        if (v < nv) {
+        const bool bad = lim + pos > s_nan[n & 1u][x];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(bad ? nan : __uint_as_float(o[k]) * inv);
+        if (it.parts > 1) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) __stcg(sums + (32 * x + k) * 256, __uint_as_float(o[k]));
+        } else if (v < nv) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             __align__(16) E y[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              y[k] = E(bad ? __uint_as_float(0x7FC00000u) : __uint_as_float(o[8 * c + k]) * inv);
+            for (int k = 0; k < 8; ++k) y[k] = E(__uint_as_float(o[8 * c + k]));
             *reinterpret_cast<uint4*>(out + 32 * x + 8 * c) = *reinterpret_cast<const uint4*>(y);
+          }
+        }
+      }
+      if (it.parts > 1) {
+        __stcg(sums + D * 256, m);
+        __stcg(sums + (D + 1) * 256, l);
+        __threadfence();
+        __syncwarp();
+        unsigned last = 0;
+        if (lane == 0) {
+          unsigned* c = a.counters + kPartCounters + (it.index - it.part) * 8 + warp;
+          last = atomicInc(c, it.parts - 1) == unsigned(it.parts - 1);
+          __threadfence();
+        }
+        last = __shfl_sync(0xffffffffu, last, 0);
+        if (last) {  // the last of the parts' warps with these vectors joins them, in the parts' order
+          const float* from = sums - size_t(it.part) * (256 * (D + 2));
+          auto at = [&](int part, int c) { return __ldcg(from + size_t(part) * (256 * (D + 2)) + c * 256); };
+          float top = -INFINITY, sum = 0.0f, w[kMaxParts];
+#pragma unroll
+          for (int k = 0; k < kMaxParts; ++k) {
+            w[k] = k < it.parts ? at(k, D) : -INFINITY;
+            top = fmaxf(top, w[k]);
+          }
+#pragma unroll
+          for (int k = 0; k < kMaxParts; ++k) {
+            w[k] = ex2(w[k] - (top == -INFINITY ? 0.0f : top));
+            if (k < it.parts) sum = fmaf(w[k], at(k, D + 1), sum);
+          }
+          const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 8) {
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < kMaxParts; ++k)
+              if (k < it.parts) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = fmaf(w[k], at(k, c + e), x[e]);
+              }
+            if (v < nv) {
+              __align__(16) E y[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] = E(x[e] * scale);
+              *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(y);
+            }
           }
         }
       }

@@ -197,6 +197,9 @@ CASES = [
     ([257], [700], 1, 2, 64, 48),
     ([129, 3, 300], [400, 3, 300], 1, 5, 128, 32),
     ([200], [1500], 2, 3, 64, 1024),
+    ([100], [3050], 1, 8, 128, 64),                       # few items: their tokens in parts
+    ([70, 1, 90, 2], [5000, 900, 90, 1], 1, 4, 64, 16),   # parts, whole items and few rows together
+    ([40, 40], [8000, 4100], 2, 2, 128, 48),
 ]
 
 
