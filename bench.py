@@ -99,6 +99,8 @@ def parse():
                          "(p2p) or two NCCL all_to_all_single calls (nccl)")
     ap.add_argument("--no-graph", action="store_true",
                     help="time plain launches instead of a captured CUDA graph")
+    ap.add_argument("--kv", choices=["fp8", "mxfp4"], default="fp8",
+                    help="KV cache of --workload model")
     ap.add_argument("--impl", choices=["ours", "reference"], default="ours")
     ap.add_argument("--cpu-sample-s", type=float, default=12.0,
                     help="seconds of CPU work for each cpu_baseline sample")
@@ -817,7 +819,7 @@ def run_model(args, world, rank, local):
     sampler.start()
     for B in (1, 16, 64):
         prompt = synthetic_prompts(B, P, model.cfg.vocab, seed=101 + B, device=dev)
-        runner = Runner(model, lib, B, P + S + 8)
+        runner = Runner(model, lib, B, P + S + 8, kv=args.kv)
         e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         e0.record(stream)
         runner.prefill(prompt)
@@ -844,7 +846,8 @@ def run_model(args, world, rank, local):
         "value": per["B64"]["decode_tokens_per_s"], "unit": "tokens/s", "n_gpus": 1,
         "steps": S, "warmup": 1, "ms_per_step": per["B64"]["ms_per_step"],
         "higher_is_better": True, "scaling": "weak", "vs_baseline": None,
-        "dtype": "mxfp4 experts and projections, bf16 activations, FP8 KV cache",
+        "dtype": "mxfp4 experts and projections, bf16 activations, "
+                 + ("FP8 KV cache" if args.kv == "fp8" else "MXFP4 KV cache"),
         "data": "synthetic (random-init weights, uniform random prompts with a repeated "
                 "32-token motif, seeded)",
         "config": {"workload": "config 4: 48 layers, 32/4 heads, head_dim 128, vocab 151936, "

@@ -27,6 +27,10 @@ operators (fp4_ext: prequant, lin_pq, attn_decode).  A test backend with the
 same interface restates the operators in torch (dequantise, fp32 matmul) so
 greedy token ids can be compared step by step.
 
+``Runner(kv="mxfp4")`` holds the keys and values in paged 4-bit caches instead
+(kv4.py: half the bytes of FP8), written and attended to by ``kv4_write`` and
+``kv4_attention``; prompts of any chunk size then run on the tensor cores.
+
 Weights are random-init (N(0, 0.02), the norms 1 + N(0, 0.02)), quantised on
 the device; there is no checkpoint or tokenizer on this path.
 """
@@ -38,6 +42,7 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn.functional as F
 
+from . import kv4
 from .layer import MoELayer, MoELayerWeights, quantize_rows, random_layer_weights
 
 
@@ -200,14 +205,37 @@ class LibBackend:
             "attn_decode_batched")
         return o
 
+    def write_kv4(self, cache, k, v, slots):
+        """Rows k, v (T, Hkv, D) into the 4-bit cache's tokens `slots`."""
+        kv4.kv4_write(cache, k, v, slots)
+
+    def attention_kv4(self, q, cache, table, lens, M, workspace):
+        """q (B * M, Hq, D): the last M of each sequence's lens tokens attend to
+        its pages of the 4-bit cache."""
+        return kv4.kv4_attention(q, cache, table, lens, workspace=workspace)
+
 
 class Runner:
-    """B sequences of the synthetic model with per-sequence FP8 KV caches."""
+    """B sequences of the synthetic model with per-sequence KV caches: FP8
+    (``kv="fp8"``) or paged 4-bit (``kv="mxfp4"``, pages of ``page`` tokens, each
+    sequence's pages dealt in turn as a pool that serves requests would)."""
 
-    def __init__(self, model: SyntheticQwen, backend, batch: int, max_len: int):
+    def __init__(self, model: SyntheticQwen, backend, batch: int, max_len: int, kv: str = "fp8",
+                 page: int = 64):
         cfg = model.cfg
         self.model, self.be, self.B, self.max_len = model, backend, batch, max_len
         dev = model.final_norm.device
+        if kv not in ("fp8", "mxfp4"):
+            raise RuntimeError("kv must be 'fp8' or 'mxfp4'")
+        self.kv4 = None
+        if kv == "mxfp4":
+            per = -(-max_len // page)
+            self.page = page
+            self.kv4 = [kv4.KV4Cache(batch * per, page, cfg.kv_heads, cfg.head_dim, device=dev)
+                        for _ in range(cfg.layers)]
+            self.table = torch.arange(batch * per, dtype=torch.int32, device=dev).view(per, batch).t().contiguous()
+            self._kv4_ws = {}
+            return
         shape = (cfg.layers, batch, max_len, cfg.kv_heads, cfg.head_dim)
         self.kvk = torch.zeros(shape, dtype=torch.uint8, device=dev)
         self.kvv = torch.zeros(shape, dtype=torch.uint8, device=dev)
@@ -230,6 +258,13 @@ class Runner:
             positions = kv_idx.repeat(B)
         else:
             positions = torch.arange(base, base + M, device=ids.device).repeat(B)
+        if self.kv4 is not None:
+            # the rows' places in the pool and the sequences' lengths, for all layers
+            pos = positions.view(B, M).long()
+            slots = (self.table.gather(1, pos // self.page).long() * self.page + pos % self.page).view(-1)
+            lens = (pos[:, -1] + 1).int()
+            if M not in self._kv4_ws:
+                self._kv4_ws[M] = kv4.attention_workspace(B, Hq, self.kv4[0], M)
         routing = []
         for L, lw in enumerate(m.layers):
             hp = rms_norm(x, lw.in_norm, cfg.eps)
@@ -242,6 +277,11 @@ class Runner:
             v = v.view(T, Hkv, D).bfloat16()
             q = apply_rope(q, positions, cfg.rope_theta)
             k = apply_rope(k, positions, cfg.rope_theta)
+            if self.kv4 is not None:
+                be.write_kv4(self.kv4[L], k, v, slots)
+                o = be.attention_kv4(q, self.kv4[L], self.table, lens, M, self._kv4_ws[M])
+                x = self._after_attention(x, o, lw, L, T, trace, routing)
+                continue
             kb = k.view(B, M, Hkv, D)
             vb = v.view(B, M, Hkv, D)
             k8 = kb.to(torch.float8_e4m3fn).view(torch.uint8)
@@ -253,23 +293,29 @@ class Runner:
                 self.kvk[L, :, base:base + M] = k8
                 self.kvv[L, :, base:base + M] = v8
             o = be.attention(q.view(B, M, Hq, D), self.kvk[L], self.kvv[L], base, M)
-            of = o.reshape(T, Hq * D).to(torch.bfloat16).contiguous()
-            aq, asc = be.prequant(of)
-            x = x + be.linear(aq, asc, lw.o, T, H, Hq * D).bfloat16()
-            if trace is not None:
-                trace.append(("attn", L, x.clone()))
-            h2 = rms_norm(x, lw.post_norm, cfg.eps)
-            moe, topi = be.moe_block(L, h2)
-            x = x + moe.bfloat16()
-            routing.append(topi)
-            if trace is not None:
-                trace.append(("moe", L, x.clone()))
+            x = self._after_attention(x, o, lw, L, T, trace, routing)
         if last_only:
             x = x.view(B, M, H)[:, -1]
         xn = rms_norm(x, m.final_norm, cfg.eps)
         lq, ls = be.prequant(xn.contiguous())
         logits = be.linear(lq, ls, m.lm_head, xn.shape[0], cfg.vocab, H)
         return (logits if last_only else logits.view(B, M, cfg.vocab)), routing
+
+    def _after_attention(self, x, o, lw, L, T, trace, routing):
+        """The rest of layer L: o projection, residual, MoE block."""
+        cfg, be = self.model.cfg, self.be
+        of = o.reshape(T, cfg.heads * cfg.head_dim).to(torch.bfloat16).contiguous()
+        aq, asc = be.prequant(of)
+        x = x + be.linear(aq, asc, lw.o, T, cfg.hidden, cfg.heads * cfg.head_dim).bfloat16()
+        if trace is not None:
+            trace.append(("attn", L, x.clone()))
+        h2 = rms_norm(x, lw.post_norm, cfg.eps)
+        moe, topi = be.moe_block(L, h2)
+        x = x + moe.bfloat16()
+        routing.append(topi)
+        if trace is not None:
+            trace.append(("moe", L, x.clone()))
+        return x
 
     # ---- generation ------------------------------------------------------
     def prefill(self, prompt: torch.Tensor, chunk: int = 64) -> None:
