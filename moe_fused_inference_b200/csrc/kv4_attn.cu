@@ -45,10 +45,12 @@ using namespace kv4;
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
 constexpr int kStages = 2;   // one read, one on its way
 constexpr unsigned kSnap = 32;  // tiles
+constexpr int kOneLevel = 8;    // parts
 
 template <int D, int kNT>
 struct Few {
-  static constexpr int kWarps = kNT == 1 ? 12 : 8;
+  static constexpr int kCtas = kNT == 1 ? 3 : 2;    // per SM
+  static constexpr int kWarps = 4;
   static constexpr int kChunk = 4;  // tiles of a pipeline stage
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
@@ -62,7 +64,7 @@ struct Few {
 
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -71,7 +73,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
 // the same with sums that start at zero
 __device__ __forceinline__ void mma16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                                uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
@@ -428,15 +430,23 @@ struct Part {
   int seq, g, v0, t_lo, t_hi, tiles;
   unsigned start;  // the piece's first unit
 };
+struct Share {
+  unsigned hi;          // the share's end
+  unsigned base, more;  // CTA c takes `base` units, one more for c < more
+};
 
 template <class E, int D, int kNT>
-__global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4_attn_few_kernel(AttnArgs a) {
   using F = Few<D, kNT>;
   constexpr int nb = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[F::kWarps][kStages];
   __shared__ int s_last;
   __shared__ float* s_sums[F::kWarps];
+  // What the tile loop has no use for, out of its registers: each warp's copy of
+  // its part, the next one, and the share
+  __shared__ Part s_now[F::kWarps], s_next[F::kWarps];
+  __shared__ Share s_share[F::kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int G = a.Hq / a.Hkv;
   uint8_t* ring = smem + warp * F::kWarpBytes;
@@ -461,10 +471,6 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   if (blockIdx.x >= ctas) return;
   const unsigned base = U / ctas, more = U - base * ctas;
   auto first_unit = [&](unsigned c) { return c * base + min(c, more); };
-  auto cta_of = [&](unsigned u) {
-    const unsigned x = more * (base + 1);
-    return u < x ? u / (base + 1) : more + (u - x) / base;
-  };
   // An end within kSnap tiles of an end of its piece moves there: what it would
   // split off costs less than the join.  A piece of up to 2 kSnap is never split.
   unsigned lo = first_unit(blockIdx.x), hi = first_unit(blockIdx.x + 1), seq_start = 0;
@@ -507,7 +513,13 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     hi = new_hi;
   }
   if (lo >= hi) return;
+  if (lane == 0) s_share[warp] = Share{hi, base, more};
   __syncthreads();  // the barriers are initialised
+  auto cta_of = [&](unsigned u) {
+    const Share h = s_share[warp];
+    const unsigned x = h.more * (h.base + 1);
+    return u < x ? u / (h.base + 1) : h.more + (u - x) / h.base;
+  };
 
   // the part that holds unit u, of a sequence at or after p.seq (which starts at unit seq_start)
   auto part_at = [&](Part& p, unsigned u) {
@@ -523,22 +535,19 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
     p.v0 = (piece - p.g * sets) * F::kVec;
     p.start = seq_start + unsigned(piece) * p.tiles;
     p.t_lo = int(u - p.start);
-    p.t_hi = int(min(hi - p.start, unsigned(p.tiles)));
+    p.t_hi = int(min(s_share[warp].hi - p.start, unsigned(p.tiles)));
   };
   // tiles go to the warps in runs of up to kChunk
   auto run_of = [&](const Part& p) { return min(F::kChunk, (p.t_hi - p.t_lo + F::kWarps - 1) / F::kWarps); };
   // the part's end in tiles that hold tokens
   auto end_of = [&](const Part& p) { return min(p.t_hi, (p.s.len + kv4::kTile - 1) / kv4::kTile); };
   const int tpp = a.page / kv4::kTile;
-  const uint64_t page_bytes = uint64_t(a.Hkv) * tpp * kv4::tile_bytes(D);
   // page id of this lane's tile t of a run, loaded well before its copy; -1: none
-  auto page_of = [&](const Part& p, int run, int t, int end) {
-    return lane < run && t < end
-               ? __ldg(a.table + p.seq * a.table_ld + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp))
-               : -1;
+  auto page_of = [&](const int* row, int run, int t, int end) {
+    return lane < run && t < end ? __ldg(row + (a.tpp_shift >= 0 ? t >> a.tpp_shift : t / tpp)) : -1;
   };
-  // bring a run's tiles (this lane's: t, on page id) into a stage; whole warp
-  auto fill = [&](const Part& p, int run, int t, int end, int id, uint32_t stage) {
+  // bring a run's tiles (this lane's: t, on page id) of head g into a stage; whole warp
+  auto fill = [&](int g, int run, int t, int end, int id, uint32_t stage) {
     uint64_t* bar = &s_bar[warp][stage];
     if (lane == 0)
       tc::mbar_expect_tx(bar, uint32_t(max(min(run, end - t), 0)) * kv4::tile_bytes(D));
@@ -548,12 +557,13 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
         kv4::report(a.err, kv4::kErrPage);
         id = 0;
       }
-      const int in = p.g * tpp + (a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp);
+      const int in = a.tpp_shift >= 0 ? t & (tpp - 1) : t % tpp;
+      const uint64_t tile = (uint64_t(unsigned(id)) * unsigned(a.Hkv) + unsigned(g)) * unsigned(tpp) + unsigned(in);
       tc::bulk_load(ring + stage * F::kStageBytes + lane * kv4::tile_bytes(D),
-                    a.pool + unsigned(id) * page_bytes + uint64_t(unsigned(in)) * kv4::tile_bytes(D),
-                    kv4::tile_bytes(D), bar);
+                    a.pool + tile * kv4::tile_bytes(D), kv4::tile_bytes(D), bar);
     }
   };
+  auto row_of = [&](const Part& p) { return a.table + p.seq * a.table_ld; };
   // the set's query rows as they are: lane (gid, tig) holds elements 8 tig .. of
   // each block of vector 8 j + gid
   auto load_q = [&](const Part& p, uint4 (&x)[kNT][nb]) {
@@ -580,31 +590,37 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
   uint4 qx[kNT][nb];
   {
     const int run = run_of(p), t = p.t_lo + warp * run + lane, end = end_of(p);
-    const int id = page_of(p, run, t, end);
+    const int id = page_of(row_of(p), run, t, end);
     // the rows before the tiles: they would wait behind them
     load_q(p, qx);
-    if (warp * run < p.t_hi - p.t_lo) fill(p, run, t, end, id, 0);
+    if (warp * run < p.t_hi - p.t_lo) fill(p.g, run, t, end, id, 0);
   }
   for (;;) {
     const int run = run_of(p), runs = (p.t_hi - p.t_lo + run - 1) / run, t_end = end_of(p);
-    int t = p.t_lo + (warp + F::kWarps) * run + lane;  // this lane's tile of the warp's next run
-    int id = page_of(p, run, t, t_end);
+    const int* row = row_of(p);
+    const int g = p.g, len = p.s.len;
+    int t0 = p.t_lo + warp * run;            // the warp's run,
+    int t = t0 + F::kWarps * run + lane;     // this lane's tile of its next one
+    int id = page_of(row, run, t, t_end);
     // the part after this one, and its first page
-    const unsigned u = p.start + p.t_hi;
-    Part np = p;
-    int nrun = 0, nid = -1, nt = 0;
-    if (u < hi) {
-      part_at(np, u);
-      nrun = run_of(np);
-      nt = np.t_lo + warp * nrun + lane;
-      nid = page_of(np, nrun, nt, end_of(np));
+    int nid = -1;
+    {
+      Part np = p;
+      if (p.start + p.t_hi < s_share[warp].hi) {
+        part_at(np, p.start + p.t_hi);
+        const int nrun = run_of(np);
+        nid = page_of(row_of(np), nrun, np.t_lo + warp * nrun + lane, end_of(np));
+      }
+      __syncwarp();  // the copies of the part before are read
+      if (lane == 0) {
+        s_now[warp] = p;
+        s_next[warp] = np;
+      }
     }
 
     // ---- query rows to B fragments, scaled to a maximum near 2^15
-    const Seq& s = p.s;
-    const int nv = s.rows * G;
     Query<D, kNT> q;
-    q.all = s.len - s.rows + p.v0 / G + 1;
+    q.all = len - p.s.rows + p.v0 / G + 1;
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
       float2 x[nb][4];
@@ -636,7 +652,7 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
         q.qs[j][i] = fmaxf(fabsf(a.scale) * 1.44269504088896341f *
                                __uint_as_float(uint32_t(127 - 14 + ee) << 23), 1e-37f);
         const int c = p.v0 + 8 * j + 2 * tig + i;
-        q.lim[j][i] = c < nv ? s.len - s.rows + c / G + 1 : 0;
+        q.lim[j][i] = c < p.s.rows * G ? len - p.s.rows + c / G + 1 : 0;
       }
     }
 
@@ -649,30 +665,37 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) w.o[j][k][0] = w.o[j][k][1] = w.o[j][k][2] = w.o[j][k][3] = 0.0f;
     }
-    for (int r = warp; r < runs; r += F::kWarps, ++it) {
-      if (r + F::kWarps < runs) {
+    for (int left = runs - warp; left > 0; left -= F::kWarps, ++it, t0 += F::kWarps * run) {
+      if (left > F::kWarps) {
         __syncwarp();  // the stage's last readers are done
-        fill(p, run, t, t_end, id, (it + 1) % kStages);
+        fill(g, run, t, t_end, id, (it + 1) % kStages);
         t += F::kWarps * run;
-        id = page_of(p, run, t, t_end);
+        id = page_of(row, run, t, t_end);
       }
       tc::mbar_wait(&s_bar[warp][it % kStages], (it / kStages) & 1u, a.err, 1);
-      const int t0 = p.t_lo + r * run;
       const int n = min(run, t_end - t0);
       const uint8_t* stage = ring + (it % kStages) * F::kStageBytes;
-      const int end = min(s.len, (t0 + n) * kv4::kTile);
+      const int end = min(len, (t0 + n) * kv4::kTile);
       if (n > 1)
         attend_tiles<D, kNT, F::kChunk>(w, q, stage, factors, t0 * kv4::kTile, end);
       else if (n == 1)
         attend_tiles<D, kNT, 1>(w, q, stage, factors, t0 * kv4::kTile, end);
     }
+    __syncwarp();
+    p = s_now[warp];
+    const Seq& s = p.s;
+    const int nv = s.rows * G;
+    const bool more_parts = p.start + p.t_hi < s_share[warp].hi;
     // the next part's first tiles and rows are on their way during the join; the
     // sums take the place of the stage read last
     float* sums = reinterpret_cast<float*>(ring + ((it + 1) % kStages) * F::kStageBytes);
-    if (u < hi) {
+    if (more_parts) {
+      const Part np = s_next[warp];
+      const int nrun = run_of(np);
       load_q(np, qx);
       __syncwarp();
-      if (warp * nrun < np.t_hi - np.t_lo) fill(np, nrun, nt, end_of(np), nid, it % kStages);
+      if (warp * nrun < np.t_hi - np.t_lo)
+        fill(np.g, nrun, np.t_lo + warp * nrun + lane, end_of(np), nid, it % kStages);
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
@@ -694,12 +717,10 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
       }
     if (lane == 0) s_sums[warp] = sums;
     __syncthreads();
-    const bool whole = p.t_lo == 0 && p.t_hi == p.tiles;
-    float* part = slot_of<D, kNT>(a.part, blockIdx.x, p.t_lo == 0 ? 1 : 0);
     constexpr int kPer = D / 4, kRows = 32 / kPer;
     const int sub = lane / kPer, d0 = (lane % kPer) * 4;
     // vectors warp * kRows + sub, .. of the sums that the first `busy` warps left
-    auto join_warps = [&](int busy, bool to_part) {
+    auto join_warps = [&](int busy, float* to) {
       for (int v = warp * kRows + sub; v < F::kVec; v += F::kWarps * kRows) {
         const float* src[F::kWarps];
         float2 ml[F::kWarps];
@@ -725,49 +746,67 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, 1) kv4_attn_few_kernel(
             o[3] = fmaf(c, x.w, o[3]);
           }
         }
-        if (to_part) {
-          *reinterpret_cast<float4*>(part + v * F::kAcc + d0) = make_float4(o[0], o[1], o[2], o[3]);
-          if (d0 == 0) *reinterpret_cast<float2*>(part + v * F::kAcc + D) = make_float2(m, l);
+        if (to) {
+          *reinterpret_cast<float4*>(to + v * F::kAcc + d0) = make_float4(o[0], o[1], o[2], o[3]);
+          if (d0 == 0) *reinterpret_cast<float2*>(to + v * F::kAcc + D) = make_float2(m, l);
         } else if (p.v0 + v < nv) {
           store_vector<E>(a, s, p.g, G, p.v0 + v, d0, o, l == 0.0f ? 0.0f : 1.0f / l, D);
         }
       }
     };
-    join_warps(min(F::kWarps, runs), !whole);
-    if (!whole) {
-      // the piece's last CTA to arrive joins the parts, in an order that does not depend on arrival
-      const unsigned c_first = cta_of(p.start + kSnap), c_last = cta_of(p.start + p.tiles - kSnap - 1);
+    // A piece that several CTAs share is joined in two levels, by the last of a
+    // group of its CTAs to arrive, then by the last of the groups; the order of
+    // the sums does not depend on who arrives when.  One level for up to kOneLevel.
+    int busy = min(F::kWarps, (p.t_hi - p.t_lo + run_of(p) - 1) / run_of(p));
+    int c_first = 0, parts = 1, group = 1, first = 0, count = 1, stride = 1;
+    if (p.t_lo != 0 || p.t_hi != p.tiles) {
+      c_first = int(cta_of(p.start + kSnap));
+      parts = int(cta_of(p.start + p.tiles - kSnap - 1)) - c_first + 1;
+      group = parts <= kOneLevel ? parts : int(ceilf(sqrtf(float(parts))));
+      first = (int(blockIdx.x) - c_first) / group * group;
+      count = min(group, parts - first);
+    }
+    // the sums of the CTA that is the i-th of the piece, and of the group that begins there
+    auto slot_at = [&](int i) { return slot_of<D, kNT>(a.part, c_first + i, i == 0); };
+    float* to = parts == 1 ? nullptr : slot_of<D, kNT>(a.part, blockIdx.x, p.t_lo == 0);
+    unsigned* counter = a.counters + 2 * (c_first + first) + (first == 0);
+    for (int joined = 1;;) {  // CTAs of the piece whose sums this one has
+      join_warps(busy, to);
+      if (!to) break;
       __syncthreads();
       if (threadIdx.x == 0) {
-        // release of the CTA's part (ordered before by the barrier), acquire of the others'
+        // release of the CTA's sums (ordered before by the barrier), acquire of the others'
         __threadfence();
-        s_last = atomicInc(a.counters + c_first, c_last - c_first) == c_last - c_first;
+        s_last = atomicInc(counter, unsigned(count - 1)) == unsigned(count - 1);
         __threadfence();
       }
       __syncthreads();
-      if (s_last) {
-        const int parts = int(c_last - c_first) + 1;
-        constexpr int kN = F::kVec / kRows;
-        float m[kN], l[kN];
-        float4 o[kN];
-        join_rows<D, kNT>(warp, F::kWarps, parts,
-                          [&](int i) { return slot_of<D, kNT>(a.part, c_first + i, i == 0); }, m, l, o);
+      if (!s_last) break;
+      constexpr int kN = F::kVec / kRows;
+      float m[kN], l[kN];
+      float4 o[kN];
+      join_rows<D, kNT>(warp, F::kWarps, count, [&](int i) { return slot_at(first + i * stride); }, m, l, o);
 #pragma unroll
-        for (int k = 0; k < kN; ++k) {
-          float* dst = sums + (k * kRows + sub) * F::kAcc;
-          *reinterpret_cast<float4*>(dst + d0) = o[k];
-          if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[k], l[k]);
-        }
-        __syncthreads();
-        join_warps(min(F::kWarps, parts), false);
+      for (int k = 0; k < kN; ++k) {
+        float* dst = sums + (k * kRows + sub) * F::kAcc;
+        *reinterpret_cast<float4*>(dst + d0) = o[k];
+        if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(m[k], l[k]);
       }
+      __syncthreads();
+      busy = min(F::kWarps, count);
+      joined *= group;
+      to = joined >= parts ? nullptr : slot_at(first);
+      first = 0;
+      stride = group;
+      count = (parts + group - 1) / group;
+      counter = a.counters + 2 * kFewCtas + c_first;
     }
-    if (u >= hi) break;
+    if (!more_parts) break;
     // the sums are read: their memory, written by ordinary stores, takes tiles
     // from bulk copies again
     tc::fence_proxy_async_smem();
     __syncthreads();
-    p = np;
+    p = s_next[warp];
   }
   if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], kStages, it);
 }
@@ -778,7 +817,7 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
   const void* fn = reinterpret_cast<const void*>(kv4_attn_few_kernel<E, D, kNT>);
   const cudaError_t e = ensure_dynamic_smem(fn, F::kSmem);
   if (e != cudaSuccess) return e;
-  kv4_attn_few_kernel<E, D, kNT><<<kCtas, F::kThreads, F::kSmem, s>>>(a);
+  kv4_attn_few_kernel<E, D, kNT><<<kSms * F::kCtas, F::kThreads, F::kSmem, s>>>(a);
   return cudaGetLastError();
 }
 

@@ -48,16 +48,19 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 }
 
 
-constexpr int kCtas = 148;                 // one per SM
-// Words of the workspace's head, zero between calls: one per CTA (few rows); for
-// many rows the next item, the CTAs that are done, and one per part and warp.
-constexpr int kItemCounter = kCtas, kDoneCounter = kCtas + 1, kPartCounters = kCtas + 2;
-constexpr size_t kCounterBytes = 8192;
+constexpr int kSms = 148;
+constexpr int kCtas = kSms;                // of the kernel for many rows
+constexpr int kFewCtas = 4 * kSms;         // most of the kernel for few rows
+// Words of the workspace's head, zero between calls.  Few rows: two per CTA for
+// the groups that begin with it, one for the pieces.  Many rows: the next item,
+// the CTAs that are done, one per part and warp.
+constexpr int kItemCounter = 3 * kFewCtas, kDoneCounter = kItemCounter + 1, kPartCounters = kItemCounter + 2;
+constexpr size_t kCounterBytes = 16384;
 static_assert(kCounterBytes >= (kPartCounters + 8 * kCtas) * sizeof(unsigned), "room for the counters");
 constexpr int kFew = 64;                   // vectors of a sequence and KV head that are few rows
 
 // Bytes of the sums that parts of a piece or item leave for each other.
-constexpr size_t few_bytes(int D) { return size_t(kCtas) * 2 * 16 * (D + 4) * sizeof(float); }
+constexpr size_t few_bytes(int D) { return size_t(kFewCtas) * 2 * 16 * (D + 4) * sizeof(float); }
 constexpr size_t many_bytes(int D) { return size_t(kCtas) * 256 * (D + 2) * sizeof(float); }
 
 __device__ __forceinline__ float ex2(float x) {
