@@ -43,14 +43,13 @@ using namespace kv4;
 //   top + 4), top the largest value code that the warp has seen: exact but for
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
-constexpr int kStages = 2;   // one read, one on its way
+constexpr int kStages = 2;   // one read, the others on their way
 constexpr unsigned kSnap = 32;  // tiles
 constexpr int kOneLevel = 8;    // parts
 
-template <int D, int kNT>
+template <int D, int kNT, int kPerSm>
 struct Few {
-  static constexpr int kCtas = kNT == 1 ? 3 : 2;    // per SM
-  static constexpr int kWarps = 4;
+  static constexpr int kWarps = kNT == 1 ? 12 / kPerSm : 8 / kPerSm;
   static constexpr int kChunk = 4;  // tiles of a pipeline stage
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
@@ -118,7 +117,7 @@ struct Query {
 // kN tiles at `base` (shared memory), the first holding token `pos0`, of which
 // tokens from `end` on count for nothing (their bytes may be anything);
 // `factors`: this warp's place for their factors.
-template <int D, int kNT, int kN>
+template <int D, int kNT, int kPerSm, int kN>
 __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, kNT>& q,
                                              const uint8_t* base, uint8_t* factors, int pos0,
                                              int end) {
@@ -129,7 +128,7 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
   // read neighbouring value rows
   const int tok = (gid & 1) * 4 + (gid >> 1);
   float* kf = reinterpret_cast<float*>(factors);                          // [tile][token][block]
-  uint32_t* vf = reinterpret_cast<uint32_t*>(factors + Few<D, kNT>::kChunk * kv4::kTile * nb * 4);  // [tile][pair][block]
+  uint32_t* vf = reinterpret_cast<uint32_t*>(factors + Few<D, kNT, kPerSm>::kChunk * kv4::kTile * nb * 4);  // [tile][pair][block]
 
   // ---- codes to factors.  Keys: one word a lane and turn.  Values: lane (tile,
   // pair) takes tokens t and t + 4, t = 0-3, 8-11
@@ -366,9 +365,9 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
 
 // Partial sums of a piece that several CTAs share: slot 0 of a CTA holds the
 // piece that began before its share, slot 1 the one that goes on after it.
-template <int D, int kNT>
+template <int D, int kNT, int kPerSm>
 __device__ __forceinline__ float* slot_of(float* part, int cta, int slot) {
-  return part + (size_t(cta) * 2 + slot) * (Few<D, kNT>::kVec * Few<D, kNT>::kAcc);
+  return part + (size_t(cta) * 2 + slot) * (Few<D, kNT, kPerSm>::kVec * Few<D, kNT, kPerSm>::kAcc);
 }
 
 template <class E>
@@ -384,12 +383,12 @@ __device__ __forceinline__ void store_vector(const AttnArgs& a, const Seq& s, in
 
 // Join what `count` warps or CTAs left of a set, each a row of kVec sums, read by
 // `at`(i): this warp takes rows first, first + step, .. of all vectors at once.
-template <int D, int kNT, class At>
+template <int D, int kNT, int kPerSm, class At>
 __device__ __forceinline__ void join_rows(int first, int step, int count, At at,
-                                          float (&m)[Few<D, kNT>::kVec * D / 128],
-                                          float (&l)[Few<D, kNT>::kVec * D / 128],
-                                          float4 (&o)[Few<D, kNT>::kVec * D / 128]) {
-  using F = Few<D, kNT>;
+                                          float (&m)[Few<D, kNT, kPerSm>::kVec * D / 128],
+                                          float (&l)[Few<D, kNT, kPerSm>::kVec * D / 128],
+                                          float4 (&o)[Few<D, kNT, kPerSm>::kVec * D / 128]) {
+  using F = Few<D, kNT, kPerSm>;
   constexpr int kPer = D / 4, kRows = 32 / kPer, kN = F::kVec / kRows;  // lanes of a vector, ..
   const int lane = threadIdx.x & 31, sub = lane / kPer, d0 = (lane % kPer) * 4;
 #pragma unroll
@@ -435,9 +434,9 @@ struct Share {
   unsigned base, more;  // CTA c takes `base` units, one more for c < more
 };
 
-template <class E, int D, int kNT>
-__global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4_attn_few_kernel(AttnArgs a) {
-  using F = Few<D, kNT>;
+template <class E, int D, int kNT, int kPerSm>
+__global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_attn_few_kernel(AttnArgs a) {
+  using F = Few<D, kNT, kPerSm>;
   constexpr int nb = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ uint64_t s_bar[F::kWarps][kStages];
@@ -677,9 +676,9 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4
       const uint8_t* stage = ring + (it % kStages) * F::kStageBytes;
       const int end = min(len, (t0 + n) * kv4::kTile);
       if (n > 1)
-        attend_tiles<D, kNT, F::kChunk>(w, q, stage, factors, t0 * kv4::kTile, end);
+        attend_tiles<D, kNT, kPerSm, F::kChunk>(w, q, stage, factors, t0 * kv4::kTile, end);
       else if (n == 1)
-        attend_tiles<D, kNT, 1>(w, q, stage, factors, t0 * kv4::kTile, end);
+        attend_tiles<D, kNT, kPerSm, 1>(w, q, stage, factors, t0 * kv4::kTile, end);
     }
     __syncwarp();
     p = s_now[warp];
@@ -767,8 +766,8 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4
       count = min(group, parts - first);
     }
     // the sums of the CTA that is the i-th of the piece, and of the group that begins there
-    auto slot_at = [&](int i) { return slot_of<D, kNT>(a.part, c_first + i, i == 0); };
-    float* to = parts == 1 ? nullptr : slot_of<D, kNT>(a.part, blockIdx.x, p.t_lo == 0);
+    auto slot_at = [&](int i) { return slot_of<D, kNT, kPerSm>(a.part, c_first + i, i == 0); };
+    float* to = parts == 1 ? nullptr : slot_of<D, kNT, kPerSm>(a.part, blockIdx.x, p.t_lo == 0);
     unsigned* counter = a.counters + 2 * (c_first + first) + (first == 0);
     for (int joined = 1;;) {  // CTAs of the piece whose sums this one has
       join_warps(busy, to);
@@ -776,16 +775,17 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4
       __syncthreads();
       if (threadIdx.x == 0) {
         // release of the CTA's sums (ordered before by the barrier), acquire of the others'
-        __threadfence();
-        s_last = atomicInc(counter, unsigned(count - 1)) == unsigned(count - 1);
-        __threadfence();
+        unsigned old;
+        asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;"
+                     : "=r"(old) : "l"(counter), "r"(unsigned(count - 1)) : "memory");
+        s_last = old == unsigned(count - 1);
       }
       __syncthreads();
       if (!s_last) break;
       constexpr int kN = F::kVec / kRows;
       float m[kN], l[kN];
       float4 o[kN];
-      join_rows<D, kNT>(warp, F::kWarps, count, [&](int i) { return slot_at(first + i * stride); }, m, l, o);
+      join_rows<D, kNT, kPerSm>(warp, F::kWarps, count, [&](int i) { return slot_at(first + i * stride); }, m, l, o);
 #pragma unroll
       for (int k = 0; k < kN; ++k) {
         float* dst = sums + (k * kRows + sub) * F::kAcc;
@@ -811,24 +811,32 @@ __global__ void __launch_bounds__(Few<D, kNT>::kThreads, Few<D, kNT>::kCtas) kv4
   if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], kStages, it);
 }
 
-template <class E, int D, int kNT>
+template <class E, int D, int kNT, int kPerSm>
 cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
-  using F = Few<D, kNT>;
-  const void* fn = reinterpret_cast<const void*>(kv4_attn_few_kernel<E, D, kNT>);
+  using F = Few<D, kNT, kPerSm>;
+  const void* fn = reinterpret_cast<const void*>(kv4_attn_few_kernel<E, D, kNT, kPerSm>);
   const cudaError_t e = ensure_dynamic_smem(fn, F::kSmem);
   if (e != cudaSuccess) return e;
-  kv4_attn_few_kernel<E, D, kNT><<<kSms * F::kCtas, F::kThreads, F::kSmem, s>>>(a);
+  kv4_attn_few_kernel<E, D, kNT, kPerSm><<<kSms * kPerSm, F::kThreads, F::kSmem, s>>>(a);
   return cudaGetLastError();
 }
 
 // 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
-// are then read and decoded half as often), else 8.  Sequences of more than
-// kFew vectors go to the kernel for many rows, whose tile is 256 vectors.
+// are then read and decoded half as often), else 8.  One large CTA an SM where few
+// pieces share the SMs (fewer sums to join: one sequence of 131072 tokens 28
+// against 31 us with three), three (two with 16 vectors) small ones where pieces
+// are many and short (one's start and join hide behind the others: 64 sequences
+// of up to 4096 tokens 35 against 49 us).
+// Sequences of more than kFew vectors go to the kernel for many rows, whose tile
+// is 256 vectors.
 template <class E, int D>
 cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
+  const bool many_pieces = (long long)a.n_seq * a.Hkv >= 32;
   a.few = kFew;
-  cudaError_t e = vectors <= 8 ? launch_few<E, D, 1>(a, s) : launch_few<E, D, 2>(a, s);
+  cudaError_t e;
+  if (vectors <= 8) e = many_pieces ? launch_few<E, D, 1, 3>(a, s) : launch_few<E, D, 1, 1>(a, s);
+  else e = many_pieces ? launch_few<E, D, 2, 2>(a, s) : launch_few<E, D, 2, 1>(a, s);
   if (e == cudaSuccess && vectors > kFew)
     e = launch_kv4_prefill(a, std::is_same<E, __nv_bfloat16>::value, D, s);
   return e;

@@ -50,7 +50,7 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 
 constexpr int kSms = 148;
 constexpr int kCtas = kSms;                // of the kernel for many rows
-constexpr int kFewCtas = 4 * kSms;         // most of the kernel for few rows
+constexpr int kFewCtas = 3 * kSms;         // most of the kernel for few rows
 // Words of the workspace's head, zero between calls.  Few rows: two per CTA for
 // the groups that begin with it, one for the pieces.  Many rows: the next item,
 // the CTAs that are done, one per part and warp.

@@ -212,7 +212,7 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
         max_q = T if max_q is None else min(int(max_q), T)
         _check(max_q >= 0, "max_q must not be negative")
     if out is None:
-        out = q.new_empty(shape)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         _check(out.shape == shape and out.dtype == q.dtype and out.device == dev
                and out.is_contiguous(), "out must be a contiguous tensor of q's shape, type and device")
