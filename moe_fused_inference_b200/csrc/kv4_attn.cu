@@ -43,14 +43,14 @@ using namespace kv4;
 //   top + 4), top the largest value code that the warp has seen: exact but for
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
-constexpr int kStages = 2;   // one read, the others on their way
 constexpr unsigned kSnap = 32;  // tiles
 constexpr int kOneLevel = 8;    // parts
 
 template <int D, int kNT, int kPerSm>
 struct Few {
   static constexpr int kWarps = kNT == 1 ? 12 / kPerSm : 8 / kPerSm;
-  static constexpr int kChunk = 4;  // tiles of a pipeline stage
+  static constexpr int kChunk = 4;   // tiles of a pipeline stage
+  static constexpr int kStages = 2;  // one read, the others on their way
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
   static constexpr int kStageBytes = kChunk * kv4::tile_bytes(D);
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   using F = Few<D, kNT, kPerSm>;
   constexpr int nb = D / 32;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ uint64_t s_bar[F::kWarps][kStages];
+  __shared__ uint64_t s_bar[F::kWarps][F::kStages];
   __shared__ int s_last;
   __shared__ float* s_sums[F::kWarps];
   // What the tile loop has no use for, out of its registers: each warp's copy of
@@ -449,10 +449,10 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
   const int G = a.Hq / a.Hkv;
   uint8_t* ring = smem + warp * F::kWarpBytes;
-  uint8_t* factors = ring + kStages * F::kStageBytes;
+  uint8_t* factors = ring + F::kStages * F::kStageBytes;
   if (threadIdx.x == 0) tc::cta_abort_init();
   if (lane == 0)
-    for (int i = 0; i < kStages; ++i) tc::mbar_init(&s_bar[warp][i], 1);
+    for (int i = 0; i < F::kStages; ++i) tc::mbar_init(&s_bar[warp][i], 1);
   tc::fence_mbar_init();
 
   // ---- this CTA's share of the work: every warp sums the sequences' units, 32
@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     const int* row = row_of(p);
     const int g = p.g, len = p.s.len;
     int t0 = p.t_lo + warp * run;            // the warp's run,
-    int t = t0 + F::kWarps * run + lane;     // this lane's tile of its next one
+    int t = t0 + F::kWarps * run + lane;     // this lane's tile of the next one to bring in
     int id = page_of(row, run, t, t_end);
     // the part after this one, and its first page
     int nid = -1;
@@ -664,16 +664,22 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) w.o[j][k][0] = w.o[j][k][1] = w.o[j][k][2] = w.o[j][k][3] = 0.0f;
     }
+    // the first run is on its way; more of them, up to F::kStages - 1
+    for (int k = 1; k < F::kStages - 1 && warp + k * F::kWarps < runs; ++k) {
+      fill(g, run, t, t_end, id, (it + k) % F::kStages);
+      t += F::kWarps * run;
+      id = page_of(row, run, t, t_end);
+    }
     for (int left = runs - warp; left > 0; left -= F::kWarps, ++it, t0 += F::kWarps * run) {
-      if (left > F::kWarps) {
+      if (left > (F::kStages - 1) * F::kWarps) {
         __syncwarp();  // the stage's last readers are done
-        fill(g, run, t, t_end, id, (it + 1) % kStages);
+        fill(g, run, t, t_end, id, (it + F::kStages - 1) % F::kStages);
         t += F::kWarps * run;
         id = page_of(row, run, t, t_end);
       }
-      tc::mbar_wait(&s_bar[warp][it % kStages], (it / kStages) & 1u, a.err, 1);
+      tc::mbar_wait(&s_bar[warp][it % F::kStages], (it / F::kStages) & 1u, a.err, 1);
       const int n = min(run, t_end - t0);
-      const uint8_t* stage = ring + (it % kStages) * F::kStageBytes;
+      const uint8_t* stage = ring + (it % F::kStages) * F::kStageBytes;
       const int end = min(len, (t0 + n) * kv4::kTile);
       if (n > 1)
         attend_tiles<D, kNT, kPerSm, F::kChunk>(w, q, stage, factors, t0 * kv4::kTile, end);
@@ -687,14 +693,14 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     const bool more_parts = p.start + p.t_hi < s_share[warp].hi;
     // the next part's first tiles and rows are on their way during the join; the
     // sums take the place of the stage read last
-    float* sums = reinterpret_cast<float*>(ring + ((it + 1) % kStages) * F::kStageBytes);
+    float* sums = reinterpret_cast<float*>(ring + ((it + F::kStages - 1) % F::kStages) * F::kStageBytes);
     if (more_parts) {
       const Part np = s_next[warp];
       const int nrun = run_of(np);
       load_q(np, qx);
       __syncwarp();
       if (warp * nrun < np.t_hi - np.t_lo)
-        fill(np.g, nrun, np.t_lo + warp * nrun + lane, end_of(np), nid, it % kStages);
+        fill(np.g, nrun, np.t_lo + warp * nrun + lane, end_of(np), nid, it % F::kStages);
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
@@ -808,7 +814,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     __syncthreads();
     p = s_next[warp];
   }
-  if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], kStages, it);
+  if (tc::cta_aborted()) tc::drain_ring(s_bar[warp], F::kStages, it);
 }
 
 template <class E, int D, int kNT, int kPerSm>
