@@ -34,15 +34,11 @@ struct ReadArgs {
   Slots s;
 };
 
-// Slot of token t, -1 for none.
-__device__ __forceinline__ int slot_of(const Slots& s, int t) {
-  const long long x = s.slots[t];
-  if (x < 0) return -1;
-  if (x >= s.capacity) {
-    kv4::report(s.err, kv4::kErrSlot);
-    return -1;
-  }
-  return int(x);
+// A slot as a token of the pool, 0 for one that is none (`live` says which).  No
+// branch hangs on the slot before a thread's other loads are on their way.
+__device__ __forceinline__ int token_of(const Slots& s, long long slot, bool& live) {
+  live = slot >= 0 && slot < s.capacity;
+  return live ? int(slot) : 0;
 }
 
 // Byte offset in the pool of the tile of (slot, head h of Hkv); row: its row there.
@@ -112,10 +108,11 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint8_t& code
 // A block takes kRwThreads / (D/8) tokens of one KV head, its neighbours the other
 // heads of the same tokens, so that the rows (T, Hkv, D) are met in order: D/8
 // lanes a token, a quad a block of 32 elements, each lane 8 elements of the key
-// and of the value.  The tokens of a tile are neighbours in memory: a warp
-// writes whole 32-byte sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53
-// written an element.  More tokens a thread cost more than they hide (2 of them:
-// 16384 tokens 30 -> 33 us with their read-back, 1021 fp32 tokens 4.9 -> 8.5 us).
+// and of the value.  The tokens of a tile are neighbours in memory: a warp writes
+// whole 32-byte sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53 written an
+// element.  16384 tokens of 4 heads of 128 written and read back take 28 us, 3.0
+// TB/s; more tokens a thread do not help (2: 27.7 us, 4: 31.6 us) and cost small
+// calls (1021 tokens of 2 heads of 64, fp32: 4.0 us, with 2 tokens a thread 4.8).
 constexpr int kRwThreads = 128;
 
 template <class E, int D, bool kVec>
@@ -123,22 +120,25 @@ __global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;
   const int Hkv = a.s.Hkv, run = blockIdx.x / Hkv, h = blockIdx.x - run * Hkv;
   const int t = run * (kRwThreads / kLanes) + threadIdx.x / kLanes, w = threadIdx.x % kLanes;
-  float k[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int slot = -1;
-  if (t < a.s.T) {
-    slot = slot_of(a.s, t);
-    load8<E, kVec>(static_cast<const E*>(a.x[0]) + t * a.row[0] + h * a.head[0] + 8 * w, k);
-    load8<E, kVec>(static_cast<const E*>(a.x[1]) + t * a.row[1] + h * a.head[1] + 8 * w, v);
-  }
+  const int b = w >> 2, q = w & 3, tt = min(t, a.s.T - 1);
+  float k[8], v[8];
+  const long long slot = __ldg(a.s.slots + tt);
+  load8<E, kVec>(static_cast<const E*>(a.x[0]) + tt * a.row[0] + h * a.head[0] + 8 * w, k);
+  load8<E, kVec>(static_cast<const E*>(a.x[1]) + tt * a.row[1] + h * a.head[1] + 8 * w, v);
   uint8_t kc, vc;
   const uint32_t kw = quantise8(k, kc), vw = quantise8(v, vc);
   // value pieces 2q, 2q+1 of blocks b and b ^ 1 make two words of the row: the
   // lane of the even block writes the one of pieces 2q, the odd block's 2q+1
   const uint32_t other = __shfl_xor_sync(0xffffffffu, vw, 4);
-  if (slot < 0) return;
+  bool live;
+  const int token = token_of(a.s, slot, live);
+  if (t >= a.s.T) return;
+  if (!live) {
+    if (slot >= 0) kv4::report(a.s.err, kv4::kErrSlot);
+    return;
+  }
   int r;
-  uint8_t* tile = a.pool + tile_of<D>(a.s, slot, h, Hkv, r);
-  const int b = w >> 2, q = w & 3;
+  uint8_t* tile = a.pool + tile_of<D>(a.s, token, h, Hkv, r);
   *reinterpret_cast<uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4) = kw;
   const uint32_t word = (b & 1) ? __byte_perm(other, vw, 0x7632) : __byte_perm(vw, other, 0x5410);
   const int piece = 2 * q + (b & 1);
@@ -153,11 +153,7 @@ __global__ void __launch_bounds__(kRwThreads) kv4_write_kernel(WriteArgs a) {
 template <class E>
 __device__ __forceinline__ void store8(E* p, uint32_t w, float s) {
   uint32_t h[4];
-  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
-      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
-      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
-      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
-      : "r"(w));
+  kv4::e2m1x8(w, h);
   __align__(16) E out[8];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -171,25 +167,30 @@ __device__ __forceinline__ void store8(E* p, uint32_t w, float s) {
 }
 
 // The write's shape, the other way round: 0.53 bytes read and 2 written (bf16) an
-// element.  131072 tokens of 4 heads of 128: 71 us, 4.8 TB/s.
+// element.  The slots, then the rows that they name, are two dependent trips to
+// memory.  131072 tokens of 4 heads of 128: 69 us, 4.9 TB/s, four bytes written for
+// one read.
 template <class E, int D>
 __global__ void __launch_bounds__(kRwThreads) kv4_read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;
   const int Hkv = a.s.Hkv, run = blockIdx.x / Hkv, h = blockIdx.x - run * Hkv;
   const int t = run * (kRwThreads / kLanes) + threadIdx.x / kLanes, w = threadIdx.x % kLanes;
+  const int b = w >> 2, q = w & 3;
   if (t >= a.s.T) return;
-  const int slot = slot_of(a.s, t);
-  uint32_t kw = 0u, vw = 0u, kc = 127u, vc = 127u;
-  if (slot >= 0) {
-    int r;
-    const uint8_t* tile = a.pool + tile_of<D>(a.s, slot, h, Hkv, r);
-    const int b = w >> 2, q = w & 3;
-    const uint8_t* vr = tile + 8 * D + r * (D / 2);
-    kw = __ldg(reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4));
-    vw = uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + (2 * q * nb + b) * 2))) |
-         uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + ((2 * q + 1) * nb + b) * 2))) << 16;
-    kc = __ldg(tile + 16 * D + r * nb + b);
-    vc = __ldg(tile + 16 * D + D / 2 + r * nb + b);
+  const long long slot = __ldg(a.s.slots + t);
+  bool live;
+  int r;
+  const int token = token_of(a.s, slot, live);
+  const uint8_t* tile = a.pool + tile_of<D>(a.s, token, h, Hkv, r);
+  const uint8_t* vr = tile + 8 * D + r * (D / 2);
+  uint32_t kw = __ldg(reinterpret_cast<const uint32_t*>(tile + r * (D / 2) + (q * nb + b) * 4));
+  uint32_t vw = uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + (2 * q * nb + b) * 2))) |
+                uint32_t(__ldg(reinterpret_cast<const uint16_t*>(vr + ((2 * q + 1) * nb + b) * 2))) << 16;
+  uint32_t kc = __ldg(tile + 16 * D + r * nb + b), vc = __ldg(tile + 16 * D + D / 2 + r * nb + b);
+  if (!live) {
+    kw = vw = 0u;
+    kc = vc = 127u;
+    if (slot >= 0) kv4::report(a.s.err, kv4::kErrSlot);
   }
   const long long at = ((long long)t * Hkv + h) * D + 8 * w;
   store8(static_cast<E*>(a.y[0]) + at, kw, kv4::code_value(kc));
@@ -210,7 +211,7 @@ int check_pool(const void* pool, int Hkv, int D, int page, int num_pages) {
   return MFI_OK;
 }
 
-int launched(const char*) {
+int launched() {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MFI_OK : set_last_error(MFI_ERR_CUDA, cudaGetErrorString(e));
 }
@@ -296,7 +297,7 @@ extern "C" int mfi_kv4_write(const void* k, long long k_row, long long k_head, c
   if (dtype == MFI_F32) mfi::launch_write<float>(a, D, vec, grid, s);
   else if (dtype == MFI_F16) mfi::launch_write<__half>(a, D, vec, grid, s);
   else mfi::launch_write<__nv_bfloat16>(a, D, vec, grid, s);
-  return mfi::launched("kv4_write");
+  return mfi::launched();
 }
 
 extern "C" int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, int dtype,
@@ -320,5 +321,5 @@ extern "C" int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, 
   if (dtype == MFI_F32) mfi::launch_read<float>(a, D, grid, s);
   else if (dtype == MFI_F16) mfi::launch_read<__half>(a, D, grid, s);
   else mfi::launch_read<__nv_bfloat16>(a, D, grid, s);
-  return mfi::launched("kv4_read");
+  return mfi::launched();
 }

@@ -39,12 +39,13 @@ __device__ __forceinline__ float code_value(uint32_t c) {
   return __uint_as_float(c == 255u ? 0x7FC00000u : (c == 0u ? 0x00400000u : c << 23));
 }
 
-// E2M1 nibble (low 4 bits of n) to its value.
-__device__ __forceinline__ float nibble_value(uint32_t n) {
-  // bits e1 e0 m at an fp32's lowest exponent bits and top mantissa bit read
-  // 2^(e-127) (1 + m/2), or m/2 2^-126 at e = 0: 2^126 times too small
-  const float f = __uint_as_float((n & 7u) << 22) * 0x1p126f;
-  return (n & 8u) ? -f : f;
+// The four bytes of w, each two E2M1 values, to fp16x2 (low nibble: low half).
+__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {
+  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
+      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
+      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
+      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
+      : "r"(w));
 }
 
 // Device error codes of the cache's kernels.

@@ -68,14 +68,6 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
-// The four bytes of w, each two E2M1 values, to fp16x2 (low nibble: low half).
-__device__ __forceinline__ void e2m1x8(uint32_t w, uint32_t (&o)[4]) {
-  asm("{\n .reg .b8 a, b, c, d;\n mov.b32 {a, b, c, d}, %4;\n"
-      " cvt.rn.f16x2.e2m1x2 %0, a;\n cvt.rn.f16x2.e2m1x2 %1, b;\n"
-      " cvt.rn.f16x2.e2m1x2 %2, c;\n cvt.rn.f16x2.e2m1x2 %3, d;\n}"
-      : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3])
-      : "r"(w));
-}
 // E8M0 codes (nb bytes) to fp32; 255 gives NaN.
 template <int nb>
 __device__ __forceinline__ void codes(uint32_t w, float (&f)[nb]) {
