@@ -7,6 +7,7 @@
 // and zeros for a row that sees no token.
 #include <cuda_fp16.h>
 
+#include <cmath>
 #include <type_traits>
 
 #include "../../include/moe_fp4.h"
@@ -23,12 +24,20 @@ namespace {
 
 using namespace kv4;
 
-// ---- few rows: vectors of a group on the legacy tensor path --------------------
+// ---- few rows: up to 64 vectors a sequence and KV head, on mma.sync -------------
 // A vector is one row of one query head; the R G vectors of a sequence and KV
 // head (v = r G + h) are taken 8 kNT at a time (a "set").  The work is the list
 // of all (sequence, KV head, set, tile of 16 tokens), in that order; CTA c takes
 // the c-th of `ctas` equal shares, whatever the sequences' lengths, and splits
-// each piece (sequence, head, set) of its share over its warps.
+// each piece (sequence, head, set) of its share over its warps.  8 or 16 vectors
+// fill the n = 8 of mma.m16n8k16; an MMA of 64 or more would multiply zeros.
+//
+// What bounds it: the tile loop runs at 5.7 TB/s of the cache's bytes (232 warp
+// instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
+// has some 14 us beside it: the launch, three dependent trips (lengths, page table,
+// tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
+// heads: 1 sequence of 131072 tokens 27.7 us, 64 of up to 4096 34.5 us, 1 of 1152
+// 11.3 us.
 //
 // Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
@@ -43,14 +52,16 @@ using namespace kv4;
 //   top + 4), top the largest value code that the warp has seen: exact but for
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
-constexpr unsigned kSnap = 32;  // tiles
+constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
 constexpr int kOneLevel = 8;    // parts
 
 template <int D, int kNT, int kPerSm>
 struct Few {
   static constexpr int kWarps = kNT == 1 ? 12 / kPerSm : 8 / kPerSm;
   static constexpr int kChunk = 4;   // tiles of a pipeline stage
-  static constexpr int kStages = 2;  // one read, the others on their way
+  // one read, the others on their way; stages of 2 tiles 3 or 4 deep: 30.3, 31.0
+  // instead of 27.7 us for 131072 tokens
+  static constexpr int kStages = 2;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
   static constexpr int kStageBytes = kChunk * kv4::tile_bytes(D);
@@ -890,9 +901,12 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: the workspace must be 256-byte aligned");
   if (workspace_bytes < mfi_kv4_attn_workspace_bytes(n_seq, Hq, Hkv, D, max_q))
     return mfi::set_last_error(MFI_ERR_WORKSPACE, "workspace smaller than the kv4_attn workspace query");
-  // units of work (a tile of a KV head for 8 vectors, at most) are counted in 31 bits
+  // units of work of the kernel for few rows (a tile of a KV head for 8 vectors, at
+  // most) are counted in 31 bits; the items of the other one are fewer than the rows
+  // of `out`
+  const double vectors = fmin(double(max_q) * (Hq / Hkv), double(mfi::kv4::kFew));
   const double units = double(n_seq) * Hkv * (double(width) * page / mfi::kv4::kTile + 1) *
-                       (double(max_q) * (Hq / Hkv) / 8 + 1);
+                       (vectors / 8 + 1);
   if (units >= 2147483648.0)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: more than 2^31 tiles of work in one call");
   mfi::kv4::AttnArgs a{};

@@ -355,6 +355,20 @@ def test_attention_in_a_graph_with_moving_lengths():
     assert _errors() == 0
 
 
+def test_attention_of_many_rows_under_a_wide_table():
+    """Rows of a prompt times the tiles that its page table has room for pass 2^31
+    (8 heads x 38400 x 8192 sets of 8): no limit of the kernel for many rows."""
+    q, cache, table = _make(9, [20], [20], 8, 8, 64, 1024, torch.bfloat16)
+    rows = 8192
+    wide = np.full((1, 600), table[0, 0], np.int32)
+    many = torch.zeros((rows, 64, 64), dtype=q.dtype, device="cuda")
+    many[-20:] = q
+    got = _call(many, cache, wide, [20], [rows])
+    assert _errors() == 0
+    assert not got[:-20].any()  # rows that see no token
+    _compare(got[-20:], q, cache, table, [20], [20])
+
+
 def test_attention_on_another_stream():
     rows, lens = [1, 1], [900, 33]
     q, cache, table = _make(4, rows, lens, 2, 8, 128, 64, torch.bfloat16)
