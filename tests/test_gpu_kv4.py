@@ -369,6 +369,19 @@ def test_attention_of_many_rows_under_a_wide_table():
     _compare(got[-20:], q, cache, table, [20], [20])
 
 
+def test_one_workspace_serves_calls_of_all_shapes_in_turn():
+    """Every call leaves the workspace as it found it, and repeats bit for bit."""
+    cases = [([1], [20011], 1, 8), ([100], [3050], 1, 8), ([1] * 40, [1 + 61 * i for i in range(40)], 1, 8),
+             ([257], [700], 1, 8), ([5], [4099], 1, 8), ([0, 0], [9, 9], 1, 8)]
+    made = [_make(20 + i, rows, lens, H, G, 128, 64, torch.bfloat16) + (lens, rows)
+            for i, (rows, lens, H, G) in enumerate(cases)]
+    want = [_call(*m) for m in made]
+    ws = kv4.attention_workspace(40, 8, made[0][1], max_q=257)
+    for i in [0, 1, 2, 3, 4, 5, 1, 0, 2, 4, 3, 3, 0, 1] * 3:
+        assert torch.equal(_call(*made[i], workspace=ws), want[i])
+    assert _errors() == 0
+
+
 def test_attention_on_another_stream():
     rows, lens = [1, 1], [900, 33]
     q, cache, table = _make(4, rows, lens, 2, 8, 128, 64, torch.bfloat16)
