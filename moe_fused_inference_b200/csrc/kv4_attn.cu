@@ -36,8 +36,8 @@ using namespace kv4;
 // instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
 // has some 14 us beside it: the launch, three dependent trips (lengths, page table,
 // tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
-// heads: 1 sequence of 131072 tokens 27.7 us, 64 of up to 4096 34.5 us, 1 of 1152
-// 11.3 us.
+// heads: 1 sequence of 131072 tokens 27.1 us, 64 of up to 4096 32.0 us, 1 of 1152
+// 11.6 us, 5 rows over 8191 tokens 17.6 us.
 //
 // Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
@@ -53,7 +53,7 @@ using namespace kv4;
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
 constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
-constexpr int kOneLevel = 8;    // parts
+constexpr int kOneLevel = 16;   // parts; 8: five rows over 8191 tokens 21.5 instead of 19.8 us, 64: 131072 tokens 28.4 of 27.5
 
 template <int D, int kNT, int kPerSm>
 struct Few {
@@ -441,9 +441,16 @@ struct Part {
   unsigned start;  // the piece's first unit
 };
 struct Share {
-  unsigned hi;          // the share's end
-  unsigned base, more;  // CTA c takes `base` units, one more for c < more
+  unsigned hi;           // the share's end
+  unsigned units, ctas;  // CTA c takes units [c units / ctas, (c + 1) units / ctas)
 };
+// (x y - less) / d of 64 bits; in 32 where `units` of the call, times the CTAs, fit
+__device__ __forceinline__ unsigned scaled(unsigned x, unsigned y, unsigned d, unsigned units,
+                                           unsigned less = 0) {
+  static_assert(kFewCtas < 512, "2^23 units times the CTAs fit 32 bits");
+  return units < (1u << 23) ? (x * y - less) / d
+                            : unsigned(((unsigned long long)x * y - less) / d);
+}
 
 template <class E, int D, int kNT, int kPerSm>
 __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_attn_few_kernel(AttnArgs a) {
@@ -472,15 +479,25 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   auto units_of = [&](const Seq& s) {
     return s.rows * G > a.few ? 0u : unsigned(seq_tiles(s)) * a.Hkv * sets_of(s);
   };
-  unsigned U = 0;
-  for (int i = lane; i < a.n_seq; i += 32) U += units_of(sequence(a, i));
+  unsigned U = 0, pieces = 0;
+  for (int i = lane; i < a.n_seq; i += 32) {
+    const Seq s = sequence(a, i);
+    const unsigned n = units_of(s);
+    U += n;
+    pieces += n ? a.Hkv * sets_of(s) : 0;
+  }
   U = __reduce_add_sync(0xffffffffu, U);
+  pieces = __reduce_add_sync(0xffffffffu, pieces);
   if (U == 0) return;
-  // one tile a warp at least.  CTA c takes `base` units, one more for c < more.
-  const unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
+  // One tile a warp at least.  A multiple of the pieces, if that leaves out no more
+  // than a quarter of the CTAs: pieces of one length then begin where shares do, and
+  // no CTA has two parts to join (five rows over 8191 tokens 17.7 instead of 20.5 us,
+  // over 32768 30 instead of 35; with an eighth 16 sequences of 4096: 20.2 instead of
+  // 17.9; ragged pieces lose up to 0.5 us of 20).
+  unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
+  if (ctas > pieces && ctas % pieces * 4 <= ctas) ctas -= ctas % pieces;
   if (blockIdx.x >= ctas) return;
-  const unsigned base = U / ctas, more = U - base * ctas;
-  auto first_unit = [&](unsigned c) { return c * base + min(c, more); };
+  auto first_unit = [&](unsigned c) { return scaled(c, U, ctas, U); };
   // An end within kSnap tiles of an end of its piece moves there: what it would
   // split off costs less than the join.  A piece of up to 2 kSnap is never split.
   unsigned lo = first_unit(blockIdx.x), hi = first_unit(blockIdx.x + 1), seq_start = 0;
@@ -523,12 +540,11 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     hi = new_hi;
   }
   if (lo >= hi) return;
-  if (lane == 0) s_share[warp] = Share{hi, base, more};
+  if (lane == 0) s_share[warp] = Share{hi, U, ctas};
   __syncthreads();  // the barriers are initialised
   auto cta_of = [&](unsigned u) {
     const Share h = s_share[warp];
-    const unsigned x = h.more * (h.base + 1);
-    return u < x ? u / (h.base + 1) : h.more + (u - x) / h.base;
+    return scaled(u + 1, h.ctas, h.units, h.units, 1u);
   };
 
   // the part that holds unit u, of a sequence at or after p.seq (which starts at unit seq_start)
