@@ -909,7 +909,7 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   if (!cu_q && (long long)n_seq * max_q != T)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: without cu_q there are n_seq * max_q rows");
   if (T == 0 || n_seq == 0 || max_q == 0) return MFI_OK;
-  if (!q || !table || !kv_lens || !out || !workspace)
+  if (!q || (!table && width > 0) || !kv_lens || !out || !workspace)
     return mfi::set_last_error(MFI_ERR_ARG, "null pointer");
   if (reinterpret_cast<uintptr_t>(out) & 15)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: out must be 16-byte aligned");

@@ -382,6 +382,16 @@ def test_one_workspace_serves_calls_of_all_shapes_in_turn():
     assert _errors() == 0
 
 
+@pytest.mark.parametrize("rows", [1, 140])
+def test_attention_of_a_table_without_pages(rows):
+    """No sequence can have a token: zeros."""
+    cache = kv4.KV4Cache(2, 16, 2, 64)
+    q = torch.randn((2 * rows, 2, 64), device="cuda").half()
+    none = torch.empty((2, 0), dtype=torch.int32, device="cuda")
+    got = kv4.kv4_attention(q, cache, none, torch.zeros(2, dtype=torch.int32, device="cuda"))
+    assert not got.any() and _errors() == 0
+
+
 def test_attention_on_another_stream():
     rows, lens = [1, 1], [900, 33]
     q, cache, table = _make(4, rows, lens, 2, 8, 128, 64, torch.bfloat16)
