@@ -489,12 +489,15 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   U = __reduce_add_sync(0xffffffffu, U);
   pieces = __reduce_add_sync(0xffffffffu, pieces);
   if (U == 0) return;
-  // One tile a warp at least.  A multiple of the pieces, if that leaves out no more
+  // One tile a warp at least, but four CTAs a piece if there are as many: a CTA
+  // takes its pieces one after the other, some 4 us each (20 pieces of 1 tile 7
+  // instead of 43 us; with one CTA a piece ragged ones of 4 to 23 tiles 14.7
+  // instead of 10.8).  A multiple of the pieces, if that leaves out no more
   // than a quarter of the CTAs: pieces of one length then begin where shares do, and
   // no CTA has two parts to join (five rows over 8191 tokens 17.7 instead of 20.5 us,
   // over 32768 30 instead of 35; with an eighth 16 sequences of 4096: 20.2 instead of
   // 17.9; ragged pieces lose up to 0.5 us of 20).
-  unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
+  unsigned ctas = min(gridDim.x, max((U + F::kWarps - 1) / F::kWarps, min(U, 4 * pieces)));
   if (ctas > pieces && ctas % pieces * 4 <= ctas) ctas -= ctas % pieces;
   if (blockIdx.x >= ctas) return;
   auto first_unit = [&](unsigned c) { return scaled(c, U, ctas, U); };
