@@ -27,8 +27,8 @@ using namespace kv4;
 // ---- few rows: up to 64 vectors a sequence and KV head, on mma.sync -------------
 // A vector is one row of one query head; the R G vectors of a sequence and KV
 // head (v = r G + h) are taken 8 kNT at a time (a "set").  The work is the list
-// of all (sequence, KV head, set, tile of 16 tokens), in that order; CTA c takes
-// the c-th of `ctas` equal shares, whatever the sequences' lengths, and splits
+// of all (sequence, KV head, set, tile of 16 tokens), in that order, short pieces
+// padded; CTA c takes the c-th of `ctas` equal shares, whatever the lengths, and splits
 // each piece (sequence, head, set) of its share over its warps.  8 or 16 vectors
 // fill the n = 8 of mma.m16n8k16; an MMA of 64 or more would multiply zeros.
 //
@@ -36,8 +36,8 @@ using namespace kv4;
 // instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
 // has some 14 us beside it: the launch, three dependent trips (lengths, page table,
 // tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
-// heads: 1 sequence of 131072 tokens 27.1 us, 64 of up to 4096 32.0 us, 1 of 1152
-// 11.6 us, 5 rows over 8191 tokens 17.6 us.
+// heads: 1 sequence of 131072 tokens 26.9 us, 64 of up to 4096 30.8 us, 1 of 1152
+// 11.6 us, 5 rows over 8191 tokens 17.7 us.
 //
 // Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
@@ -53,6 +53,7 @@ using namespace kv4;
 //   products below 2^-28 of the largest weight times the largest scale, which
 //   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
 constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
+constexpr unsigned kLeast = 32;  // units of a piece at least
 constexpr int kOneLevel = 16;   // parts; 8: five rows over 8191 tokens 21.5 instead of 19.8 us, 64: 131072 tokens 28.4 of 27.5
 
 template <int D, int kNT, int kPerSm>
@@ -102,6 +103,17 @@ __device__ __forceinline__ uint32_t nonzero_half2(uint32_t a) {
 __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
 }
+
+// Units of work of sequence s's pieces: their tiles, but kLeast at least, for a
+// piece costs its start and joins (some 4 us) whatever its length: counted by their
+// tiles, 20 pieces of 1 tile went to two CTAs one after the other (43 us, now 7),
+// 8 empty ones beside 16 long ones cost 30 us more.  64 of up to 4096 tokens with 16
+// units 31.5 us, 32 30.8, 64 31.1.  Pieces of up to 2 kSnap units are never split, so
+// only whole ones have units without tiles.
+__device__ __forceinline__ int seq_units(const Seq& s) {
+  return s.rows > 0 ? max(int(kLeast), seq_tiles(s)) : 0;
+}
+static_assert(kLeast <= 2 * kSnap, "padded pieces are not split");
 
 // A warp's state: the running maximum (log2 domain) of each vector, the sum of
 // its weights times 2^10, and O^T times 2^(127 + 15 - top), top the largest
@@ -438,7 +450,7 @@ __device__ __forceinline__ void join_rows(int first, int step, int count, At at,
 struct Part {
   Seq s;
   int seq, g, v0, t_lo, t_hi, tiles;
-  unsigned start;  // the piece's first unit
+  unsigned start, next;  // the piece's first unit, the first one after this part
 };
 struct Share {
   unsigned hi;           // the share's end
@@ -477,7 +489,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   // at a time, then finds the sequences that hold the share's ends
   auto sets_of = [&](const Seq& s) { return (s.rows * G + F::kVec - 1) / F::kVec; };
   auto units_of = [&](const Seq& s) {
-    return s.rows * G > a.few ? 0u : unsigned(seq_tiles(s)) * a.Hkv * sets_of(s);
+    return s.rows * G > a.few ? 0u : unsigned(seq_units(s)) * a.Hkv * sets_of(s);
   };
   unsigned U = 0, pieces = 0;
   for (int i = lane; i < a.n_seq; i += 32) {
@@ -489,15 +501,12 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   U = __reduce_add_sync(0xffffffffu, U);
   pieces = __reduce_add_sync(0xffffffffu, pieces);
   if (U == 0) return;
-  // One tile a warp at least, but four CTAs a piece if there are as many: a CTA
-  // takes its pieces one after the other, some 4 us each (20 pieces of 1 tile 7
-  // instead of 43 us; with one CTA a piece ragged ones of 4 to 23 tiles 14.7
-  // instead of 10.8).  A multiple of the pieces, if that leaves out no more
+  // One unit a warp at least.  A multiple of the pieces, if that leaves out no more
   // than a quarter of the CTAs: pieces of one length then begin where shares do, and
   // no CTA has two parts to join (five rows over 8191 tokens 17.7 instead of 20.5 us,
   // over 32768 30 instead of 35; with an eighth 16 sequences of 4096: 20.2 instead of
   // 17.9; ragged pieces lose up to 0.5 us of 20).
-  unsigned ctas = min(gridDim.x, max((U + F::kWarps - 1) / F::kWarps, min(U, 4 * pieces)));
+  unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
   if (ctas > pieces && ctas % pieces * 4 <= ctas) ctas -= ctas % pieces;
   if (blockIdx.x >= ctas) return;
   auto first_unit = [&](unsigned c) { return scaled(c, U, ctas, U); };
@@ -510,7 +519,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     for (int i0 = 0; i0 < a.n_seq && before < hi; i0 += 32) {
       const int i = i0 + lane;
       const Seq s = i < a.n_seq ? sequence(a, i) : Seq{0, 0, 0};
-      const unsigned n = units_of(s), tiles = seq_tiles(s);
+      const unsigned n = units_of(s), each = seq_units(s);
       unsigned start = n;
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -520,8 +529,8 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
       const unsigned sum = __shfl_sync(0xffffffffu, start, 31);
       start += before - n;
       auto moved = [&](unsigned e) {
-        const unsigned in = (e - start) % tiles, out = tiles - in;
-        if (tiles > 2 * kSnap) return in <= kSnap ? e - in : (out <= kSnap ? e + out : e);
+        const unsigned in = (e - start) % each, out = each - in;
+        if (each > 2 * kSnap) return in <= kSnap ? e - in : (out <= kSnap ? e + out : e);
         return in < out ? e - in : e + out;
       };
       const unsigned has_lo = __ballot_sync(0xffffffffu, start <= lo && lo < start + n);
@@ -559,12 +568,14 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
       n = units_of(p.s);
     }
     p.tiles = seq_tiles(p.s);
-    const int piece = int((u - seq_start) / p.tiles), sets = sets_of(p.s);
+    const unsigned each = seq_units(p.s), hi = s_share[warp].hi;
+    const int piece = int((u - seq_start) / each), sets = sets_of(p.s);
     p.g = piece / sets;
     p.v0 = (piece - p.g * sets) * F::kVec;
-    p.start = seq_start + unsigned(piece) * p.tiles;
+    p.start = seq_start + unsigned(piece) * each;
+    p.next = min(hi, p.start + each);
     p.t_lo = int(u - p.start);
-    p.t_hi = int(min(s_share[warp].hi - p.start, unsigned(p.tiles)));
+    p.t_hi = int(min(hi - p.start, unsigned(p.tiles)));
   };
   // tiles go to the warps in runs of up to kChunk
   auto run_of = [&](const Part& p) { return min(F::kChunk, (p.t_hi - p.t_lo + F::kWarps - 1) / F::kWarps); };
@@ -635,8 +646,8 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     int nid = -1;
     {
       Part np = p;
-      if (p.start + p.t_hi < s_share[warp].hi) {
-        part_at(np, p.start + p.t_hi);
+      if (p.next < s_share[warp].hi) {
+        part_at(np, p.next);
         const int nrun = run_of(np);
         nid = page_of(row_of(np), nrun, np.t_lo + warp * nrun + lane, end_of(np));
       }
@@ -720,7 +731,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     p = s_now[warp];
     const Seq& s = p.s;
     const int nv = s.rows * G;
-    const bool more_parts = p.start + p.t_hi < s_share[warp].hi;
+    const bool more_parts = p.next < s_share[warp].hi;
     // the next part's first tiles and rows are on their way during the join; the
     // sums take the place of the stage read last
     float* sums = reinterpret_cast<float*>(ring + ((it + F::kStages - 1) % F::kStages) * F::kStageBytes);
@@ -924,7 +935,7 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   // most) are counted in 31 bits; the items of the other one are fewer than the rows
   // of `out`
   const double vectors = fmin(double(max_q) * (Hq / Hkv), double(mfi::kv4::kFew));
-  const double units = double(n_seq) * Hkv * (double(width) * page / mfi::kv4::kTile + 1) *
+  const double units = double(n_seq) * Hkv * (double(width) * page / mfi::kv4::kTile + mfi::kLeast) *
                        (vectors / 8 + 1);
   if (units >= 2147483648.0)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: more than 2^31 tiles of work in one call");

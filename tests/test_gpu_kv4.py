@@ -392,6 +392,19 @@ def test_attention_of_a_table_without_pages(rows):
     assert not got.any() and _errors() == 0
 
 
+@pytest.mark.parametrize("rows,lens,Hkv,G", [
+    ([1] * 12, [1, 5000, 0, 17, 3, 2100, 16, 0, 1, 1030, 33, 2], 4, 4),     # whole and split pieces, empty ones
+    ([1] * 9, [1, 1, 1, 1, 1, 1, 1, 1, 9000], 8, 2),
+    ([3, 1, 4, 2, 1], [3, 1100, 2500, 0, 1], 8, 5),
+    ([1] * 300, [i % 5 * 7 for i in range(300)], 2, 2),                     # more pieces than CTAs
+])
+def test_attention_of_very_unequal_lengths(rows, lens, Hkv, G):
+    q, cache, table = _make(31, rows, lens, Hkv, G, 64, 16, torch.bfloat16)
+    got = _call(q, cache, table, lens, rows)
+    assert _errors() == 0
+    _compare(got, q, cache, table, lens, rows)
+
+
 def test_attention_on_another_stream():
     rows, lens = [1, 1], [900, 33]
     q, cache, table = _make(4, rows, lens, 2, 8, 128, 64, torch.bfloat16)
