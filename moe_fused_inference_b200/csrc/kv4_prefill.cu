@@ -585,7 +585,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (!ok) break;
         tc::tc_fence_after();
         const uint32_t kref = s_ref[step % (4 * kSlots)].x, vref = s_ref[step % (4 * kSlots)].y;
-        const float sc = qs * __uint_as_float((127 + kref - 127 - kUp) << 23);
+        // not zero: a masked score of -inf has to stay -inf (S is below 2^37: what the
+        // bound adds to a score is below 2^-85)
+        const float sc = fmaxf(qs * __uint_as_float((127 + kref - 127 - kUp) << 23), 1e-37f);
         uint32_t s[kTok];
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c)

@@ -1,0 +1,54 @@
+"""Attention over the paged 4-bit KV cache where numbers run out of range: small,
+large and NaN keys, values and queries, against oracle/kv4.py in 64 bits."""
+
+import numpy as np
+import pytest
+import torch
+
+from moe_fused_inference_b200 import _lib, kv4
+from oracle import kv4 as ok
+from tests.test_gpu_kv4 import _call, _compare, _errors, _np
+
+pytestmark = pytest.mark.gpu
+
+
+def _cache(k, v, page=32):
+    """A cache that holds the tokens k, v (L, Hkv, D) on its pages in order, and
+    the page table of that one sequence."""
+    L, H, D = k.shape
+    cache = kv4.KV4Cache(max(1, -(-L // page)), page, H, D)
+    kv4.kv4_write(cache, k, v, torch.arange(L, device="cuda"))
+    return cache, np.arange(cache.num_pages, dtype=np.int32)[None]
+
+
+def _randn(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+# ---- small queries over small keys ----------------------------------------------
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("key_std", [0.0, 2.0 ** -60, 2.0 ** -30, 1.0])
+@pytest.mark.parametrize("q_std,scale", [(0.0, None), (2.0 ** -120, None), (2.0 ** -30, None),
+                                         (2.0 ** -24, None), (1.0, 0.0), (1.0, 2.0 ** -100)])
+def test_scores_too_small_to_tell_apart(rows, key_std, q_std, scale):
+    """The mean of the tokens that a row sees, not NaN: queries, keys or scales
+    whose product with the other two leaves fp32."""
+    L, H, G, D = 200, 2, 4, 128
+    k, v = _randn(1, 2, L, H, D)
+    cache, table = _cache(k * key_std, v)
+    q = (_randn(2, rows, H * G, D) * q_std).bfloat16()
+    _compare(_call(q, cache, table, [L], [rows], scale=scale), q, cache, table, [L], [rows], scale)
+    assert _errors() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("length", [0, 1, 200])
+def test_zero_rows_over_a_fresh_cache(rows, length):
+    """A padded or warm-up call: a pool that nobody wrote to, rows of zeros, and
+    rows that see no token give zeros."""
+    cache = kv4.KV4Cache(8, 32, 2, 64)
+    table = np.arange(8, dtype=np.int32)[None]
+    for q in (torch.zeros((rows, 8, 64), device="cuda").bfloat16(), _randn(3, rows, 8, 64).half()):
+        got = _call(q, cache, table, [length], [rows])
+        assert torch.equal(got, torch.zeros_like(q))
+    assert _errors() == 0
