@@ -95,10 +95,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-// all ones in the halves of a that are not zero
-__device__ __forceinline__ uint32_t nonzero_half2(uint32_t a) {
-  return __hne2_mask(*reinterpret_cast<const __half2*>(&a), __half2half2(__ushort_as_half(0)));
-}
 // Tiles of sequence s's pieces and their count of sets.
 __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
@@ -184,6 +180,27 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
     tops = __vmaxu2((ca + 0x00010001u) & 0x00FF00FFu, ((ca >> 8) + 0x00010001u) & 0x00FF00FFu);
     tops = __vmaxu2(tops, (cb + 0x00010001u) & 0x00FF00FFu);
     tops = __vmaxu2(tops, ((cb >> 8) + 0x00010001u) & 0x00FF00FFu);
+  }
+  // A NaN value block (rare) makes NaN of the vectors that see its token, whatever
+  // the weight, and of no others: written here, left out of the products.
+  const uint32_t bada = __vcmpeq4(ca, 0xFFFFFFFFu), badb = __vcmpeq4(cb, 0xFFFFFFFFu);
+  if (uint32_t left = __ballot_sync(0xffffffffu, (bada | badb) != 0u)) {
+    ca &= ~bada;
+    cb &= ~badb;
+    for (; left; left &= left - 1) {
+      const int src = __ffs(left) - 1;
+      const uint32_t a = __shfl_sync(0xffffffffu, bada, src), b = __shfl_sync(0xffffffffu, badb, src);
+      const int pa = pos0 + __shfl_sync(0xffffffffu, ti * kv4::kTile + ta, src);
+#pragma unroll
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t bad = (pa < q.lim[j][i] ? a : 0u) | (pa + 4 < q.lim[j][i] ? b : 0u);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            if ((bad >> (8 * (k / 2))) & 1u) w.o[j][k][i] = w.o[j][k][i + 2] = __uint_as_float(0x7FC00000u);
+        }
+    }
   }
   const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xFFFFu, tops >> 16));
   if (top > w.top) {
@@ -343,15 +360,6 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
         for (int b = 0; b < nb; ++b) {
           pf[j][b][0] = mul_half2(pa, ga[b]);
           pf[j][b][1] = mul_half2(pb, gb[b]);
-        }
-        if (edge) {
-          // a token that a vector does not see makes no NaN of its zero, whatever its code
-          const uint32_t ka = nonzero_half2(pa), kb = nonzero_half2(pb);
-#pragma unroll
-          for (int b = 0; b < nb; ++b) {
-            pf[j][b][0] &= ka;
-            pf[j][b][1] &= kb;
-          }
         }
       }
     }

@@ -52,3 +52,24 @@ def test_zero_rows_over_a_fresh_cache(rows, length):
         got = _call(q, cache, table, [length], [rows])
         assert torch.equal(got, torch.zeros_like(q))
     assert _errors() == 0
+
+
+# ---- a value that is NaN under a weight that rounds to zero ------------------------
+@pytest.mark.parametrize("rows", [1, 3, 8, 20, 140])
+@pytest.mark.parametrize("at", [0, 100, 250, 292, 297])
+@pytest.mark.parametrize("D", [64, 128])
+def test_nan_value_of_a_token_that_hardly_counts(rows, at, D):
+    """0 x NaN: the rows that see the token have NaN in its block of 32, wherever
+    the token lies and however small its weight, the others do not."""
+    L, H, G = 300, 2, 4
+    k, v = _randn(4, 2, L, H, D)
+    k[at] = -8.0                       # a score some 4 x 8 sqrt(D) below the others
+    v[at, 1, 40] = float("nan")
+    cache, table = _cache(k, v)
+    q = (4.0 + 0.1 * _randn(5, rows, H * G, D)).bfloat16()
+    got = _call(q, cache, table, [L], [rows])
+    first = max(0, at - (L - rows))    # first row that sees the token
+    want = torch.zeros_like(got, dtype=torch.bool)
+    want[first:, G:, 32:64] = True
+    assert torch.equal(got.isnan(), want)
+    assert _errors() == 0
