@@ -49,9 +49,11 @@ using namespace kv4;
 // * The query rows are scaled by a power of two to a maximum in [2^14, 2^15),
 //   which keeps all bits of a bf16 or fp16 row down to 2^-39 of its maximum.
 // * p is rounded to fp16 (2^-12) after a factor 2^10, and multiplied by 2^(c_b -
-//   top + 4), top the largest value code that the warp has seen: exact but for
-//   products below 2^-28 of the largest weight times the largest scale, which
-//   lose bits and vanish below 2^-39; codes 29 and more below top count as zero.
+//   top_b + 4), top_b the largest code that the warp has seen in block b of the
+//   values: exact but for products below 2^-28 of the largest weight times the
+//   block's largest scale, which lose bits and vanish below 2^-39; codes 29 and
+//   more below top_b count as zero.  (One top for all blocks dropped channels
+//   2^29 weaker than others.)
 constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
 constexpr unsigned kLeast = 32;  // units of a piece at least
 constexpr int kOneLevel = 16;   // parts; 8: five rows over 8191 tokens 21.5 instead of 19.8 us, 64: 131072 tokens 28.4 of 27.5
@@ -95,6 +97,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
+__device__ __forceinline__ uint32_t half_of(uint32_t w, int i) { return i ? w >> 16 : w & 0xFFFFu; }
 // Tiles of sequence s's pieces and their count of sets.
 __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;
@@ -112,12 +115,12 @@ __device__ __forceinline__ int seq_units(const Seq& s) {
 static_assert(kLeast <= 2 * kSnap, "padded pieces are not split");
 
 // A warp's state: the running maximum (log2 domain) of each vector, the sum of
-// its weights times 2^10, and O^T times 2^(127 + 15 - top), top the largest
-// value code plus one so far (a code of 255, NaN, counts as 0; two such
-// neighbours may carry one too many).
+// its weights times 2^10, and block b of O^T times 2^(127 + 15 - top_b), top_b the
+// block's largest value code plus one so far (a code of 255, NaN, counts as 0; two
+// such neighbours may carry one too many): halves of top[b % 2].
 template <int D, int kNT>
 struct Running {
-  uint32_t top;
+  uint32_t top[2];
   float m[kNT][2], l[kNT][2];
   float o[kNT][D / 16][4];
 };
@@ -164,7 +167,7 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
       }
     }
   }
-  uint32_t ca = 0, cb = 0, tops = 0;
+  uint32_t ca = 0, cb = 0, t0 = w.top[0], t1 = w.top[1];
   const int ti = lane >> 3, pr = lane & 7, ta = pr < 4 ? pr : pr + 4;
   if (ti < kN) {
     const uint8_t* c = base + ti * kv4::tile_bytes(D) + 16 * D + D / 2 + ta * nb;
@@ -177,9 +180,8 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
     }
     if (pos0 + ti * kv4::kTile + ta >= end) ca = 0;
     if (pos0 + ti * kv4::kTile + ta + 4 >= end) cb = 0;
-    tops = __vmaxu2((ca + 0x00010001u) & 0x00FF00FFu, ((ca >> 8) + 0x00010001u) & 0x00FF00FFu);
-    tops = __vmaxu2(tops, (cb + 0x00010001u) & 0x00FF00FFu);
-    tops = __vmaxu2(tops, ((cb >> 8) + 0x00010001u) & 0x00FF00FFu);
+    t0 = __vmaxu2(__vmaxu2(t0, (ca + 0x00010001u) & 0x00FF00FFu), (cb + 0x00010001u) & 0x00FF00FFu);
+    t1 = __vmaxu2(__vmaxu2(t1, ((ca >> 8) + 0x00010001u) & 0x00FF00FFu), ((cb >> 8) + 0x00010001u) & 0x00FF00FFu);
   }
   // A NaN value block (rare) makes NaN of the vectors that see its token, whatever
   // the weight, and of no others: written here, left out of the products.
@@ -202,28 +204,36 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
         }
     }
   }
-  const uint32_t top = __reduce_max_sync(0xffffffffu, max(tops & 0xFFFFu, tops >> 16));
-  if (top > w.top) {
-    const float c = __uint_as_float(max(127 + int(w.top) - int(top), 0) << 23);
-    w.top = top;
+  if (__any_sync(0xffffffffu, t0 != w.top[0] || t1 != w.top[1])) {
+    t0 = __reduce_max_sync(0xffffffffu, t0 & 0xFFFFu) | __reduce_max_sync(0xffffffffu, t0 >> 16) << 16;
+    t1 = __reduce_max_sync(0xffffffffu, t1 & 0xFFFFu) | __reduce_max_sync(0xffffffffu, t1 >> 16) << 16;
 #pragma unroll
-    for (int j = 0; j < kNT; ++j)
+    for (int b = 0; b < nb; ++b) {
+      const uint32_t now = half_of(b % 2 ? t1 : t0, b / 2), then = half_of(w.top[b % 2], b / 2);
+      const float c = __uint_as_float(max(127 + int(then) - int(now), 0) << 23);
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        w.o[j][k][0] *= c;
-        w.o[j][k][1] *= c;
-        w.o[j][k][2] *= c;
-        w.o[j][k][3] *= c;
-      }
+      for (int j = 0; j < kNT; ++j)
+#pragma unroll
+        for (int k = 2 * b; k < 2 * b + 2; ++k) {
+          w.o[j][k][0] *= c;
+          w.o[j][k][1] *= c;
+          w.o[j][k][2] *= c;
+          w.o[j][k][3] *= c;
+        }
+    }
+    w.top[0] = t0;
+    w.top[1] = t1;
   }
   if (ti < kN) {
-    const float u = __uint_as_float((127 + 127 + 5 - w.top) << 23);  // 2^(127 + 5 - top)
     float fa[nb], fb[nb];
     codes<nb>(ca, fa);
     codes<nb>(cb, fb);
     uint32_t h[nb];
 #pragma unroll
-    for (int b = 0; b < nb; ++b) h[b] = pack_half(fa[b] * u, fb[b] * u);
+    for (int b = 0; b < nb; ++b) {
+      const float u = __uint_as_float((127 + 127 + 5 - half_of(w.top[b % 2], b / 2)) << 23);  // 2^(127 + 5 - top_b)
+      h[b] = pack_half(fa[b] * u, fb[b] * u);
+    }
     uint32_t* dst = vf + (ti * 8 + pr) * nb;
     if (nb == 4)
       *reinterpret_cast<uint4*>(dst) = make_uint4(h[0], h[1], h[nb - 2], h[nb - 1]);
@@ -705,7 +715,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     }
 
     Running<D, kNT> w;
-    w.top = 29;  // a block of zeros
+    w.top[0] = w.top[1] = 29u << 16 | 29u;  // blocks of zeros
 #pragma unroll
     for (int j = 0; j < kNT; ++j) {
       w.m[j][0] = w.m[j][1] = -INFINITY;
@@ -753,7 +763,9 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
-    const float unit = __uint_as_float((w.top - 5) << 23);  // 2^(top - 127 - 15 + 10)
+    float unit[nb];  // 2^(top_b - 127 - 15 + 10)
+#pragma unroll
+    for (int b = 0; b < nb; ++b) unit[b] = __uint_as_float((half_of(w.top[b % 2], b / 2) - 5) << 23);
 #pragma unroll
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
@@ -765,8 +777,8 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
 #pragma unroll
         for (int b = 0; b < nb; ++b)
           *reinterpret_cast<float4*>(dst + 32 * b + 4 * gid) =
-              make_float4(w.o[j][2 * b][i] * unit, w.o[j][2 * b][i + 2] * unit,
-                          w.o[j][2 * b + 1][i] * unit, w.o[j][2 * b + 1][i + 2] * unit);
+              make_float4(w.o[j][2 * b][i] * unit[b], w.o[j][2 * b][i + 2] * unit[b],
+                          w.o[j][2 * b + 1][i] * unit[b], w.o[j][2 * b + 1][i + 2] * unit[b]);
         if (gid == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(w.m[j][i], w.l[j][i]);
       }
     if (lane == 0) s_sums[warp] = sums;

@@ -73,3 +73,34 @@ def test_nan_value_of_a_token_that_hardly_counts(rows, at, D):
     want[first:, G:, 32:64] = True
     assert torch.equal(got.isnan(), want)
     assert _errors() == 0
+
+
+# ---- values of very different strength -----------------------------------------------
+def _compare_blocks(got, q, cache, table, L):
+    """The bound of oracle/kv4.py for each block of 32 channels by itself, with the
+    largest value that the row sees in that block instead of the whole head; and
+    2^-31 of it for each token, whose weight and scale may fall below fp16."""
+    pool, (R, Hq, D) = cache.data.cpu().numpy(), q.shape
+    want, bound = ok.attention(_np(q), pool, table, [L], [R])
+    pos = np.arange(L)
+    _, v = ok.read(pool, table[0][pos // cache.page].astype(np.int64) * cache.page + pos % cache.page)
+    err = np.abs(_np(got) - want)
+    for r in range(R):
+        for h in range(Hq):
+            seen = np.abs(v[:L - R + r + 1, h * pool.shape[1] // Hq])
+            top = seen.reshape(len(seen), D // 32, 32).max((0, 2))
+            tol = np.repeat((bound[r, h, 0] / seen.max() + L * 2.0 ** -31) * top, 32)
+            assert (err[r, h] <= tol + 2.0 ** -8 * np.abs(want[r, h])).all(), (r, h)
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8])
+@pytest.mark.parametrize("D", [64, 128])
+def test_weak_channels_beside_strong_ones(rows, D):
+    """Blocks of channels 2^-70 to 2^40 of each other keep their own accuracy."""
+    L, H, G = 333, 2, 4
+    k, v = _randn(6, 2, L, H, D)
+    strength = torch.tensor([2.0 ** 20, 2.0 ** -20, 2.0 ** 30, 2.0 ** -40][:D // 32], device="cuda")
+    cache, table = _cache(k, v * strength.repeat_interleave(32))
+    q = (2.0 * _randn(7, rows, H * G, D)).bfloat16()
+    _compare_blocks(_call(q, cache, table, [L], [rows]), q, cache, table, L)
+    assert _errors() == 0
