@@ -97,7 +97,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
-__device__ __forceinline__ uint32_t half_of(uint32_t w, int i) { return i ? w >> 16 : w & 0xFFFFu; }
 // Tiles of sequence s's pieces and their count of sets.
 __device__ __forceinline__ int seq_tiles(const Seq& s) {
   return s.rows > 0 ? max(1, (s.len + kv4::kTile - 1) / kv4::kTile) : 0;

@@ -63,6 +63,7 @@ constexpr int kFew = 64;                   // vectors of a sequence and KV head 
 constexpr size_t few_bytes(int D) { return size_t(kFewCtas) * 2 * 16 * (D + 4) * sizeof(float); }
 constexpr size_t many_bytes(int D) { return size_t(kCtas) * 256 * (D + 2) * sizeof(float); }
 
+__device__ __forceinline__ uint32_t half_of(uint32_t w, int i) { return i ? w >> 16 : w & 0xFFFFu; }
 __device__ __forceinline__ float ex2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));

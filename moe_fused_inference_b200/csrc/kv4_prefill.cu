@@ -21,13 +21,15 @@
 // takes 50 clocks and one of 128 takes 65 (both operands from shared memory).
 //
 // The operands are fp16: a query row times a power of two that brings its
-// maximum to [2^14, 2^15), a key or value element times 2^(c - ref + 12) with
-// ref the largest code (of the keys' 64 tokens, of the item's values so far):
-// exact unless 2^-36 below it.
-// P is rounded to fp16 after a factor 2^3; the maximum that it refers to moves
-// when it is passed by 2^9 (2^7: 1.76 instead of 1.71 ms), the value scale that O
-// refers to when passed by 2^3,
-// so P stays below 2^15.  l and O are fp32.
+// maximum to [2^14, 2^15), a key or value element times 2^(c - ref + 13).  The
+// keys' ref is the largest code of the 64 tokens: exact unless 2^-37 below it.  The
+// values have one for each block of 32 channels, which O refers to as well: set 3
+// above the block's largest code, and again when a code passes it, so exact unless
+// 2^-34 below the largest so far of the same block.
+// P is rounded to fp16 after a factor 2^6; the maximum that it refers to moves
+// when it is passed by 2^9 (2^7: 1.76 instead of 1.71 ms), so P stays below 2^15;
+// weights below 2^-20 of the reference lose bits, those below 2^-31 vanish.  l and O
+// are fp32.
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -49,9 +51,9 @@ constexpr int kRows = 128;                 // vectors of a tile
 constexpr int kThreads = 512;
 constexpr int kRegsSoftmax = 168, kRegsDecode = 112, kRegsOther = 64;
 static_assert(2 * kRegsSoftmax + kRegsDecode + kRegsOther <= 512, "registers of the launch: 128 a thread");
-constexpr float kLazy = 9.0f, kShift = 3.0f;  // log2: the maximum's slack, the weights' factor
-constexpr int kVSlack = 3;                    // log2: the value scale's slack
-constexpr int kUp = 12;                       // log2: the elements' factor
+constexpr float kLazy = 9.0f, kShift = 6.0f;  // log2: the maximum's slack, the weights' factor
+constexpr uint32_t kVSlack = 3;               // log2: the value references' slack
+constexpr int kUp = 13;                       // log2: the elements' factor
 
 template <int D>
 struct Many {
@@ -163,8 +165,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   __shared__ Bars bar;
   __shared__ Item s_item[2];
   __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN
-  // of a step: the key and value codes that its operands refer to, whether there
-  // are NaN values.  Its writer is at most 2 kSlots steps ahead of its last reader.
+  // of a step: the key code that its operands refer to, whether there are NaN values
+  // (bit 0) and whether the values' codes are others than the step's before (bit 1),
+  // these, of blocks 0 and 2 (halves), 1 and 3.  Its writer is at most 2 kSlots steps
+  // ahead of its last reader.
   __shared__ uint4 s_ref[4 * kSlots];
   __shared__ uint32_t s_tmem;
   // (from lane 0: the roles' branches are then known to be uniform)
@@ -384,8 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       }
       if (tc::cta_aborted() && leader) tc::drain_mma(&bar.drain[i]);
     } else if (warp == 15) {
-      // ---- the largest codes (255, NaN, not counted): of the step's keys, of the
-      // item's values so far
+      // ---- the codes that the operands refer to (255, NaN, not counted)
       uint32_t step = 0;
       bool ok = true;
       for (uint32_t n = 0; ok; ++n) {
@@ -393,46 +396,66 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
         const int valid = s_item[slot].valid, steps = s_item[slot].steps;
         const int pos = s_item[slot].step0 * kTok, len = s_item[slot].len - pos;  // of the part
-        uint32_t vtop = 28u;  // a block of zeros
+        uint32_t v02 = 28u << 16 | 28u, v13 = v02;  // blocks of zeros
         for (int j = 0; valid && j < steps; ++j, ++step) {
           ok = wait_slot(bar.raw_full, step, 1);
           if (!ok) break;
           const uint8_t* raw = smem + M::kOffRaw + (step % kSlots) * M::kRaw;
-          uint32_t ref[2];
-          bool nan[2];
+          uint32_t wk[kTok / 32], wv[kTok / 32];  // codes of tokens lane, lane + 32
 #pragma unroll
-          for (int kv = 0; kv < 2; ++kv) {
-            uint32_t w[kTok / 32], m = 0;  // codes of tokens lane, lane + 32
+          for (int x = 0; x < kTok / 32; ++x) {
+            const int tok = x * 32 + lane;
+            const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + (tok % kTile) * nb;
+            wk[x] = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+            c += D / 2;
+            wv[x] = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
+            if (j * kTok + tok >= len) wk[x] = wv[x] = 0u;
+          }
+          auto evens = [](const uint32_t (&w)[kTok / 32]) { return __vmaxu2(w[0] & 0x00FF00FFu, w[1] & 0x00FF00FFu); };
+          auto odds = [](const uint32_t (&w)[kTok / 32]) {
+            return __vmaxu2((w[0] >> 8) & 0x00FF00FFu, (w[1] >> 8) & 0x00FF00FFu);
+          };
+          static_assert(kTok == 64, "two tokens a lane");
+          auto largest = [&] {
+            const uint32_t m = __vmaxu2(evens(wk), odds(wk));
+            return __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
+          };
+          uint32_t kref = largest();
+          if (kref == 255u) {  // rare: once more without them
+#pragma unroll
+            for (int x = 0; x < kTok / 32; ++x) wk[x] &= ~__vcmpeq4(wk[x], 0xFFFFFFFFu);
+            kref = largest();
+          }
+          kref = max(kref, 28u);
+          // the values' references, of 254 at most, move when a code passes one
+          uint32_t e = __vmaxu2(evens(wv), v02), o = __vmaxu2(odds(wv), v13), nan = 0u, moved = 0u;
+          if (__any_sync(0xffffffffu, e != v02 || o != v13)) {
 #pragma unroll
             for (int x = 0; x < kTok / 32; ++x) {
-              const int tok = x * 32 + lane;
-              const uint8_t* c = raw + (tok / kTile) * tile_bytes(D) + 16 * D + kv * (D / 2) + (tok % kTile) * nb;
-              w[x] = nb == 4 ? *reinterpret_cast<const uint32_t*>(c) : *reinterpret_cast<const uint16_t*>(c);
-              if (j * kTok + tok >= len) w[x] = 0u;
-              m = __vmaxu2(__vmaxu2(m, w[x] & 0x00FF00FFu), (w[x] >> 8) & 0x00FF00FFu);
+              const uint32_t bad = __vcmpeq4(wv[x], 0xFFFFFFFFu);
+              // a NaN value block counts for the rows that see it only: noted here,
+              // written at the end, and zero in the product
+              for (int b = 0; b < nb; ++b)
+                if ((bad >> (8 * b)) & 1u) atomicMin(&s_nan[slot][b], pos + j * kTok + x * 32 + lane);
+              wv[x] &= ~bad;
+              nan |= bad;
             }
-            m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
-            nan[kv] = m == 255u;
-            if (nan[kv]) {  // rare: once more without them
-              m = 0;
-#pragma unroll
-              for (int x = 0; x < kTok / 32; ++x) {
-                const uint32_t bad = __vcmpeq4(w[x], 0xFFFFFFFFu);
-                // a NaN value block counts for the rows that see it only: noted here,
-                // written at the end, and zero in the product
-                for (int b = 0; b < nb; ++b)
-                  if (kv && ((bad >> (8 * b)) & 1u)) atomicMin(&s_nan[slot][b], pos + j * kTok + x * 32 + lane);
-                w[x] &= ~bad;
-                m = __vmaxu2(__vmaxu2(m, w[x] & 0x00FF00FFu), (w[x] >> 8) & 0x00FF00FFu);
-              }
-              m = __reduce_max_sync(0xffffffffu, max(m & 0xFFFFu, m >> 16));
-            }
-            ref[kv] = max(m, 28u);
+            nan = __any_sync(0xffffffffu, nan != 0u);
+            e = __vmaxu2(evens(wv), v02);
+            o = __vmaxu2(odds(wv), v13);
+            auto passed = [&](uint32_t now, uint32_t then) {
+              const uint32_t top = __reduce_max_sync(0xffffffffu, now);
+              return top > then ? min(top + kVSlack, 254u) : then;
+            };
+            const uint32_t n02 = passed(e & 0xFFFFu, v02 & 0xFFFFu) | passed(e >> 16, v02 >> 16) << 16;
+            const uint32_t n13 = passed(o & 0xFFFFu, v13 & 0xFFFFu) | passed(o >> 16, v13 >> 16) << 16;
+            moved = j > 0 && (n02 != v02 || n13 != v13) ? 2u : 0u;
+            v02 = n02;
+            v13 = n13;
           }
-          vtop = max(vtop, ref[1]);
           __syncwarp();
           if (lane == 0) {
-            s_ref[step % (4 * kSlots)] = make_uint4(ref[0], vtop, nan[1], 0u);
+            s_ref[step % (4 * kSlots)] = make_uint4(kref, nan | moved, v02, v13);
             tc::mbar_arrive(&bar.ref_full[step % kSlots]);
           }
         }
@@ -479,20 +502,25 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
               w[kv][x][0] = y.x; w[kv][x][1] = y.y;
             }
           }
+        float u[2][nb];  // 2^(127 + kUp - ref)
+#pragma unroll
+        for (int b = 0; b < nb; ++b) {
+          u[0][b] = __uint_as_float((127 + 127 + kUp - ref.x) << 23);
+          u[1][b] = __uint_as_float((127 + 127 + kUp - half_of(b % 2 ? ref.w : ref.z, b / 2)) << 23);
+        }
         ok = step < kSlots || wait_slot(bar.kv_empty, step - kSlots, 1);
         if (!ok) break;
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           const uint32_t dst = (kv ? M::kOffV : M::kOffK) + st * M::kOperand + at;
-          const float u = __uint_as_float((127 + 127 + kUp - (kv ? ref.y : ref.x)) << 23);  // 2^(127 + kUp - ref)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            if (kv && ref.z) cw[kv][x] &= ~__vcmpeq4(cw[kv][x], 0xFFFFFFFFu);
+            if (kv && (ref.y & 1u)) cw[kv][x] &= ~__vcmpeq4(cw[kv][x], 0xFFFFFFFFu);
             float f[nb];
             codes<nb>(cw[kv][x], f);
 #pragma unroll
             for (int b = 0; b < nb; ++b) {
-              const uint32_t h = pack_half(f[b] * u, f[b] * u);
+              const uint32_t h = pack_half(f[b] * u[kv][b], f[b] * u[kv][b]);
               // values: pieces 2t and 2t + 1 of a block make its 8 elements
               const uint32_t e = kv ? __byte_perm(w[kv][x][b / 2], w[kv][x][nb / 2 + b / 2], b % 2 ? 0x7632 : 0x5410)
                                     : w[kv][x][b];
@@ -578,15 +606,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const int lim = v < nv ? it.len - it.rows + v / G + 1 - pos : 0;
       const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1 - pos;
       float m = -INFINITY, l = 0.0f;
-      uint32_t vrun = 0;  // the value code that O refers to
       for (int j = 0; j < it.steps; ++j, ++step) {
         const uint32_t buf = step & 1u, tb = ts + buf * 64;
         ok = wait(&bar.s_full[i][buf], step >> 1, 3);
         if (!ok) break;
         tc::tc_fence_after();
-        const uint32_t kref = s_ref[step % (4 * kSlots)].x, vref = s_ref[step % (4 * kSlots)].y;
-        // not zero: a masked score of -inf has to stay -inf (S is below 2^37: what the
-        // bound adds to a score is below 2^-85)
+        const uint32_t kref = s_ref[step % (4 * kSlots)].x;
+        const bool vup = (s_ref[step % (4 * kSlots)].y & 2u) != 0u;
+        // not zero: a masked score of -inf has to stay -inf (S is below 2^38: what the
+        // bound adds to a score is below 2^-84)
         const float sc = fmaxf(qs * __uint_as_float((127 + kref - 127 - kUp) << 23), 1e-37f);
         uint32_t s[kTok];
 #pragma unroll
@@ -607,15 +635,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         }
         const float top = fmaxf(t0, t1) * sc;
         const bool up = top > m + kLazy;
-        const bool vup = j == 0 || int(vref) > int(vrun) + kVSlack;
         if (__any_sync(0xffffffffu, up) || vup) {
-          float c = up ? ex2(m - top) : 1.0f;
+          const float c = up ? ex2(m - top) : 1.0f;
           if (up) m = top;
           l *= c;
-          if (vup) {
-            c *= j == 0 ? 0.0f : __uint_as_float(uint32_t(max(127 + int(vrun) - int(vref), 0)) << 23);
-            vrun = vref;
-          }
           if (j > 0) {
             // the products of the step before (those before that are complete: these
             // scores came after them)
@@ -624,19 +647,23 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             tc::tc_fence_after();
 #pragma unroll 1
             for (int x = 0; x < D / 16; ++x) {
+              float cv = c;
+              if (vup) {
+                const int b = x / 2;
+                const uint4 now = s_ref[step % (4 * kSlots)], then = s_ref[(step - 1) % (4 * kSlots)];
+                const uint32_t moved = half_of(b % 2 ? now.w - then.w : now.z - then.z, b / 2);
+                cv *= __uint_as_float(uint32_t(max(127 - int(moved), 0)) << 23);
+              }
               uint32_t o[16];
               tc::tmem_ld_32x32b_x16(to + 16 * x, o);
               tc::tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * c);
+              for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * cv);
               tmem_st_x16(to + 16 * x, o);
             }
           }
         }
-        // p 2^(kShift + vref - vrun), l without the latter
-        const int dv = int(vref) - int(vrun);
-        const float down = __uint_as_float(uint32_t(127 - dv) << 23);  // 2^-dv, dv = 0 .. kVSlack
-        const float b0 = kShift + float(dv) - (m == -INFINITY ? 0.0f : m);
+        const float b0 = kShift - (m == -INFINITY ? 0.0f : m);
         const float2 sc2 = make_float2(sc, sc), b2 = make_float2(b0, b0);
         float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -655,7 +682,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           tmem_st_x16(tb + 16 * h, p);
         }
         sum0 = add2(sum0, sum1);
-        l = fmaf(sum0.x + sum0.y, down, l);
+        l += sum0.x + sum0.y;
         tmem_st_wait();
         tc::tc_fence_before();
         __syncwarp();
@@ -672,21 +699,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       ok = wait(&bar.o_done[i][(step - 1) & 1u], (step - 1) >> 1, 3);
       if (!ok) break;
       tc::tc_fence_after();
-      const float unit = __uint_as_float((vrun - kUp) << 23);  // O's: 2^(vrun - 127 - kUp)
+      const uint4 ref = s_ref[(step - 1) % (4 * kSlots)];
       const float nan = __uint_as_float(0x7FC00000u);
       E* out = static_cast<E*>(a.out) +
                ((long long)(it.row0 + v / G) * a.Hq + it.g * G + v % G) * D;
       // a part leaves [D + 2][256 vectors] sums
       float* sums = a.part + size_t(it.index) * (256 * (D + 2)) + i * kRows + r;
-      const float inv = it.parts > 1 ? unit : (l == 0.0f ? 0.0f : unit / l);
+      const float inv = it.parts > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
         tc::tmem_ld_32x32b_x32(to + 32 * x, o);
         tc::tmem_ld_wait();
         const bool bad = lim + pos > s_nan[n & 1u][x];
+        const float unit = __uint_as_float((half_of(x % 2 ? ref.w : ref.z, x / 2) - kUp) << 23);  // O's: 2^(ref - 127 - kUp)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(bad ? nan : __uint_as_float(o[k]) * inv);
+        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(bad ? nan : __uint_as_float(o[k]) * inv * unit);
         if (it.parts > 1) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) __stcg(sums + (32 * x + k) * 256, __uint_as_float(o[k]));

@@ -93,7 +93,7 @@ def _compare_blocks(got, q, cache, table, L):
             assert (err[r, h] <= tol + 2.0 ** -8 * np.abs(want[r, h])).all(), (r, h)
 
 
-@pytest.mark.parametrize("rows", [1, 3, 8])
+@pytest.mark.parametrize("rows", [1, 3, 8, 40])
 @pytest.mark.parametrize("D", [64, 128])
 def test_weak_channels_beside_strong_ones(rows, D):
     """Blocks of channels 2^-70 to 2^40 of each other keep their own accuracy."""
@@ -102,5 +102,18 @@ def test_weak_channels_beside_strong_ones(rows, D):
     strength = torch.tensor([2.0 ** 20, 2.0 ** -20, 2.0 ** 30, 2.0 ** -40][:D // 32], device="cuda")
     cache, table = _cache(k, v * strength.repeat_interleave(32))
     q = (2.0 * _randn(7, rows, H * G, D)).bfloat16()
+    _compare_blocks(_call(q, cache, table, [L], [rows]), q, cache, table, L)
+    assert _errors() == 0
+
+
+@pytest.mark.parametrize("L,rows", [(3000, 1), (3000, 40), (300, 140)])
+def test_values_that_grow_along_the_sequence(L, rows):
+    """The references of the values move with the tokens: 2^-90 to 2^60, one block
+    falling while the others rise, in parts that are joined as well."""
+    H, G, D = 1, 4, 128
+    k, v = _randn(8, 2, L, H, D)
+    power = torch.linspace(-90.0, 60.0, L, device="cuda")[:, None] * torch.tensor([1.0, -1.0, 0.5, 0.0], device="cuda")
+    cache, table = _cache(k, v * torch.exp2(power.floor()).repeat_interleave(32, 1)[:, None])
+    q = _randn(9, rows, H * G, D).bfloat16()
     _compare_blocks(_call(q, cache, table, [L], [rows]), q, cache, table, L)
     assert _errors() == 0
