@@ -47,13 +47,15 @@ using namespace kv4;
 // go to the few scores and weights.  A stage's codes are turned into factors by
 // one lane each and read back from shared memory.
 // * The query rows are scaled by a power of two to a maximum in [2^14, 2^15),
-//   which keeps all bits of a bf16 or fp16 row down to 2^-39 of its maximum.
+//   which keeps all bits of a bf16 or fp16 row down to 2^-39 of its maximum; the key
+//   factors by 2^-13, so that a score of keys up to 2^117 fits fp32.
 // * p is rounded to fp16 (2^-12) after a factor 2^10, and multiplied by 2^(c_b -
 //   top_b + 4), top_b the largest code that the warp has seen in block b of the
 //   values: exact but for products below 2^-28 of the largest weight times the
 //   block's largest scale, which lose bits and vanish below 2^-39; codes 29 and
 //   more below top_b count as zero.  (One top for all blocks dropped channels
 //   2^29 weaker than others.)
+constexpr float kKeyUnit = 0x1p-13f;
 constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
 constexpr unsigned kLeast = 32;  // units of a piece at least
 constexpr int kOneLevel = 16;   // parts; 8: five rows over 8191 tokens 21.5 instead of 19.8 us, 64: 131072 tokens 28.4 of 27.5
@@ -162,7 +164,8 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
       if (kN * kWords % 32 == 0 || i < kN) {
         float f[4];
         codes<4>(*reinterpret_cast<const uint32_t*>(base + i * kv4::tile_bytes(D) + 16 * D + 4 * x), f);
-        *reinterpret_cast<float4*>(kf + (i * kWords + x) * 4) = make_float4(f[0], f[1], f[2], f[3]);
+        *reinterpret_cast<float4*>(kf + (i * kWords + x) * 4) =
+            make_float4(f[0] * kKeyUnit, f[1] * kKeyUnit, f[2] * kKeyUnit, f[3] * kKeyUnit);
       }
     }
   }
@@ -241,7 +244,7 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
   }
   __syncwarp();
 
-  // ---- scores, without qs
+  // ---- scores, without qs (which has the keys' 2^13)
   float s[kN][kNT][4];
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
@@ -707,7 +710,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
       for (int i = 0; i < 2; ++i) {
         const int ee = __shfl_sync(0xffffffffu, e, (2 * tig + i) * 4);
         q.qs[j][i] = fmaxf(fabsf(a.scale) * 1.44269504088896341f *
-                               __uint_as_float(uint32_t(127 - 14 + ee) << 23), 1e-37f);
+                               __uint_as_float(uint32_t(127 - 14 + 13 + ee) << 23), 1e-37f);
         const int c = p.v0 + 8 * j + 2 * tig + i;
         q.lim[j][i] = c < p.s.rows * G ? len - p.s.rows + c / G + 1 : 0;
       }

@@ -548,7 +548,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
     const int i = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + i * 128, to = tmem + lanes + 256 + i * 128;
-    // load the item's query row, scaled to a maximum near 2^15; its scores lack qs
+    // load the item's query row, scaled to a maximum near 2^15; its scores lack qs 2^-13
+    // (a power that keeps qs off the ends of fp32)
     auto load_q = [&](const Item& it) {
       const int v = it.v0 + i * kRows + r;
       uint4 x[D / 8];
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       tc::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&bar.q_full[i]);
-      return fmaxf(fabsf(a.scale) * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + e) << 23), 1e-37f);
+      return fabsf(a.scale) * 1.44269504088896341f * __uint_as_float(uint32_t(127 - 14 + 13 + e) << 23);
     };
     uint32_t step = 0;
     Item it{};
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         const bool vup = (s_ref[step % (4 * kSlots)].y & 2u) != 0u;
         // not zero: a masked score of -inf has to stay -inf (S is below 2^38: what the
         // bound adds to a score is below 2^-84)
-        const float sc = fmaxf(qs * __uint_as_float((127 + kref - 127 - kUp) << 23), 1e-37f);
+        const float sc = fmaxf(qs * __uint_as_float((127 + kref - 127 - kUp - 13) << 23), 1e-37f);
         uint32_t s[kTok];
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c)

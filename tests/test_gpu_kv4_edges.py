@@ -117,3 +117,16 @@ def test_values_that_grow_along_the_sequence(L, rows):
     q = _randn(9, rows, H * G, D).bfloat16()
     _compare_blocks(_call(q, cache, table, [L], [rows]), q, cache, table, L)
     assert _errors() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 3, 140])
+@pytest.mark.parametrize("key,query,scale", [(110, -110, None), (-90, 92, None), (112, -95, 2.0 ** -20),
+                                             (110, 0, 2.0 ** -113), (-80, -30, 2.0 ** 108)])
+def test_scores_of_ordinary_size_from_extreme_factors(rows, key, query, scale):
+    """Keys, queries and scales far from 1 whose product is not."""
+    L, H, G, D = 300, 2, 4, 128
+    k, v = _randn(10, 2, L, H, D)
+    cache, table = _cache(k * 2.0 ** key, v)
+    q = (_randn(11, rows, H * G, D) * 2.0 ** query).bfloat16()
+    _compare(_call(q, cache, table, [L], [rows], scale=scale), q, cache, table, [L], [rows], scale)
+    assert _errors() == 0
