@@ -126,26 +126,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   return r;
 }
 
-// Wait for a phase of a barrier, as a whole warp.  The polls are a loop inside the
-// instruction block: few instructions (they take issue slots from the other
-// roles), and no divergence in the compiler's eyes (the issuing warps' descriptors
-// stay in uniform registers).  A poll sleeps in hardware; the count limits them to
-// seconds.
-__device__ __forceinline__ bool wait_uniform(uint32_t bar, uint32_t parity, int* err, int code) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 0;\n"
-      "AGAIN:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
-      " add.u32 n, n, 1;\n setp.lt.u32 q, n, 4000000;\n @q bra AGAIN;\n"
-      "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  const bool all = __all_sync(0xffffffffu, ok != 0) != 0;
-  if (!all) tc::cta_fail(err, code);
-  return all;
-}
-
 struct Bars {
   uint64_t item_full[2], item_empty[2];            // the next item's description
   uint64_t raw_full[kSlots], raw_empty[kSlots];    // a step's tiles,
@@ -207,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   // wait for the n-th completion (from 0) of a barrier; the warp goes on or gives
   // up as one
   auto wait = [&](uint64_t* b, uint32_t n, int code) {
-    return wait_uniform(tc::smem_u32(b), n & 1u, err, code);
+    return tc::mbar_wait_warp(b, n & 1u, err, code);
   };
   // the n-th completion of the barrier of step n's slot
   auto wait_slot = [&](uint64_t* b, uint32_t n, int code) { return wait(b + n % kSlots, n / kSlots, code); };

@@ -14,6 +14,7 @@
 // NaN (only NaN-ness is observable downstream: the quantiser maps every NaN
 // to the same code).
 #include "mx_common.cuh"
+#include "tc_ptx.cuh"
 #include "work.cuh"
 
 #include "../../include/moe_fp4.h"
@@ -64,6 +65,47 @@ __global__ void __launch_bounds__(256) selftest_kernel(unsigned long long* out) 
   }
 }
 
+// The bounded waits of a CTA's roles (tc_ptx.cuh), one warp waiting: on a barrier that
+// completes, on one that never does, and on one that never does while the other
+// warp reports a failure after 1 ms.  out[2 i], out[2 i + 1]: what the i-th wait
+// returned, and its ns; out[6]: the code that the second one reported.
+template <bool kWarp>
+__global__ void __launch_bounds__(64) selftest_wait_kernel(unsigned long long* out) {
+  __shared__ uint64_t done, never;
+  __shared__ int err[2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    tc::mbar_init(&done, 1);
+    tc::mbar_init(&never, 1);
+    tc::fence_mbar_init();
+    tc::cta_abort_init();
+    err[0] = err[1] = 0;
+  }
+  __syncthreads();
+  if (threadIdx.x == 32) tc::mbar_arrive(&done);
+  for (int i = 0; i < 3; ++i) {
+    if (i == 2 && threadIdx.x == 0) tc::cta_abort_init();
+    __syncthreads();
+    if (i == 2 && threadIdx.x == 32) {
+      const uint64_t t0 = tc::globaltimer_ns();
+      while (tc::globaltimer_ns() - t0 < 1000000ull) __nanosleep(1000);
+      tc::cta_fail(&err[1], 9);
+    }
+    if (warp == 0) {
+      const uint64_t t0 = tc::globaltimer_ns();
+      uint64_t* bar = i == 0 ? &done : &never;
+      const bool ok = kWarp ? tc::mbar_wait_warp(bar, 0, &err[0], 3) : tc::mbar_wait(bar, 0, &err[0], 3);
+      const uint64_t ns = tc::globaltimer_ns() - t0;
+      if (lane == 0) {
+        out[2 * i] = ok;
+        out[2 * i + 1] = ns;
+      }
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[6] = (unsigned long long)err[0];
+}
+
 __global__ void selftest_init_kernel(unsigned long long* out) {
   if (threadIdx.x < 4) out[threadIdx.x] = threadIdx.x < 2 ? 0ull : ~0ull;
 }
@@ -78,6 +120,17 @@ extern "C" int mfi_selftest_numerics(unsigned long long* out, void* stream) {
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   mfi::selftest_init_kernel<<<1, 32, 0, st>>>(out);
   mfi::selftest_kernel<<<148 * 8, 256, 0, st>>>(out);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MFI_OK : mfi::set_last_error(MFI_ERR_CUDA, cudaGetErrorString(e));
+}
+
+extern "C" int mfi_selftest_waits(unsigned long long* out, void* stream) {
+  if (!out) return mfi::set_last_error(MFI_ERR_ARG, "null pointer");
+  if (reinterpret_cast<uintptr_t>(out) & 7)
+    return mfi::set_last_error(MFI_ERR_ARG, "selftest: out must be 8-byte aligned");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  mfi::selftest_wait_kernel<false><<<1, 64, 0, st>>>(out);
+  mfi::selftest_wait_kernel<true><<<1, 64, 0, st>>>(out + 7);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? MFI_OK : mfi::set_last_error(MFI_ERR_CUDA, cudaGetErrorString(e));
 }
