@@ -273,8 +273,9 @@ int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, in
  * page 0, lengths cut to [0, width * page], sequences with a row range outside
  * [0, T] or above max_q left out (device error 11).
  * The workspace (256-byte aligned) is initialised once by
- * mfi_kv4_attn_init_workspace; each call leaves it ready for the next.  Calls
- * that overlap on the GPU need one each. */
+ * mfi_kv4_attn_init_workspace; each call leaves it ready for the next, one that
+ * gave up a wait (device errors 1 to 3) too.  Calls that overlap on the GPU need
+ * one each. */
 size_t mfi_kv4_attn_workspace_bytes(int n_seq, int Hq, int Hkv, int D, int max_q);
 int mfi_kv4_attn_init_workspace(void* workspace, size_t workspace_bytes, void* stream);
 int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long q_head, const uint8_t* pool,

@@ -520,6 +520,8 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   }
   U = __reduce_add_sync(0xffffffffu, U);
   pieces = __reduce_add_sync(0xffffffffu, pieces);
+  // counters of the kernel for many rows: 8 a CTA and one more
+  if (a.many && warp == 0 && blockIdx.x < kCtas && lane < 9) a.counters[kItemCounter + blockIdx.x * 8 + lane] = 0u;
   if (U == 0) return;
   // One unit a warp at least.  A multiple of the pieces, if that leaves out no more
   // than a quarter of the CTAs: pieces of one length then begin where shares do, and
@@ -903,10 +905,11 @@ cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
   const bool many_pieces = (long long)a.n_seq * a.Hkv >= 32;
   a.few = kFew;
+  a.many = vectors > kFew;
   cudaError_t e;
   if (vectors <= 8) e = many_pieces ? launch_few<E, D, 1, 3>(a, s) : launch_few<E, D, 1, 1>(a, s);
   else e = many_pieces ? launch_few<E, D, 2, 2>(a, s) : launch_few<E, D, 2, 1>(a, s);
-  if (e == cudaSuccess && vectors > kFew)
+  if (e == cudaSuccess && a.many)
     e = launch_kv4_prefill(a, std::is_same<E, __nv_bfloat16>::value, D, s);
   return e;
 }

@@ -16,10 +16,11 @@ struct AttnArgs {
   const int* cu_q;           // (n_seq + 1) or null: max_q rows each
   void* out;                 // (T, Hq, D)
   int* err;
-  unsigned* counters;        // kCounterBytes, zero between calls
+  unsigned* counters;        // kCounterBytes
   float* part;               // few_bytes or many_bytes
   int T, max_q, n_seq, Hq, Hkv, page, num_pages, width;
   int few;                   // sequences of up to this many vectors (rows x heads of a group) are `few`
+  bool many;                 // there may be others: the kernel for many rows follows
   bool q_vec;                // every query row starts on a 16-byte boundary
   int tpp_shift;             // log2 of the tiles of a page, -1 if that is no power of two
   float scale;
@@ -51,12 +52,14 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int i) {
 constexpr int kSms = 148;
 constexpr int kCtas = kSms;                // of the kernel for many rows
 constexpr int kFewCtas = 3 * kSms;         // most of the kernel for few rows
-// Words of the workspace's head, zero between calls.  Few rows: two per CTA for
-// the groups that begin with it, one for the pieces.  Many rows: the next item,
-// the CTAs that are done, one per part and warp.
-constexpr int kItemCounter = 3 * kFewCtas, kDoneCounter = kItemCounter + 1, kPartCounters = kItemCounter + 2;
+// Words of the workspace's head.  Few rows: two per CTA for the groups that begin
+// with it, one for the pieces; every call takes them back to zero.  Many rows: the
+// next item, one per part and warp; a CTA that gives up a wait leaves some of them
+// behind, so the kernel for few rows, which runs first in every call, zeroes them.
+constexpr int kItemCounter = 3 * kFewCtas, kPartCounters = kItemCounter + 1;
+constexpr int kManyCounters = 1 + 8 * kCtas;
 constexpr size_t kCounterBytes = 16384;
-static_assert(kCounterBytes >= (kPartCounters + 8 * kCtas) * sizeof(unsigned), "room for the counters");
+static_assert(kCounterBytes >= (kItemCounter + kManyCounters) * sizeof(unsigned), "room for the counters");
 constexpr int kFew = 64;                   // vectors of a sequence and KV head that are few rows
 
 // Bytes of the sums that parts of a piece or item leave for each other.

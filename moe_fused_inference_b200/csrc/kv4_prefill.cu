@@ -295,9 +295,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (!ok) break;
       }
       if (tc::cta_aborted()) tc::drain_ring(bar.raw_full, kSlots, filled);
-      // the last CTA to see no item left resets the counter for the next call
-      if (lane == 0 && atomicInc(a.counters + kDoneCounter, gridDim.x - 1) == gridDim.x - 1)
-        atomicExch(a.counters + kItemCounter, 0u);
     } else if (warp == 12 || warp == 14) {
       // ---- MMA issue of tile i: the whole warp goes along, so that the descriptors stay in
       // uniform registers, one lane issues.  Descriptors are advanced by adding to

@@ -130,3 +130,23 @@ def test_scores_of_ordinary_size_from_extreme_factors(rows, key, query, scale):
     q = (_randn(11, rows, H * G, D) * 2.0 ** query).bfloat16()
     _compare(_call(q, cache, table, [L], [rows], scale=scale), q, cache, table, [L], [rows], scale)
     assert _errors() == 0
+
+
+# ---- a workspace that an aborted call has left -------------------------------------
+def test_counters_that_an_aborted_call_left_do_not_reach_the_next():
+    """A CTA of the kernel for many rows that gives up a wait does not arrive at its
+    parts' counters.  The next call on the workspace starts them anew: with ones in
+    the words after the few-row kernel's 3 x 444, rows joined from parts are those of
+    a fresh workspace."""
+    L, rows, H, G, D = 3050, 100, 1, 8, 128
+    k, v = _randn(12, 2, L, H, D)
+    cache, table = _cache(k, v)
+    q = _randn(13, rows, H * G, D).bfloat16()
+    want = _call(q, cache, table, [L], [rows])
+    ws = kv4.attention_workspace(1, H * G, cache, max_q=rows)
+    words = ws[:16384].view(torch.int32)
+    for _ in range(2):
+        words[3 * 444:] = 1
+        assert torch.equal(_call(q, cache, table, [L], [rows], workspace=ws), want)
+        assert not words[:3 * 444].any()
+    assert _errors() == 0
