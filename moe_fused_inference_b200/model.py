@@ -229,6 +229,8 @@ class Runner:
             raise RuntimeError("kv must be 'fp8' or 'mxfp4'")
         self.kv4 = None
         if kv == "mxfp4":
+            if max_len <= 0 or page <= 0:
+                raise RuntimeError("max_len and page must be positive")
             per = -(-max_len // page)
             self.page = page
             self.kv4 = [kv4.KV4Cache(batch * per, page, cfg.kv_heads, cfg.head_dim, device=dev)
@@ -244,9 +246,14 @@ class Runner:
         """ids (B, M) at positions base .. base + M - 1 of every sequence;
         returns fp32 logits (B, M, V) (or (B, V) of the last row) and the
         top-k expert ids of every layer.  ``trace`` (a list) receives the
-        residual stream after every layer's attention and MoE block."""
+        residual stream after every layer's attention and MoE block.
+        Positions lie below max_len: an int ``base`` is checked; rows past it
+        under a device ``base`` leave the 4-bit caches alone and are reported
+        through the device error flag (11, 12)."""
         cfg, be, m = self.model.cfg, self.be, self.model
         B, M = ids.shape
+        if not torch.is_tensor(base) and (base < 0 or base + M > self.max_len):
+            raise RuntimeError(f"positions {base} .. {base + M - 1} outside the caches' {self.max_len}")
         T = B * M
         H, Hq, Hkv, D = cfg.hidden, cfg.heads, cfg.kv_heads, cfg.head_dim
         x = dequant_rows(m.embed[0], m.embed[1], H, ids.reshape(-1))
@@ -261,7 +268,11 @@ class Runner:
         if self.kv4 is not None:
             # the rows' places in the pool and the sequences' lengths, for all layers
             pos = positions.view(B, M).long()
-            slots = (self.table.gather(1, pos // self.page).long() * self.page + pos % self.page).view(-1)
+            at = pos.clamp(0, self.max_len - 1) if on_device else pos
+            slots = self.table.gather(1, at // self.page).long() * self.page + at % self.page
+            if on_device:  # a row past max_len: a slot past the pool, a length past the table
+                slots = torch.where(at == pos, slots, self.kv4[0].capacity)
+            slots = slots.view(-1)
             lens = (pos[:, -1] + 1).int()
             if M not in self._kv4_ws:
                 self._kv4_ws[M] = kv4.attention_workspace(B, Hq, self.kv4[0], M)
@@ -423,6 +434,7 @@ class GraphDecoder:
         self.step = torch.zeros((1,), dtype=torch.long, device=dev)
         self.tokens = torch.zeros((B, max_steps), dtype=torch.long, device=dev)
         self.graph = None
+        self.pos = self.done = 0  # the next step's position, steps since start()
 
     def _body(self):
         logits, _ = self.runner.forward(self.ids, self.base, last_only=True)
@@ -433,6 +445,7 @@ class GraphDecoder:
         self.step.add_(1)
 
     def _set(self, last_ids: torch.Tensor, base: int):
+        self.pos, self.done = base, 0
         self.ids.copy_(last_ids)
         self.base.fill_(base)
         self.step.zero_()
@@ -443,9 +456,11 @@ class GraphDecoder:
         (captured once, after an eager warm-up step whose KV row and token
         the replays then write again)."""
         r = self.runner
+        pos = prompt.shape[1] - 1
+        if pos + 1 > r.max_len:
+            raise RuntimeError(f"the prompt's {pos + 1} positions leave the caches' {r.max_len}")
         if prefill:
             r.prefill(prompt, chunk)
-        pos = prompt.shape[1] - 1
         dev = self.ids.device
         if self.graph is None:
             self._set(prompt[:, -1:], pos)
@@ -463,10 +478,14 @@ class GraphDecoder:
 
     def decode(self, steps: int) -> torch.Tensor:
         """`steps` greedy tokens (B, steps) after start()."""
-        if steps > self.max_steps:
+        if self.done + steps > self.max_steps:
             raise RuntimeError(f"at most {self.max_steps} steps")
+        if self.pos + steps > self.runner.max_len:
+            raise RuntimeError(f"positions up to {self.pos + steps - 1} outside the caches' {self.runner.max_len}")
         for _ in range(steps):
             self.graph.replay()
+        self.done += steps
+        self.pos += steps
         return self.tokens[:, :steps]
 
 
