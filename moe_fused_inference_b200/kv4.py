@@ -42,6 +42,14 @@ def _stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+def _device() -> int:
+    """The current device's index, without torch's own look at its initialisation.
+    Launches, the error flag and the kernels' attributes belong to the current
+    device: where the tensors are on another one, an entry point calls itself
+    under ``torch.cuda.device``."""
+    return torch._C._cuda_getDevice()
+
+
 class KV4Cache:
     """A pool of pages.  ``data`` is uint8 (num_pages, kv_heads, page // 16,
     17 * head_dim); token slot ``s`` is token ``s % page`` of page ``s // page``."""
@@ -103,6 +111,9 @@ def kv4_write(cache: KV4Cache, k: torch.Tensor, v: torch.Tensor, slots: torch.Te
         _check(len(shape) == 3 and v.shape == shape and shape[1:] == cache.vector,
                "k and v must be (T, kv_heads, head_dim) of the cache")
         _check_slots(slots, shape[0], cache)
+    if dev.index != _device():
+        with torch.cuda.device(dev):
+            return kv4_write(cache, k, v, slots)
     T = shape[0]
     if T == 0:
         return
@@ -134,6 +145,9 @@ def kv4_read(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.bf
         _check(cache.data.is_cuda, "tensors must be cuda")
         _check(dtype in _DT, "dtype must be bfloat16, float16 or float32")
         _check_slots(slots, slots.shape[0] if slots.dim() else 0, cache)
+    if dev.index != _device():
+        with torch.cuda.device(dev):
+            return kv4_read(cache, slots, dtype)
     T = slots.shape[0]
     out = slots.new_empty((2, T, *cache.vector), dtype=dtype)
     if T:
@@ -155,7 +169,10 @@ def attention_workspace(num_seqs: int, heads: int, cache: KV4Cache, max_q: int =
     lib = _lib.load()
     n = int(lib.mfi_kv4_attn_workspace_bytes(num_seqs, heads, cache.kv_heads, cache.head_dim, max_q))
     _check(n > 0, "num_seqs and max_q must be positive and heads a positive multiple of kv_heads")
-    dev = cache.data.device
+    dev = cache.device
+    if dev.index != _device():
+        with torch.cuda.device(dev):
+            return attention_workspace(num_seqs, heads, cache, max_q)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     _lib.check(lib.mfi_kv4_attn_init_workspace(ws.data_ptr(), n, _stream(ws.device.index)),
                "kv4_attn_init_workspace")
@@ -199,6 +216,9 @@ def kv4_attention(q: torch.Tensor, cache: KV4Cache, page_table: torch.Tensor,
                "heads must be a positive multiple of kv_heads")
         _check(page_table.dtype == torch.int32 and page_table.dim() == 2, "page_table must be int32 (n, pages)")
         _check(False, "kv_lens must be int32 (n,)")
+    if dev.index != _device():
+        with torch.cuda.device(dev):
+            return kv4_attention(q, cache, page_table, kv_lens, cu_q, max_q, scale, out, workspace)
     T, heads, D = shape
     n, width = page_table.shape
     if cu_q is None:

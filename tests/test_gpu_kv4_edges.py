@@ -150,3 +150,40 @@ def test_counters_that_an_aborted_call_left_do_not_reach_the_next():
         assert torch.equal(_call(q, cache, table, [L], [rows], workspace=ws), want)
         assert not words[:3 * 444].any()
     assert _errors() == 0
+
+
+# ---- another device is current -------------------------------------------------------
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    """With another device current every entry point makes its tensors' device
+    current for its launches.  (One device is enough: the query says 1 until the
+    entry point changes it.)"""
+    L, H, G, D = 70, 2, 4, 64
+    k, v = _randn(14, 2, L, H, D)
+    cache, table = _cache(k, v)
+    q = _randn(15, 3, H * G, D).bfloat16()
+    table = torch.from_numpy(table).cuda()
+    lens = torch.tensor([L], dtype=torch.int32, device="cuda")
+    slots = torch.arange(L, device="cuda")
+    want = kv4.kv4_attention(q, cache, table, lens), *kv4.kv4_read(cache, slots)
+    current, entered = [1], []
+
+    class device:
+        def __init__(self, to):
+            self.to = torch.device(to)
+
+        def __enter__(self):
+            self.was, current[0] = current[0], self.to.index
+            entered.append(self.to)
+
+        def __exit__(self, *exc):
+            current[0] = self.was
+
+    monkeypatch.setattr(kv4, "_device", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    other = kv4.KV4Cache.wrap(torch.zeros_like(cache.data))
+    kv4.kv4_write(other, k, v, slots)
+    ws = kv4.attention_workspace(1, H * G, other, max_q=3)
+    got = kv4.kv4_attention(q, other, table, lens, workspace=ws), *kv4.kv4_read(other, slots)
+    assert entered == [cache.device] * 4 and current == [1]
+    assert torch.equal(other.data, cache.data)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
