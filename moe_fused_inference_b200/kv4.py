@@ -166,6 +166,7 @@ def attention_workspace(num_seqs: int, heads: int, cache: KV4Cache, max_q: int =
     of up to ``max_q`` rows each, initialised on the current stream.  Calls
     leave it ready for the next; calls that may run at the same time need one
     each."""
+    _check(cache.data.is_cuda, "the cache must be cuda")
     lib = _lib.load()
     n = int(lib.mfi_kv4_attn_workspace_bytes(num_seqs, heads, cache.kv_heads, cache.head_dim, max_q))
     _check(n > 0, "num_seqs and max_q must be positive and heads a positive multiple of kv_heads")
