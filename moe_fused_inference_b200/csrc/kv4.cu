@@ -247,9 +247,11 @@ Slots make_slots(const int64_t* slots, int T, int Hkv, int page, int num_pages) 
   return s;
 }
 
-// Blocks of a call; 0: more than a grid holds.
+// Blocks of a call; 0: more than a grid holds, or tokens that the last block's count
+// of 31 bits would pass.
 unsigned rw_grid(int T, int Hkv, int D) {
   const int per = kRwThreads / (D / 8);
+  if (T > 0x7FFFFFFF - per) return 0u;
   const long long n = ((long long)T + per - 1) / per * Hkv;
   return n > 0x7FFFFFFFLL ? 0u : unsigned(n);
 }
@@ -279,6 +281,8 @@ extern "C" int mfi_kv4_write(const void* k, long long k_row, long long k_head, c
   if (rc != MFI_OK) return rc;
   if (T == 0) return MFI_OK;
   if (!k || !v || !slots) return mfi::set_last_error(MFI_ERR_ARG, "null pointer");
+  const unsigned grid = mfi::rw_grid(T, Hkv, D);
+  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_write: too many rows");
   mfi::WriteArgs a{};
   a.x[0] = k; a.x[1] = v;
   a.row[0] = k_row; a.row[1] = v_row;
@@ -291,8 +295,6 @@ extern "C" int mfi_kv4_write(const void* k, long long k_row, long long k_head, c
   for (int i = 0; i < 2; ++i)
     vec = vec && !((reinterpret_cast<uintptr_t>(a.x[i]) | uintptr_t(a.row[i] * size) |
                     uintptr_t(a.head[i] * size)) & 15);
-  const unsigned grid = mfi::rw_grid(T, Hkv, D);
-  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_write: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == MFI_F32) mfi::launch_write<float>(a, D, vec, grid, s);
   else if (dtype == MFI_F16) mfi::launch_write<__half>(a, D, vec, grid, s);
@@ -311,12 +313,12 @@ extern "C" int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, 
   if (!k || !v || !slots) return mfi::set_last_error(MFI_ERR_ARG, "null pointer");
   if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: k and v must be 16-byte aligned");
+  const unsigned grid = mfi::rw_grid(T, Hkv, D);
+  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: too many rows");
   mfi::ReadArgs a{};
   a.pool = pool;
   a.y[0] = k; a.y[1] = v;
   a.s = mfi::make_slots(slots, T, Hkv, page, num_pages);
-  const unsigned grid = mfi::rw_grid(T, Hkv, D);
-  if (grid == 0) return mfi::set_last_error(MFI_ERR_ARG, "kv4_read: too many rows");
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == MFI_F32) mfi::launch_read<float>(a, D, grid, s);
   else if (dtype == MFI_F16) mfi::launch_read<__half>(a, D, grid, s);
