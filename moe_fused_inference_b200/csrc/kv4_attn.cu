@@ -956,13 +956,14 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: the workspace must be 256-byte aligned");
   if (workspace_bytes < mfi_kv4_attn_workspace_bytes(n_seq, Hq, Hkv, D, max_q))
     return mfi::set_last_error(MFI_ERR_WORKSPACE, "workspace smaller than the kv4_attn workspace query");
-  // units of work of the kernel for few rows (a tile of a KV head for 8 vectors, at
-  // most) are counted in 31 bits; the items of the other one are fewer than the rows
-  // of `out`
+  // units of work of the kernel for few rows (a tile of a KV head for a set of
+  // vectors) are counted in 31 bits: as many as the table has room for, and sets as
+  // the rows allow.  The items of the other one are fewer than the rows of `out`.
   const double vectors = fmin(double(max_q) * (Hq / Hkv), double(mfi::kv4::kFew));
-  const double units = double(n_seq) * Hkv * (double(width) * page / mfi::kv4::kTile + mfi::kLeast) *
-                       (vectors / 8 + 1);
-  if (units >= 2147483648.0)
+  const double per = vectors <= 8 ? 8 : 16;
+  const double sets = fmin(n_seq * ceil(vectors / per), n_seq + double(T) * (Hq / Hkv) / per);
+  const double tiles = fmax(ceil(double(width) * page / mfi::kv4::kTile), mfi::kLeast);
+  if (sets * Hkv * tiles >= 2147483648.0)
     return mfi::set_last_error(MFI_ERR_ARG, "kv4_attn: more than 2^31 tiles of work in one call");
   mfi::kv4::AttnArgs a{};
   a.q = q; a.q_row = q_row; a.q_head = q_head;

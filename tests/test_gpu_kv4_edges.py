@@ -187,3 +187,34 @@ def test_calls_run_on_their_tensors_device(monkeypatch):
     assert entered == [cache.device] * 4 and current == [1]
     assert torch.equal(other.data, cache.data)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- wide page tables -------------------------------------------------------------------
+@pytest.mark.parametrize("n,heads,rows,width", [(500, 8, 1, 1 << 19), (500, 16, 4, 282144),
+                                                (4096, 32, 4, 24000)])
+def test_many_short_sequences_under_a_wide_table(n, heads, rows, width):
+    """The count of work that a call may have goes by its rows and the table's room,
+    not by more sets of vectors than there are: rows is the largest count of a
+    sequence, the others have one."""
+    H, D = 8, 64
+    k, v = _randn(16, 2, 16, H, D)
+    cache, table = _cache(k, v, page=16)
+    each = [rows] + [1] * (n - 1)
+    q = _randn(17, sum(each), heads, D).bfloat16()
+    wide = torch.from_numpy(table).cuda().expand(n, width)
+    lens = torch.full((n,), 16, dtype=torch.int32, device="cuda")
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(each)]), dtype=torch.int32, device="cuda")
+    got = kv4.kv4_attention(q, cache, wide, lens, cu_q=cu, max_q=rows)
+    assert _errors() == 0
+    some = list(range(rows)) + [len(q) // 2, len(q) - 1]
+    lens_of = [16 - rows + 1 + r for r in range(rows)] + [16, 16]
+    _compare(got[some], q[some], cache, np.repeat(table, len(some), 0), lens_of, [1] * len(some))
+
+
+def test_more_work_than_31_bits_is_refused():
+    cache = kv4.KV4Cache(1, 16, 8, 64)
+    q = torch.zeros((600, 8, 64), device="cuda").bfloat16()
+    wide = torch.zeros((1, 1), dtype=torch.int32, device="cuda").expand(600, 1 << 19)
+    lens = torch.ones(600, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="2\\^31 tiles"):
+        kv4.kv4_attention(q, cache, wide, lens)
