@@ -727,16 +727,10 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) w.o[j][k][0] = w.o[j][k][1] = w.o[j][k][2] = w.o[j][k][3] = 0.0f;
     }
-    // the first run is on its way; more of them, up to F::kStages - 1
-    for (int k = 1; k < F::kStages - 1 && warp + k * F::kWarps < runs; ++k) {
-      fill(g, run, t, t_end, id, (it + k) % F::kStages);
-      t += F::kWarps * run;
-      id = page_of(row, run, t, t_end);
-    }
     for (int left = runs - warp; left > 0; left -= F::kWarps, ++it, t0 += F::kWarps * run) {
-      if (left > (F::kStages - 1) * F::kWarps) {
+      if (left > F::kWarps) {  // the next one; this one is on its way
         __syncwarp();  // the stage's last readers are done
-        fill(g, run, t, t_end, id, (it + F::kStages - 1) % F::kStages);
+        fill(g, run, t, t_end, id, (it + 1) % F::kStages);
         t += F::kWarps * run;
         id = page_of(row, run, t, t_end);
       }
@@ -756,7 +750,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     const bool more_parts = p.next < s_share[warp].hi;
     // the next part's first tiles and rows are on their way during the join; the
     // sums take the place of the stage read last
-    float* sums = reinterpret_cast<float*>(ring + ((it + F::kStages - 1) % F::kStages) * F::kStageBytes);
+    float* sums = reinterpret_cast<float*>(ring + ((it + 1) % F::kStages) * F::kStageBytes);
     if (more_parts) {
       const Part np = s_next[warp];
       const int nrun = run_of(np);
