@@ -887,17 +887,23 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
 }
 
 // 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
-// are then read and decoded half as often), else 8.  One large CTA an SM where few
-// pieces share the SMs (fewer sums to join: one sequence of 131072 tokens 28
-// against 31 us with three), three (two with 16 vectors) small ones where pieces
-// are many and short (one's start and join hide behind the others: 64 sequences
-// of up to 4096 tokens 35 against 49 us).
-// Sequences of more than kFew vectors go to the kernel for many rows, whose tile
-// is 256 vectors.
+// are then read and decoded half as often), else 8.  One large CTA an SM for up to
+// 64 pairs of a sequence and KV head (fewer sums to join), three (two with 16
+// vectors) small ones for more (one's start and join hide behind the others).
+// Large / small, us, 8 query heads a KV head, D 128:
+//   pairs                 4         32        64        128       256
+//   1024 tokens each      10.4/12.1 10.9/12.6 11.0/14.4 11.0/14.2 19.2/18.1
+//   4096                  14.5/16.2 13.7/16.6 17.1/18.1 22.4/25.3 48.6/43.3
+//   103 .. 4096           11.6/13.9 13.7/17.8 18.3/17.4 29.1/21.0 44.6/28.0
+//   two rows each, 4096   19.1/22.9 17.2/22.8 22.9/22.9 31.2/33.8 66.0/53.7
+// (pairs of up to 256 tokens gain 1 us from small CTAs at any count.)
+// Sequences of more than kFew vectors go to the kernel for many rows, which reads a
+// tile for 256 vectors at once.  Few / many, us, 4096 tokens: one sequence 17.2/35.9 with 64 vectors a KV head, 17.1/37.0 with 128; 16
+// sequences 54.2/56.6 with 48, 63.9/57.3 with 64, 74.7/57.6 with 80.
 template <class E, int D>
 cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
-  const bool many_pieces = (long long)a.n_seq * a.Hkv >= 32;
+  const bool many_pieces = (long long)a.n_seq * a.Hkv > 64;
   a.few = kFew;
   a.many = vectors > kFew;
   cudaError_t e;

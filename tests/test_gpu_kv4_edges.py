@@ -7,7 +7,7 @@ import torch
 
 from moe_fused_inference_b200 import _lib, kv4
 from oracle import kv4 as ok
-from tests.test_gpu_kv4 import _call, _compare, _errors, _np
+from tests.test_gpu_kv4 import _call, _compare, _errors, _make, _np
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +218,15 @@ def test_more_work_than_31_bits_is_refused():
     lens = torch.ones(600, dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="2\\^31 tiles"):
         kv4.kv4_attention(q, cache, wide, lens)
+
+
+# ---- both sizes of CTA of the kernel for few rows --------------------------------------------
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("n", [32, 33])  # 64 and 66 pairs of a sequence and KV head
+@pytest.mark.parametrize("most,G", [(1, 8), (3, 5)])
+def test_either_side_of_64_pieces(n, most, G, D):
+    rows = [1 + i % most for i in range(n)]
+    lens = [(97 * i) % 613 for i in range(n)]
+    q, cache, table = _make(40 + n, rows, lens, 2, G, D, 48, torch.bfloat16)
+    _compare(_call(q, cache, table, lens, rows), q, cache, table, lens, rows)
+    assert _errors() == 0
