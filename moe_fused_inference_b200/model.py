@@ -205,6 +205,10 @@ class LibBackend:
             "attn_decode_batched")
         return o
 
+    def workspace_kv4(self, cache, B, M):
+        """What attention_kv4 keeps for B sequences of M rows."""
+        return kv4.attention_workspace(B, self.model.cfg.heads, cache, M)
+
     def write_kv4(self, cache, k, v, slots):
         """Rows k, v (T, Hkv, D) into the 4-bit cache's tokens `slots`."""
         kv4.kv4_write(cache, k, v, slots)
@@ -275,7 +279,7 @@ class Runner:
             slots = slots.view(-1)
             lens = (pos[:, -1] + 1).int()
             if M not in self._kv4_ws:
-                self._kv4_ws[M] = kv4.attention_workspace(B, Hq, self.kv4[0], M)
+                self._kv4_ws[M] = be.workspace_kv4(self.kv4[0], B, M)
         routing = []
         for L, lw in enumerate(m.layers):
             hp = rms_norm(x, lw.in_norm, cfg.eps)
