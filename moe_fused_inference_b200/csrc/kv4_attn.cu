@@ -7,6 +7,7 @@
 // and zeros for a row that sees no token.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 #include <type_traits>
 
@@ -886,11 +887,21 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-// 16 vectors a set where a sequence has more than 8 in all (a KV head's bytes
-// are then read and decoded half as often), else 8.  One large CTA an SM for up to
-// 64 pairs of a sequence and KV head (fewer sums to join), three (two with 16
-// vectors) small ones for more (one's start and join hide behind the others).
-// Large / small, us, 8 query heads a KV head, D 128:
+// Vectors of a set: 8, or 16 (a KV head's bytes are then read and decoded half as
+// often, at 255 registers and some spills) where the call has more than 24 sets of 8.
+// 8 / 16, us, for 256, 1024, 4096, 16384, 65536 tokens:
+//    8 sets (4 pairs, 16 vectors)   8.4/10.1  10.6/13.2  13.1/19.0  16.1/19.9  26.1/25.5
+//   20      (4, 40)                 8.7/10.6  10.9/13.5  12.6/17.1  19.4/20.9  44.3/44.2
+//   32      (4, 64)                 8.8/10.7  10.9/13.6  13.6/17.1  24.8/23.9  68.4/54.4
+//   32      (16, 16)                8.8/10.6  10.9/13.5  13.5/17.3  24.8/23.7  69.4/55.4
+//   64      (32, 16)                8.9/10.7  11.0/13.7  17.0/17.1  39.1/34.6
+int set_vectors(long long n_seq, int Hkv, long long vectors) {
+  return n_seq * Hkv * ((std::min(vectors, (long long)kFew) + 7) / 8) <= 24 || vectors <= 8 ? 8 : 16;
+}
+
+// One large CTA an SM for up to 64 pairs of a sequence and KV head (fewer sums to
+// join), three (two with 16 vectors) small ones for more (one's start and join hide
+// behind the others).  Large / small, us, 8 query heads a KV head, D 128:
 //   pairs                 4         32        64        128       256
 //   1024 tokens each      10.4/12.1 10.9/12.6 11.0/14.4 11.0/14.2 19.2/18.1
 //   4096                  14.5/16.2 13.7/16.6 17.1/18.1 22.4/25.3 48.6/43.3
@@ -898,8 +909,9 @@ cudaError_t launch_few(const AttnArgs& a, cudaStream_t s) {
 //   two rows each, 4096   19.1/22.9 17.2/22.8 22.9/22.9 31.2/33.8 66.0/53.7
 // (pairs of up to 256 tokens gain 1 us from small CTAs at any count.)
 // Sequences of more than kFew vectors go to the kernel for many rows, which reads a
-// tile for 256 vectors at once.  Few / many, us, 4096 tokens: one sequence 17.2/35.9 with 64 vectors a KV head, 17.1/37.0 with 128; 16
-// sequences 54.2/56.6 with 48, 63.9/57.3 with 64, 74.7/57.6 with 80.
+// tile for 256 vectors at once.  Few / many, us, 4096 tokens: one sequence 17.2/35.9
+// with 64 vectors a KV head, 17.1/37.0 with 128; 16 sequences 54.2/56.6 with 48,
+// 63.9/57.3 with 64, 74.7/57.6 with 80.
 template <class E, int D>
 cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   const long long vectors = (long long)a.max_q * (a.Hq / a.Hkv);
@@ -907,8 +919,10 @@ cudaError_t launch(AttnArgs& a, cudaStream_t s) {
   a.few = kFew;
   a.many = vectors > kFew;
   cudaError_t e;
-  if (vectors <= 8) e = many_pieces ? launch_few<E, D, 1, 3>(a, s) : launch_few<E, D, 1, 1>(a, s);
-  else e = many_pieces ? launch_few<E, D, 2, 2>(a, s) : launch_few<E, D, 2, 1>(a, s);
+  if (set_vectors(a.n_seq, a.Hkv, vectors) == 8)
+    e = many_pieces ? launch_few<E, D, 1, 3>(a, s) : launch_few<E, D, 1, 1>(a, s);
+  else
+    e = many_pieces ? launch_few<E, D, 2, 2>(a, s) : launch_few<E, D, 2, 1>(a, s);
   if (e == cudaSuccess && a.many)
     e = launch_kv4_prefill(a, std::is_same<E, __nv_bfloat16>::value, D, s);
   return e;
@@ -960,7 +974,7 @@ extern "C" int mfi_kv4_attn(const void* q, int dtype, long long q_row, long long
   // vectors) are counted in 31 bits: as many as the table has room for, and sets as
   // the rows allow.  The items of the other one are fewer than the rows of `out`.
   const double vectors = fmin(double(max_q) * (Hq / Hkv), double(mfi::kv4::kFew));
-  const double per = vectors <= 8 ? 8 : 16;
+  const double per = mfi::set_vectors(n_seq, Hkv, (long long)max_q * (Hq / Hkv));
   const double sets = fmin(n_seq * ceil(vectors / per), n_seq + double(T) * (Hq / Hkv) / per);
   const double tiles = fmax(ceil(double(width) * page / mfi::kv4::kTile), mfi::kLeast);
   if (sets * Hkv * tiles >= 2147483648.0)

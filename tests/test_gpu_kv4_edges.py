@@ -230,3 +230,12 @@ def test_either_side_of_64_pieces(n, most, G, D):
     q, cache, table = _make(40 + n, rows, lens, 2, G, D, 48, torch.bfloat16)
     _compare(_call(q, cache, table, lens, rows), q, cache, table, lens, rows)
     assert _errors() == 0
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,Hkv", [([3, 1], 2), ([6, 6], 2), ([6, 7], 2), ([8], 3), ([8, 2], 3)])
+def test_either_side_of_24_sets_of_vectors(rows, Hkv, D):
+    lens = [700, 41][:len(rows)]
+    q, cache, table = _make(50, rows, lens, Hkv, 8, D, 32, torch.float16)
+    _compare(_call(q, cache, table, lens, rows), q, cache, table, lens, rows)
+    assert _errors() == 0
