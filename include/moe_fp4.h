@@ -272,6 +272,18 @@ int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, in
  * sequence owns are not written.  Page ids outside [0, num_pages) are read as
  * page 0, lengths cut to [0, width * page], sequences with a row range outside
  * [0, T] or above max_q left out (device error 11).
+ * Scores, sums and outputs are fp32 up to the last rounding; the weights are
+ * rounded to fp16 (2^-12; the sum of the weights is of the unrounded ones).
+ * An output is off by that of the largest value that its row sees in the same
+ * block of 32 channels, and by what leaves fp16: where a sequence has up to 64
+ * vectors (rows times Hq / Hkv) a weight times a value below 2^-38 of the
+ * largest weight times the block's largest scale, and a value 2^29 below that
+ * scale; with more vectors a weight below 2^-31 of the row's largest, a value
+ * 2^34 below its block's largest and a key 2^37 below the largest of its 64
+ * tokens, the largest being those of the tokens that any of the neighbouring
+ * rows sees.  A key or value that is NaN makes NaN of the rows that see it.
+ * A call has at most 2^31 tiles of work: sequences times KV heads times sets of
+ * 8 or 16 vectors times the tiles that the table has room for (MFI_ERR_ARG).
  * The workspace (256-byte aligned) is initialised once by
  * mfi_kv4_attn_init_workspace; each call leaves it ready for the next, one that
  * gave up a wait (device errors 1 to 3) too.  Calls that overlap on the GPU need

@@ -109,10 +109,12 @@ __device__ __forceinline__ uint32_t quantise8(const float (&v)[8], uint8_t& code
 // heads of the same tokens, so that the rows (T, Hkv, D) are met in order: D/8
 // lanes a token, a quad a block of 32 elements, each lane 8 elements of the key
 // and of the value.  The tokens of a tile are neighbours in memory: a warp writes
-// whole 32-byte sectors.  Bound by HBM: 2 bytes read (bf16) and 0.53 written an
-// element.  16384 tokens of 4 heads of 128 written and read back take 28 us, 3.0
-// TB/s; more tokens a thread do not help (2: 27.7 us, 4: 31.6 us) and cost small
-// calls (1021 tokens of 2 heads of 64, fp32: 4.0 us, with 2 tokens a thread 4.8).
+// whole 32-byte sectors.  2 bytes are read (bf16) and 0.53 written an element, but
+// what bounds it is instruction issue: some 500 warp instructions for the 16 elements
+// of a lane, 80% of the issue slots taken.  16384 tokens of 4 heads of 128, slices of
+// a fused projection: 19.9 us, 2.1 TB/s; more tokens a thread do not help (written
+// and read back with 1, 2, 4: 28, 27.7, 31.6 us) and cost small calls (1021 tokens of
+// 2 heads of 64, fp32, with 1, 2: 3.9, 4.8 us).
 constexpr int kRwThreads = 128;
 
 template <class E, int D, bool kVec>
@@ -168,8 +170,8 @@ __device__ __forceinline__ void store8(E* p, uint32_t w, float s) {
 
 // The write's shape, the other way round: 0.53 bytes read and 2 written (bf16) an
 // element.  The slots, then the rows that they name, are two dependent trips to
-// memory.  131072 tokens of 4 heads of 128: 69 us, 4.9 TB/s, four bytes written for
-// one read.
+// memory.  131072 tokens of 4 heads of 128: 69.6 us, 4.9 TB/s, four bytes written for
+// one read; 16384 tokens 9.3 us, 4.6 TB/s.
 template <class E, int D>
 __global__ void __launch_bounds__(kRwThreads) kv4_read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8, nb = D / 32;

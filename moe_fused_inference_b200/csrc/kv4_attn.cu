@@ -37,8 +37,9 @@ using namespace kv4;
 // instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
 // has some 14 us beside it: the launch, three dependent trips (lengths, page table,
 // tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
-// heads: 1 sequence of 131072 tokens 26.9 us, 64 of up to 4096 30.8 us, 1 of 1152
-// 11.6 us, 5 rows over 8191 tokens 17.7 us.
+// heads, the cache not in L2: 1 sequence of 131072 tokens 27.3 us, 64 of up to 4096
+// 30.9 us, 1 of 1152 11.7 us, 5 rows over 8191 tokens 14.4 us.  (The figures of the
+// constants below are of one call over and over, its cache in L2.)
 //
 // Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,
@@ -57,16 +58,18 @@ using namespace kv4;
 //   more below top_b count as zero.  (One top for all blocks dropped channels
 //   2^29 weaker than others.)
 constexpr float kKeyUnit = 0x1p-13f;
-constexpr unsigned kSnap = 32;  // tiles; 16: 131072 tokens 35 instead of 30 us, 64: batches alike
+// Tiles; 16, 32, 64: 64 sequences of up to 4096 tokens 31.6, 29.0, 32.8 us, three rows
+// over 8191 tokens 12.8, 12.8, 15.3, 32 sequences of up to 2003 16.0, 17.2, 21.9.
+constexpr unsigned kSnap = 32;
 constexpr unsigned kLeast = 32;  // units of a piece at least
-constexpr int kOneLevel = 16;   // parts; 8: five rows over 8191 tokens 21.5 instead of 19.8 us, 64: 131072 tokens 28.4 of 27.5
+constexpr int kOneLevel = 16;    // parts; 8: three rows over 8191 tokens 14.7 instead of 12.8 us, 64: alike
 
 template <int D, int kNT, int kPerSm>
 struct Few {
   static constexpr int kWarps = kNT == 1 ? 12 / kPerSm : 8 / kPerSm;
   static constexpr int kChunk = 4;   // tiles of a pipeline stage
-  // one read, the others on their way; stages of 2 tiles 3 or 4 deep: 30.3, 31.0
-  // instead of 27.7 us for 131072 tokens
+  // one read, one on its way; stages of 2 tiles 3 or 4 deep cost 2.6 and 3.3 us more
+  // for 131072 tokens
   static constexpr int kStages = 2;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kVec = 8 * kNT;
@@ -106,11 +109,11 @@ __device__ __forceinline__ int seq_tiles(const Seq& s) {
 }
 
 // Units of work of sequence s's pieces: their tiles, but kLeast at least, for a
-// piece costs its start and joins (some 4 us) whatever its length: counted by their
-// tiles, 20 pieces of 1 tile went to two CTAs one after the other (43 us, now 7),
-// 8 empty ones beside 16 long ones cost 30 us more.  64 of up to 4096 tokens with 16
-// units 31.5 us, 32 30.8, 64 31.1.  Pieces of up to 2 kSnap units are never split, so
-// only whole ones have units without tiles.
+// piece costs its start and joins (some 4 us) whatever its length.  With 1, 16, 32, 64
+// units: 20 pieces of 1 tile 44.3, 7.4, 7.5, 7.5 us (with 1 they go to two CTAs one
+// after the other), 16 sequences of 3000 tokens beside 8 empty ones 84.4, 19.1, 18.0,
+// 18.7, 64 of up to 4096 34.3, 29.7, 29.0, 28.6.  Pieces of up to 2 kSnap units are
+// never split, so only whole ones have units without tiles.
 __device__ __forceinline__ int seq_units(const Seq& s) {
   return s.rows > 0 ? max(int(kLeast), seq_tiles(s)) : 0;
 }
@@ -526,9 +529,10 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
   if (U == 0) return;
   // One unit a warp at least.  A multiple of the pieces, if that leaves out no more
   // than a quarter of the CTAs: pieces of one length then begin where shares do, and
-  // no CTA has two parts to join (five rows over 8191 tokens 17.7 instead of 20.5 us,
-  // over 32768 30 instead of 35; with an eighth 16 sequences of 4096: 20.2 instead of
-  // 17.9; ragged pieces lose up to 0.5 us of 20).
+  // no CTA has two parts to join.  With / without: five rows over 8191 tokens 14.4/15.8
+  // us, over 32768 27.8/31.6, 16 sequences of 4096 17.0/22.2 (with an eighth 22.3), 48
+  // of 1500 18.4/24.0.  Ragged ones lose by it: 16 of 1640 to 4096 21.5/19.6, 48 of 600
+  // to 1500 21.2/20.7, 160 drawn calls 13.36/13.29 in the geometric mean.
   unsigned ctas = min(gridDim.x, (U + F::kWarps - 1) / F::kWarps);
   if (ctas > pieces && ctas % pieces * 4 <= ctas) ctas -= ctas % pieces;
   if (blockIdx.x >= ctas) return;

@@ -17,7 +17,7 @@
 // TMEM: of each tile two S of 64 columns (P in the first half of its S), then O_0
 // and O_1.  Two S a tile keep the softmax supplied while the tensor cores are at
 // the step before; with one S of 128 tokens a tile its warps and the tensor cores
-// waited for each other (16384 rows: 1.98 ms), although a product of 64 columns
+// waited for each other (16384 rows: 1.98 ms, now 1.72), although a product of 64 columns
 // takes 50 clocks and one of 128 takes 65 (both operands from shared memory).
 //
 // The operands are fp16: a query row times a power of two that brings its
@@ -27,7 +27,7 @@
 // above the block's largest code, and again when a code passes it, so exact unless
 // 2^-34 below the largest so far of the same block.
 // P is rounded to fp16 after a factor 2^6; the maximum that it refers to moves
-// when it is passed by 2^9 (2^7: 1.76 instead of 1.71 ms), so P stays below 2^15;
+// when it is passed by 2^9 (2^7: 3% more for a prompt of 16384 tokens), so P stays below 2^15;
 // weights below 2^-20 of the reference lose bits, those below 2^-31 vanish.  l and O
 // are fp32.
 #include <cuda_fp16.h>
@@ -73,7 +73,9 @@ struct Item {
 
 // Parts of an item: no more than the CTAs allow, of at least kMinSteps steps (a
 // part starts in about 5 us, 8 steps take about as long), at most kMaxParts (they
-// are joined by one CTA's warps).
+// are joined by one CTA's warps).  kMinSteps 4, 8, 16: 100 rows over 2048 tokens, 4
+// KV heads of 8, 40.0, 40.1, 50.4 us, over 1024 33.8, 32.6, 32.8; kMaxParts 6, 12,
+// 18: 100 rows over 8192, one KV head, 51.5, 47.4, 53.2, 40 over 32768 114, 81, 75.
 constexpr int kMinSteps = 8, kMaxParts = 12;
 
 // An operand of R rows: halves of 64 elements, each R rows of 128 bytes in the
