@@ -788,6 +788,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     __syncthreads();
     constexpr int kPer = D / 4, kRows = 32 / kPer;
     const int sub = lane / kPer, d0 = (lane % kPer) * 4;
+    unsigned again = 0;  // this warp's vectors that are taken once more
     // vectors warp * kRows + sub, .. of the sums that the first `busy` warps left
     auto join_warps = [&](int busy, float* to) {
       for (int v = warp * kRows + sub; v < F::kVec; v += F::kWarps * kRows) {
@@ -818,8 +819,10 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
         if (to) {
           *reinterpret_cast<float4*>(to + v * F::kAcc + d0) = make_float4(o[0], o[1], o[2], o[3]);
           if (d0 == 0) *reinterpret_cast<float2*>(to + v * F::kAcc + D) = make_float2(m, l);
-        } else if (p.v0 + v < nv) {
-          store_vector<E>(a, s, p.g, G, p.v0 + v, d0, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+        } else {
+          const bool live = p.v0 + v < nv, redo = out_of_range(m);
+          if (live && !redo) store_vector<E>(a, s, p.g, G, p.v0 + v, d0, o, l == 0.0f ? 0.0f : 1.0f / l, D);
+          again |= __reduce_or_sync(0xffffffffu, live && redo ? 1u << v : 0u);
         }
       }
     };
@@ -870,6 +873,12 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
       stride = group;
       count = (parts + group - 1) / group;
       counter = a.counters + 2 * kFewCtas + c_first;
+    }
+    for (; again; again &= again - 1) {
+      const int v = s_now[warp].v0 + __ffs(again) - 1;
+      const Seq& x = s_now[warp].s;
+      attend_exactly<E, D>(a, s_now[warp].seq, x.row0 + v / G, s_now[warp].g * G + v % G,
+                           x.len - x.rows + v / G + 1);
     }
     if (!more_parts) break;
     // the sums are read: their memory, written by ordinary stores, takes tiles

@@ -110,6 +110,72 @@ __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
+// Whether a vector whose running maximum is m has left what the tensor cores' form
+// holds, and is taken by attend_exactly instead: s qs - m in one rounding keeps what m
+// has lost in its own, from 2^24 on more than a weight's exponent holds.
+__device__ __forceinline__ bool out_of_range(float m) { return fabsf(m) > 0x1p20f && m != -INFINITY; }
+
+// One vector (row `row`, head h, over the first `see` tokens of sequence seq) by one
+// warp on the CUDA cores, in fp32 throughout: for the few vectors whose weights leave
+// fp16.  Some 60 instructions a token.
+template <class E, int D>
+__device__ __forceinline__ void attend_exactly(const AttnArgs& a, int seq, int row, int h, int see) {
+  constexpr int nb = D / 32, kE = D / 32;  // channels of a lane
+  const int lane = threadIdx.x & 31, el = kE * lane, b = el / 32, i = el % 32;
+  const int key_at = ((i / 8) * nb + b) * 4 + (i % 8) / 2, value_at = ((i / 4) * nb + b) * 2 + (i % 4) / 2;
+  const int tpp = a.page / kTile, g = h / (a.Hq / a.Hkv);
+  const E* src = static_cast<const E*>(a.q) + (long long)row * a.q_row + h * a.q_head + el;
+  float q[kE], o[kE], m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    q[e] = float(src[e]) * a.scale * 1.44269504088896341f;
+    o[e] = 0.0f;
+  }
+  // elements of the lane at p, times s: a nibble's low bits are an exponent and one bit
+  // of a significand, subnormal at 0
+  auto elements = [](const uint8_t* p, float s, float (&x)[kE]) {
+    const uint32_t w = kE == 4 ? *reinterpret_cast<const uint16_t*>(p) : *p;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) {
+      const float y = __uint_as_float(((w >> (4 * e)) & 7u) << 22) * 0x1p126f;
+      x[e] = ((w >> (4 * e)) & 8u ? -y : y) * s;
+    }
+  };
+#pragma unroll 1
+  for (int t = 0; t < see; ++t) {
+    const int tile = t / kTile, r = t % kTile;
+    int id = __ldg(a.table + seq * a.table_ld + tile / tpp);
+    if (unsigned(id) >= unsigned(a.num_pages)) id = 0;  // reported where its tiles are brought in
+    const uint8_t* p = a.pool + ((uint64_t(unsigned(id)) * unsigned(a.Hkv) + unsigned(g)) * unsigned(tpp) +
+                                 unsigned(tile % tpp)) * tile_bytes(D);
+    const uint8_t* c = p + 16 * D + r * nb + b;
+    float k[kE], v[kE], x = 0.0f;
+    elements(p + r * (D / 2) + key_at, code_value(c[0]), k);
+    elements(p + 8 * D + r * (D / 2) + value_at, code_value(c[D / 2]), v);
+#pragma unroll
+    for (int e = 0; e < kE; ++e) x = fmaf(q[e], k[e], x);
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
+    if (x > m) {
+      const float f = ex2(m - x);
+      m = x;
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < kE; ++e) o[e] *= f;
+    }
+    const float w = ex2(x - (m == -INFINITY ? 0.0f : m));
+    l += w;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] = fmaf(w, v[e], o[e]);
+  }
+  __align__(8) E y[kE];
+#pragma unroll
+  for (int e = 0; e < kE; ++e) y[e] = E(l == 0.0f ? 0.0f : o[e] / l);
+  E* dst = static_cast<E*>(a.out) + ((long long)row * a.Hq + h) * D + el;
+  if (kE == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(y);
+  else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(y);
+}
+
 }  // namespace kv4
 
 // Launch the kernel for many rows on the sequences of more than a.few vectors.

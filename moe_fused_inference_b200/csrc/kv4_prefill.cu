@@ -683,6 +683,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const float nan = __uint_as_float(0x7FC00000u);
       E* out = static_cast<E*>(a.out) +
                ((long long)(it.row0 + v / G) * a.Hq + it.g * G + v % G) * D;
+      // vectors whose scores are huge (rare): once more, by the warp
+      bool redo = v < nv && out_of_range(m);
+      auto again = [&] {
+        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
+          const int x = __shfl_sync(0xffffffffu, v, __ffs(left) - 1);
+          attend_exactly<E, D>(a, it.seq, it.row0 + x / G, it.g * G + x % G, it.len - it.rows + x / G + 1);
+        }
+      };
       // a part leaves [D + 2][256 vectors] sums
       float* sums = a.part + size_t(it.index) * (256 * (D + 2)) + i * kRows + r;
       const float inv = it.parts > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
@@ -698,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (it.parts > 1) {
 #pragma unroll
           for (int k = 0; k < 32; ++k) __stcg(sums + (32 * x + k) * 256, __uint_as_float(o[k]));
-        } else if (v < nv) {
+        } else if (v < nv && !redo) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             __align__(16) E y[8];
@@ -708,8 +716,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           }
         }
       }
-      if (it.parts > 1) {
-        __stcg(sums + D * 256, m);
+      if (it.parts == 1) {
+        again();
+      } else {
+        __stcg(sums + D * 256, redo ? INFINITY : m);
         __stcg(sums + (D + 1) * 256, l);
         __threadfence();
         __syncwarp();
@@ -735,6 +745,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             if (k < it.parts) sum = fmaf(w[k], at(k, D + 1), sum);
           }
           const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+          redo = v < nv && out_of_range(top);
 #pragma unroll 1
           for (int c = 0; c < D; c += 8) {
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -744,13 +755,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
 #pragma unroll
                 for (int e = 0; e < 8; ++e) x[e] = fmaf(w[k], at(k, c + e), x[e]);
               }
-            if (v < nv) {
+            if (v < nv && !redo) {
               __align__(16) E y[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) y[e] = E(x[e] * scale);
               *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(y);
             }
           }
+          again();
         }
       }
       tc::tc_fence_before();

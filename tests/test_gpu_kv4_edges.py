@@ -239,3 +239,32 @@ def test_either_side_of_24_sets_of_vectors(rows, Hkv, D):
     q, cache, table = _make(50, rows, lens, Hkv, 8, D, 32, torch.float16)
     _compare(_call(q, cache, table, lens, rows), q, cache, table, lens, rows)
     assert _errors() == 0
+
+
+# ---- huge scores -----------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 3, 8, 40, 140])
+@pytest.mark.parametrize("power", [6, 9, 12, 16, 30, 50])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_huge_scores_leave_one_weight(rows, power, sign):
+    """Scores of 2^(2 power) and more, all positive or all negative: the tokens of the
+    largest one alone (the others are an eighth of it away at least)."""
+    L, H, G, D = 300, 2, 4, 64
+    g = np.random.default_rng(power)
+    e = g.permutation(L) % 24
+    score = np.exp2(e // 3 + power) * np.array([1.0, 1.25, 1.5])[e % 3]    # exact in 4 bits, two blocks
+    k = torch.zeros((L, H, D), device="cuda")
+    k[:, :, 0] = sign * torch.from_numpy(np.exp2(e // 3 + power)).float().cuda()[:, None]
+    k[:, :, 32] = sign * torch.from_numpy(score - np.exp2(e // 3 + power)).float().cuda()[:, None]
+    v = _randn(20, L, H, D)
+    cache, table = _cache(k, v)
+    q = torch.zeros((rows, H * G, D), device="cuda")
+    q[:, :, 0] = q[:, :, 32] = 2.0 ** power
+    got = _np(_call(q.bfloat16(), cache, table, [L], [rows], scale=1.0))
+    _, held = kv4.kv4_read(cache, torch.arange(L, device="cuda"), dtype=torch.float32)
+    held = _np(held)
+    for r in range(rows):
+        s = sign * score[:L - rows + r + 1]
+        want = held[:len(s)][s == s.max()].mean(0)          # (H, D): equal scores share
+        tol = 2.0 ** -8 * np.abs(want) + 2.0 ** -11 * np.abs(held).max()
+        assert (np.abs(got[r].reshape(H, G, D) - want[:, None]) <= tol[:, None]).all()
+    assert _errors() == 0
