@@ -227,6 +227,22 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
           w.o[j][k][3] *= c;
         }
     }
+    // Tokens that some vectors do not see yet, 2^24 stronger than others of their block
+    // (rare): these vectors would lose what they see.  They are asked for once more.
+    if (end > q.all) {
+      bool far = false;
+#pragma unroll
+      for (int b = 0; b < nb; ++b) {
+        const uint32_t then = half_of(w.top[b % 2], b / 2), now = half_of(b % 2 ? t1 : t0, b / 2);
+        const uint32_t x = (ca >> (8 * b)) & 0xFFu, y = (cb >> (8 * b)) & 0xFFu;
+        const uint32_t lo = min(then > 29u ? then - 1 : 255u, min(x > 28u ? x : 255u, y > 28u ? y : 255u));
+        far |= now > max(then, lo + 24u);
+      }
+      if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int j = 0; j < kNT; ++j) w.m[j][0] = w.m[j][1] = INFINITY;
+      }
+    }
     w.top[0] = t0;
     w.top[1] = t1;
   }

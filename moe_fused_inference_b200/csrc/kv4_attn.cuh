@@ -112,12 +112,14 @@ __device__ __forceinline__ float2 two_floats<__nv_bfloat16>(uint32_t w) {
 
 // Whether a vector whose running maximum is m has left what the tensor cores' form
 // holds, and is taken by attend_exactly instead: s qs - m in one rounding keeps what m
-// has lost in its own, from 2^24 on more than a weight's exponent holds.
+// has lost in its own, from 2^24 on more than a weight's exponent holds.  Infinity: a
+// part of the vector asks for it (a NaN or an infinity in the scores does not).
 __device__ __forceinline__ bool out_of_range(float m) { return fabsf(m) > 0x1p20f && m != -INFINITY; }
 
 // One vector (row `row`, head h, over the first `see` tokens of sequence seq) by one
-// warp on the CUDA cores, in fp32 throughout: for the few vectors whose weights leave
-// fp16.  Some 60 instructions a token.
+// warp on the CUDA cores, in fp32 throughout: for the few vectors whose operands or
+// weights leave fp16 (out_of_range, values far stronger than those that the row sees).
+// Some 60 instructions a token.
 template <class E, int D>
 __device__ __forceinline__ void attend_exactly(const AttnArgs& a, int seq, int row, int h, int see) {
   constexpr int nb = D / 32, kE = D / 32;  // channels of a lane

@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ Bars bar;
   __shared__ Item s_item[2];
-  __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN
+  __shared__ int s_nan[2][4];     // of an item: first token whose value block is NaN,
+  __shared__ int s_far[2];        // values far stronger than others that some rows see without them
   // of a step: the key code that its operands refer to, whether there are NaN values
   // (bit 0) and whether the values' codes are others than the step's before (bit 1),
   // these, of blocks 0 and 2 (halves), 1 and 3.  Its writer is at most 2 kSlots steps
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (lane == 0) {
           s_item[slot] = it;
           for (int b = 0; b < 4; ++b) s_nan[slot][b] = 0x7FFFFFFF;
+          s_far[slot] = 0;
           tc::mbar_arrive(&bar.item_full[slot]);
         }
         if (!it.valid) break;
@@ -375,6 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         if (!wait(&bar.item_full[slot], n >> 1, 1)) break;
         const int valid = s_item[slot].valid, steps = s_item[slot].steps;
         const int pos = s_item[slot].step0 * kTok, len = s_item[slot].len - pos;  // of the part
+        const int all = len - s_item[slot].rows + s_item[slot].v0 / G + 1;  // tokens that all rows see
         uint32_t v02 = 28u << 16 | 28u, v13 = v02;  // blocks of zeros
         for (int j = 0; valid && j < steps; ++j, ++step) {
           ok = wait_slot(bar.raw_full, step, 1);
@@ -429,6 +432,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             const uint32_t n02 = passed(e & 0xFFFFu, v02 & 0xFFFFu) | passed(e >> 16, v02 >> 16) << 16;
             const uint32_t n13 = passed(o & 0xFFFFu, v13 & 0xFFFFu) | passed(o >> 16, v13 >> 16) << 16;
             moved = j > 0 && (n02 != v02 || n13 != v13) ? 2u : 0u;
+            if ((j + 1) * kTok > all) {
+              bool far = false;
+#pragma unroll
+              for (int b = 0; b < nb; ++b) {
+                const uint32_t then = half_of(b % 2 ? v13 : v02, b / 2), now = half_of(b % 2 ? n13 : n02, b / 2);
+                uint32_t lo = then > 28u ? then - kVSlack : 255u;
+#pragma unroll
+                for (int x = 0; x < kTok / 32; ++x) {
+                  const uint32_t c = (wv[x] >> (8 * b)) & 0xFFu;
+                  if (c > 28u) lo = min(lo, c);
+                }
+                far |= now > then && int(now) - int(__reduce_min_sync(0xffffffffu, lo)) > 28 + int(kVSlack);
+              }
+              if (far && lane == 0) s_far[slot] = 1;
+            }
             v02 = n02;
             v13 = n13;
           }
@@ -585,7 +603,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const int pos = it.step0 * kTok;
       const int lim = v < nv ? it.len - it.rows + v / G + 1 - pos : 0;
       const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1 - pos;
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY, l = 0.0f, most = 0.0f;
       for (int j = 0; j < it.steps; ++j, ++step) {
         const uint32_t buf = step & 1u, tb = ts + buf * 64;
         ok = wait(&bar.s_full[i][buf], step >> 1, 3);
@@ -596,6 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         // not zero: a masked score of -inf has to stay -inf (S is below 2^38: what the
         // bound adds to a score is below 2^-84)
         const float sc = fmaxf(qs * __uint_as_float((127 + kref - 127 - kUp - 13) << 23), 1e-37f);
+        most = fmaxf(most, sc);
         uint32_t s[kTok];
 #pragma unroll
         for (int c = 0; c < kTok / 32; ++c)
@@ -683,8 +702,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const float nan = __uint_as_float(0x7FC00000u);
       E* out = static_cast<E*>(a.out) +
                ((long long)(it.row0 + v / G) * a.Hq + it.g * G + v % G) * D;
-      // vectors whose scores are huge (rare): once more, by the warp
-      bool redo = v < nv && out_of_range(m);
+      // Vectors that some values are lost to, whose scores are huge, or whose keys of a
+      // step are so strong that what others lose in fp16 would count (rare: S, of which
+      // an operand below its range takes 2^-3 at most, is scaled by sc): once more, by
+      // the warp.
+      bool redo = v < nv && (s_far[n & 1u] != 0 || out_of_range(m) || most > 0x1p-12f);
       auto again = [&] {
         for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
           const int x = __shfl_sync(0xffffffffu, v, __ffs(left) - 1);

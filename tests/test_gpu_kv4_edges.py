@@ -268,3 +268,26 @@ def test_huge_scores_leave_one_weight(rows, power, sign):
         tol = 2.0 ** -8 * np.abs(want) + 2.0 ** -11 * np.abs(held).max()
         assert (np.abs(got[r].reshape(H, G, D) - want[:, None]) <= tol[:, None]).all()
     assert _errors() == 0
+
+
+# ---- strong tokens that a row does not see --------------------------------------------------
+@pytest.mark.parametrize("rows", [2, 5, 8, 33, 140])
+@pytest.mark.parametrize("back", [1, 2, 30])
+@pytest.mark.parametrize("what", ["values", "keys", "both"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_rows_do_not_depend_on_tokens_after_theirs(rows, back, what, D):
+    """A token 2^100 stronger than the others takes nothing from the rows before it;
+    the rows that see it stay within the bound of what they see."""
+    L, H, G = 300, 2, 4
+    k, v = _randn(18, 2, L, H, D)
+    at = L - min(back, rows - 1)
+    if what != "keys":
+        v[at] *= 2.0 ** 100
+        v[at + 1:at + 2, 0] *= 2.0 ** 50
+    if what != "values":
+        k[at] *= 2.0 ** 60
+    cache, table = _cache(k, v)
+    q = _randn(19, rows, H * G, D).bfloat16()
+    got = _call(q, cache, table, [L], [rows])
+    _compare_blocks(got, q, cache, table, L)
+    assert got.isfinite().all() and _errors() == 0
