@@ -71,12 +71,13 @@ int mfi_device_error(int clear);
 int mfi_selftest_numerics(unsigned long long* out, void* stream);
 
 /* Self-check of the bounded waits that the kernels' roles use.  Asynchronous on
- * `stream`, about 4 s; out (device, 14 words, 8-byte aligned) receives, for the
+ * `stream`, about 8 s; out (device, 16 words, 8-byte aligned) receives, for the
  * wait of one thread and then for that of a warp, seven words: result (1: the
  * barrier completed) and nanoseconds of a wait on a barrier that completes, of
  * one that never does (0 after some 2 s), of one that never does while another role
  * of its CTA fails after 1 ms (0 soon after), and the error code that the second
- * reported (3). */
+ * reported (3); then result and nanoseconds of a warp's wait of 3 s while another
+ * role has announced work (1). */
 int mfi_selftest_waits(unsigned long long* out, void* stream);
 
 /* ------------------------------------------------------------------------

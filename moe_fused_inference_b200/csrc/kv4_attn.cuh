@@ -143,32 +143,46 @@ __device__ __forceinline__ void attend_exactly(const AttnArgs& a, int seq, int r
       x[e] = ((w >> (4 * e)) & 8u ? -y : y) * s;
     }
   };
+  constexpr int kRun = 4;  // tokens on their way at once, of one tile
 #pragma unroll 1
-  for (int t = 0; t < see; ++t) {
-    const int tile = t / kTile, r = t % kTile;
+  for (int t = 0; t < see; t += kRun) {
+    const int tile = t / kTile;
     int id = __ldg(a.table + seq * a.table_ld + tile / tpp);
     if (unsigned(id) >= unsigned(a.num_pages)) id = 0;  // reported where its tiles are brought in
     const uint8_t* p = a.pool + ((uint64_t(unsigned(id)) * unsigned(a.Hkv) + unsigned(g)) * unsigned(tpp) +
                                  unsigned(tile % tpp)) * tile_bytes(D);
-    const uint8_t* c = p + 16 * D + r * nb + b;
-    float k[kE], v[kE], x = 0.0f;
-    elements(p + r * (D / 2) + key_at, code_value(c[0]), k);
-    elements(p + 8 * D + r * (D / 2) + value_at, code_value(c[D / 2]), v);
+    float v[kRun][kE], x[kRun], top = m;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) x = fmaf(q[e], k[e], x);
+    for (int n = 0; n < kRun; ++n) {
+      const int r = (t + n) % kTile;
+      const uint8_t* c = p + 16 * D + r * nb + b;
+      float k[kE];
+      elements(p + r * (D / 2) + key_at, code_value(c[0]), k);
+      elements(p + 8 * D + r * (D / 2) + value_at, code_value(c[D / 2]), v[n]);
+      x[n] = 0.0f;
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) x += __shfl_xor_sync(0xffffffffu, x, off);
-    if (x > m) {
-      const float f = ex2(m - x);
-      m = x;
-      l *= f;
-#pragma unroll
-      for (int e = 0; e < kE; ++e) o[e] *= f;
+      for (int e = 0; e < kE; ++e) x[n] = fmaf(q[e], k[e], x[n]);
     }
-    const float w = ex2(x - (m == -INFINITY ? 0.0f : m));
-    l += w;
 #pragma unroll
-    for (int e = 0; e < kE; ++e) o[e] = fmaf(w, v[e], o[e]);
+    for (int n = 0; n < kRun; ++n) {
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) x[n] += __shfl_xor_sync(0xffffffffu, x[n], off);
+      if (t + n < see) top = fmaxf(top, x[n]);
+    }
+    const float f = top == -INFINITY ? 1.0f : ex2(m - top);
+    m = top;
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) o[e] *= f;
+#pragma unroll
+    for (int n = 0; n < kRun; ++n) {
+      if (t + n < see) {  // what a row does not see is not multiplied by zero: it may be NaN
+        const float w = ex2(x[n] - (m == -INFINITY ? 0.0f : m));
+        l += w;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) o[e] = fmaf(w, v[n][e], o[e]);
+      }
+    }
   }
   __align__(8) E y[kE];
 #pragma unroll

@@ -708,10 +708,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       // the warp.
       bool redo = v < nv && (s_far[n & 1u] != 0 || out_of_range(m) || most > 0x1p-12f);
       auto again = [&] {
-        for (unsigned left = __ballot_sync(0xffffffffu, redo); left; left &= left - 1) {
+        unsigned left = __ballot_sync(0xffffffffu, redo);
+        if (left == 0) return;
+        if (lane == 0) tc::cta_busy(1);
+        for (; left; left &= left - 1) {
           const int x = __shfl_sync(0xffffffffu, v, __ffs(left) - 1);
           attend_exactly<E, D>(a, it.seq, it.row0 + x / G, it.g * G + x % G, it.len - it.rows + x / G + 1);
         }
+        if (lane == 0) tc::cta_busy(-1);
       };
       // a part leaves [D + 2][256 vectors] sums
       float* sums = a.part + size_t(it.index) * (256 * (D + 2)) + i * kRows + r;

@@ -68,7 +68,9 @@ __global__ void __launch_bounds__(256) selftest_kernel(unsigned long long* out) 
 // The bounded waits of a CTA's roles (tc_ptx.cuh), one warp waiting: on a barrier that
 // completes, on one that never does, and on one that never does while the other
 // warp reports a failure after 1 ms.  out[2 i], out[2 i + 1]: what the i-th wait
-// returned, and its ns; out[6]: the code that the second one reported.
+// returned, and its ns; out[6]: the code that the second one reported.  The wait of a
+// warp once more, on a barrier that the other warp completes after 3 s of work that it
+// has announced (cta_busy): out[7], out[8].
 template <bool kWarp>
 __global__ void __launch_bounds__(64) selftest_wait_kernel(unsigned long long* out) {
   __shared__ uint64_t done, never;
@@ -104,6 +106,25 @@ __global__ void __launch_bounds__(64) selftest_wait_kernel(unsigned long long* o
     __syncthreads();
   }
   if (threadIdx.x == 0) out[6] = (unsigned long long)err[0];
+  if (!kWarp) return;
+  if (threadIdx.x == 0) {
+    tc::cta_abort_init();
+    tc::cta_busy(1);
+  }
+  __syncthreads();
+  const uint64_t t0 = tc::globaltimer_ns();
+  if (threadIdx.x == 32) {
+    while (tc::globaltimer_ns() - t0 < 3000000000ull) __nanosleep(1000);
+    tc::mbar_arrive(&never);
+    tc::cta_busy(-1);
+  }
+  if (warp == 0) {
+    const bool ok = tc::mbar_wait_warp(&never, 0, &err[0], 3);
+    if (lane == 0) {
+      out[7] = ok;
+      out[8] = tc::globaltimer_ns() - t0;
+    }
+  }
 }
 
 __global__ void selftest_init_kernel(unsigned long long* out) {

@@ -58,10 +58,13 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // waits with mbar_wait clears the word from thread 0 (cta_abort_init) before
 // its first __syncthreads.
 __device__ __forceinline__ volatile int* cta_abort_word() {
-  __shared__ int word;
-  return &word;
+  __shared__ int words[2];  // and the count of warps at work that mbar_wait_warp waits out
+  return words;
 }
-__device__ __forceinline__ void cta_abort_init() { *cta_abort_word() = 0; }
+__device__ __forceinline__ void cta_abort_init() { cta_abort_word()[0] = cta_abort_word()[1] = 0; }
+// A warp's work that may take longer than a wait's limit, begun and done: the limit of
+// mbar_wait_warp starts anew while there is any.
+__device__ __forceinline__ void cta_busy(int change) { atomicAdd(const_cast<int*>(&cta_abort_word()[1]), change); }
 __device__ __forceinline__ bool cta_aborted() { return *cta_abort_word() != 0; }
 // Record `code` in the device error flag (first error wins) and stop this CTA.
 __device__ __forceinline__ void cta_fail(int* err, int code) {
@@ -98,7 +101,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
 // room in the instruction cache, from the other roles of the CTA), and no divergence in
 // the compiler's eyes (what the warp keeps in uniform registers stays there).  Each
 // poll looks at the abort word.  The limit is a count: a poll that fails has slept in
-// hardware for 4.0 us, so kWaitPolls are 2.1 s (mfi_selftest_waits measures it).  With
+// hardware for 4.0 us, so kWaitPolls are 2.1 s (mfi_selftest_waits measures it); it
+// starts anew while a warp has announced longer work (cta_busy).  With
 // the clock read in the block a prompt's attention takes 1.74 ms instead of 1.72, with
 // mbar_wait 1.89.
 constexpr uint32_t kWaitPolls = 1u << 19;
@@ -109,6 +113,7 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, i
       "POLL:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
       " ld.volatile.shared.u32 w, [%3];\n setp.ne.u32 q, w, 0;\n @q bra DONE;\n"
       " add.u32 n, n, 1;\n setp.lt.u32 q, n, %4;\n @q bra POLL;\n"
+      " ld.volatile.shared.u32 w, [%3+4];\n mov.u32 n, 0;\n setp.ne.u32 q, w, 0;\n @q bra POLL;\n"
       "DONE:\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
       : "r"(smem_u32(bar)), "r"(parity), "r"(smem_u32(const_cast<const int*>(cta_abort_word()))),
