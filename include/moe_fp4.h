@@ -279,10 +279,11 @@ int mfi_kv4_read(const uint8_t* pool, const int64_t* slots, void* k, void* v, in
  * block of 32 channels, and by what leaves fp16: where a sequence has up to 64
  * vectors (rows times Hq / Hkv) a weight times a value below 2^-38 of the
  * largest weight times the block's largest scale, and a value 2^29 below that
- * scale; with more vectors a weight below 2^-31 of the row's largest, a value
- * 2^34 below its block's largest and a key 2^37 below the largest of its 64
- * tokens, the largest being those of the tokens that any of the neighbouring
- * rows sees.  A key or value that is NaN makes NaN of the rows that see it.
+ * scale; with more vectors a weight below 2^-31 of the row's largest and a value
+ * 2^34 below its block's largest.  A row does not depend on tokens that it does
+ * not see: rows whose neighbours see far stronger ones, and rows of huge scores
+ * or keys, are computed once more in fp32, some hundred times slower.  A key
+ * or value that is NaN makes NaN of the rows that see it.
  * A call has at most 2^31 tiles of work: sequences times KV heads times sets of
  * 8 or 16 vectors times the tiles that the table has room for (MFI_ERR_ARG).
  * The workspace (256-byte aligned) is initialised once by

@@ -37,9 +37,10 @@ using namespace kv4;
 // instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
 // has some 14 us beside it: the launch, three dependent trips (lengths, page table,
 // tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
-// heads, the cache not in L2: 1 sequence of 131072 tokens 27.3 us, 64 of up to 4096
-// 30.9 us, 1 of 1152 11.7 us, 5 rows over 8191 tokens 14.4 us.  (The figures of the
-// constants below are of one call over and over, its cache in L2.)
+// heads, the cache not in L2: 1 sequence of 131072 tokens 27.9 us, 64 of up to 4096
+// 31.2 us, 1 of 1152 12.1 us, 5 rows over 8191 tokens 14.7 us.  (The figures of the
+// constants below are of one call over and over, its cache in L2, without the check of
+// the maximum at the end, which costs up to 2%.)
 //
 // Per tile and warp, with mma.m16n8k16 (fp16 operands, fp32 sums):
 //   S^T (16 tokens x 8 vectors) = K_b . Q_b^T for each block b of 32 elements,

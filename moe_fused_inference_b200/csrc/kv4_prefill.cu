@@ -17,7 +17,7 @@
 // TMEM: of each tile two S of 64 columns (P in the first half of its S), then O_0
 // and O_1.  Two S a tile keep the softmax supplied while the tensor cores are at
 // the step before; with one S of 128 tokens a tile its warps and the tensor cores
-// waited for each other (16384 rows: 1.98 ms, now 1.72), although a product of 64 columns
+// waited for each other (16384 rows: 1.98 ms, now 1.66), although a product of 64 columns
 // takes 50 clocks and one of 128 takes 65 (both operands from shared memory).
 //
 // The operands are fp16: a query row times a power of two that brings its
@@ -25,7 +25,8 @@
 // keys' ref is the largest code of the 64 tokens: exact unless 2^-37 below it.  The
 // values have one for each block of 32 channels, which O refers to as well: set 3
 // above the block's largest code, and again when a code passes it, so exact unless
-// 2^-34 below the largest so far of the same block.
+// 2^-34 below the largest so far of the same block.  The few rows that lose by it (they
+// do not see the strong values, or their scores are huge) are taken once more in fp32.
 // P is rounded to fp16 after a factor 2^6; the maximum that it refers to moves
 // when it is passed by 2^9 (2^7: 3% more for a prompt of 16384 tokens), so P stays below 2^15;
 // weights below 2^-20 of the reference lose bits, those below 2^-31 vanish.  l and O

@@ -102,9 +102,8 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
 // the compiler's eyes (what the warp keeps in uniform registers stays there).  Each
 // poll looks at the abort word.  The limit is a count: a poll that fails has slept in
 // hardware for 4.0 us, so kWaitPolls are 2.1 s (mfi_selftest_waits measures it); it
-// starts anew while a warp has announced longer work (cta_busy).  With
-// the clock read in the block a prompt's attention takes 1.74 ms instead of 1.72, with
-// mbar_wait 1.89.
+// starts anew while a warp has announced longer work (cta_busy).  With the clock read
+// in the block a prompt's attention took 1% more time, with mbar_wait 9%.
 constexpr uint32_t kWaitPolls = 1u << 19;
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, int* err, int code) {
   uint32_t ok;
