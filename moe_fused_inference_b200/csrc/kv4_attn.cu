@@ -783,9 +783,10 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
     }
 
     // ---- join the warps: sums of l over the quad's lanes, then through shared memory
-    float unit[nb];  // 2^(top_b - 127 - 15 + 10)
+    // the weights' 2^10 goes as well: values near the end of fp32 have no room for it
+    float unit[nb];  // 2^(top_b - 127 - 15)
 #pragma unroll
-    for (int b = 0; b < nb; ++b) unit[b] = __uint_as_float((half_of(w.top[b % 2], b / 2) - 5) << 23);
+    for (int b = 0; b < nb; ++b) unit[b] = __uint_as_float((half_of(w.top[b % 2], b / 2) - 15) << 23);
 #pragma unroll
     for (int j = 0; j < kNT; ++j)
 #pragma unroll
@@ -799,7 +800,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
           *reinterpret_cast<float4*>(dst + 32 * b + 4 * gid) =
               make_float4(w.o[j][2 * b][i] * unit[b], w.o[j][2 * b][i + 2] * unit[b],
                           w.o[j][2 * b + 1][i] * unit[b], w.o[j][2 * b + 1][i + 2] * unit[b]);
-        if (gid == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(w.m[j][i], w.l[j][i]);
+        if (gid == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(w.m[j][i], w.l[j][i] * 0x1p-10f);
       }
     if (lane == 0) s_sums[warp] = sums;
     __syncthreads();

@@ -718,9 +718,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
         }
         if (lane == 0) tc::cta_busy(-1);
       };
-      // a part leaves [D + 2][256 vectors] sums
+      // a part leaves [D + 2][256 vectors]: its own outputs (a sum of values near the end
+      // of fp32 has no room for the weights), their maximum and sum of weights
       float* sums = a.part + size_t(it.index) * (256 * (D + 2)) + i * kRows + r;
-      const float inv = it.parts > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
@@ -768,10 +769,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           }
 #pragma unroll
           for (int k = 0; k < kMaxParts; ++k) {
-            w[k] = ex2(w[k] - (top == -INFINITY ? 0.0f : top));
-            if (k < it.parts) sum = fmaf(w[k], at(k, D + 1), sum);
+            w[k] = k < it.parts ? ex2(w[k] - (top == -INFINITY ? 0.0f : top)) * at(k, D + 1) : 0.0f;
+            sum += w[k];
           }
           const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+          for (int k = 0; k < kMaxParts; ++k) w[k] *= scale;
           redo = v < nv && out_of_range(top);
 #pragma unroll 1
           for (int c = 0; c < D; c += 8) {
@@ -785,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
             if (v < nv && !redo) {
               __align__(16) E y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] = E(x[e] * scale);
+              for (int e = 0; e < 8; ++e) y[e] = E(x[e]);
               *reinterpret_cast<uint4*>(out + c) = *reinterpret_cast<const uint4*>(y);
             }
           }

@@ -291,3 +291,16 @@ def test_rows_do_not_depend_on_tokens_after_theirs(rows, back, what, D):
     got = _call(q, cache, table, [L], [rows])
     _compare_blocks(got, q, cache, table, L)
     assert got.isfinite().all() and _errors() == 0
+
+
+@pytest.mark.parametrize("L,rows", [(1, 1), (7, 3), (40, 40), (3000, 1), (3000, 30)])
+def test_values_near_the_end_of_fp32(L, rows):
+    """Values of up to 2^126: the weights' factor has no room beside them."""
+    H, G, D = 1, 8, 128
+    k, v = _randn(21, 2, L, H, D)
+    cache, table = _cache(0.1 * k, v.clamp(-2, 2) * 2.0 ** 125)
+    q = _randn(22, rows, H * G, D).bfloat16() * (1.0 if L < 3000 else 40.0)   # few tokens count
+    got = _call(q, cache, table, [L], [rows])
+    assert got.isfinite().all()
+    _compare_blocks(got, q, cache, table, L)
+    assert _errors() == 0
