@@ -344,7 +344,9 @@ __device__ __forceinline__ void attend_tiles(Running<D, kNT>& w, const Query<D, 
     // the reference moves only when it is passed by more than 1 (p <= 2)
     const bool up0 = t0 > w.m[j][0] + 1.0f, up1 = t1 > w.m[j][1] + 1.0f;
     if (__any_sync(0xffffffffu, up0 || up1)) {
-      const float m0 = up0 ? t0 : w.m[j][0], m1 = up1 ? t1 : w.m[j][1];
+      // (sums of scores out of range are none: asked for once more)
+      const float m0 = up0 ? (out_of_range(w.m[j][0]) ? INFINITY : t0) : w.m[j][0];
+      const float m1 = up1 ? (out_of_range(w.m[j][1]) ? INFINITY : t1) : w.m[j][1];
       const float c0 = up0 ? ex2(w.m[j][0] - m0) : 1.0f, c1 = up1 ? ex2(w.m[j][1] - m1) : 1.0f;
       w.m[j][0] = m0;
       w.m[j][1] = m1;
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(Few<D, kNT, kPerSm>::kThreads, kPerSm) kv4_att
         float l = 0.0f, o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < F::kWarps; ++i) {
-          if (i < busy) {
+          if (i < busy && !out_of_range(ml[i].x)) {  // such sums are none: of no weight, or the vector is taken once more
             const float c = ex2(ml[i].x - ref);
             const float4 x = *reinterpret_cast<const float4*>(src[i] + d0);
             l = fmaf(c, ml[i].y, l);

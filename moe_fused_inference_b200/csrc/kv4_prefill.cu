@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       const int pos = it.step0 * kTok;
       const int lim = v < nv ? it.len - it.rows + v / G + 1 - pos : 0;
       const int all = it.len - it.rows + (it.v0 + i * kRows) / G + 1 - pos;
-      float m = -INFINITY, l = 0.0f, most = 0.0f;
+      float m = -INFINITY, l = 0.0f, most = 0.0f, far = 0.0f;
       for (int j = 0; j < it.steps; ++j, ++step) {
         const uint32_t buf = step & 1u, tb = ts + buf * 64;
         ok = wait(&bar.s_full[i][buf], step >> 1, 3);
@@ -664,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
           }
         }
         const float b0 = kShift - (m == -INFINITY ? 0.0f : m);
+        far = fmaxf(far, fabsf(b0));
         const float2 sc2 = make_float2(sc, sc), b2 = make_float2(b0, b0);
         float2 sum0 = make_float2(0.f, 0.f), sum1 = make_float2(0.f, 0.f);
 #pragma unroll
@@ -707,7 +708,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_attn_many_kernel(AttnArgs a) 
       // step are so strong that what others lose in fp16 would count (rare: S, of which
       // an operand below its range takes 2^-3 at most, is scaled by sc): once more, by
       // the warp.
-      bool redo = v < nv && (s_far[n & 1u] != 0 || out_of_range(m) || most > 0x1p-12f);
+      bool redo = v < nv && (s_far[n & 1u] != 0 || out_of_range(far) || most > 0x1p-12f);
       auto again = [&] {
         unsigned left = __ballot_sync(0xffffffffu, redo);
         if (left == 0) return;

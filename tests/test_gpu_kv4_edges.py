@@ -304,3 +304,35 @@ def test_values_near_the_end_of_fp32(L, rows):
     assert got.isfinite().all()
     _compare_blocks(got, q, cache, table, L)
     assert _errors() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 3, 8, 140])
+@pytest.mark.parametrize("L", [17, 300, 2000])
+@pytest.mark.parametrize("power", [20, 26, 70])
+@pytest.mark.parametrize("first", [True, False])
+def test_hugely_negative_scores_beside_ordinary_ones(rows, L, power, first):
+    """Half of the tokens of a weight of zero, in tiles and parts of their own: the other
+    half's alone count."""
+    H, G, D = 2, 4, 64
+    k, v = _randn(23, 2, L, H, D)
+    q = _randn(24, rows, H * G, D).bfloat16()
+    q[..., 0] = 4.0
+    k[..., 0] = 0.0
+    k[: L // 2 if first else None, :, :32] = 0.0
+    (k[: L // 2] if first else k[1 - L % 2::2])[..., 0] = -2.0 ** power
+    cache, table = _cache(k, v, page=16)
+    got = _call(q, cache, table, [L], [rows])
+    want, _ = ok.attention(_np(q), cache.data.cpu().numpy(), table, [L], [rows])
+    # the scores that count are ordinary: the bound without the others' size
+    held, vals = (_np(x) for x in kv4.kv4_read(cache, torch.arange(L, device="cuda"), dtype=torch.float32))
+    live = held[:, 0, 0] == 0
+    if rows > L:
+        return
+    for r in range(rows):
+        see = np.arange(L) <= L - rows + r
+        if not (live & see).any():
+            continue
+        ds = 2 * D * 2.0 ** -24 * np.abs(held[live]).max() * np.abs(_np(q)[r]).max() * D ** 0.5
+        tol = (2.0 ** -12 + 2 * ds + 2.0 ** -18 + L * 2.0 ** -31) * np.abs(vals).max() + 2.0 ** -8 * np.abs(want[r])
+        assert (np.abs(_np(got[r]) - want[r]) <= tol).all()
+    assert got.isfinite().all() and _errors() == 0
