@@ -37,8 +37,8 @@ using namespace kv4;
 // instructions a tile of 4.25 bits an element, the conversions' pipe first), a call
 // has some 14 us beside it: the launch, three dependent trips (lengths, page table,
 // tiles), the join of the warps and of the CTAs.  4 KV heads of 128, 32 query
-// heads, the cache not in L2: 1 sequence of 131072 tokens 27.9 us, 64 of up to 4096
-// 31.2 us, 1 of 1152 12.1 us, 5 rows over 8191 tokens 14.7 us.  (The figures of the
+// heads, the cache not in L2: 1 sequence of 131072 tokens 27.6 us, 64 of up to 4096
+// 31.6 us, 1 of 1152 11.8 us, 5 rows over 8191 tokens 14.6 us.  (The figures of the
 // constants below are of one call over and over, its cache in L2, without the check of
 // the maximum at the end, which costs up to 2%.)
 //

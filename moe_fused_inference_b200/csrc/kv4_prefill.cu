@@ -17,7 +17,7 @@
 // TMEM: of each tile two S of 64 columns (P in the first half of its S), then O_0
 // and O_1.  Two S a tile keep the softmax supplied while the tensor cores are at
 // the step before; with one S of 128 tokens a tile its warps and the tensor cores
-// waited for each other (16384 rows: 1.98 ms, now 1.66), although a product of 64 columns
+// waited for each other (16384 rows: 1.98 ms, now 1.67), although a product of 64 columns
 // takes 50 clocks and one of 128 takes 65 (both operands from shared memory).
 //
 // The operands are fp16: a query row times a power of two that brings its
